@@ -473,7 +473,6 @@ def _own_prefix(st):
 
 def _own_layout(st):
     c, be = st["case"], _backend()
-    nb = be.batch_layout_workspace_size(c["seqs"])
     _check(be.batch_layout(
         ctx_lens=st["ctx"].data_ptr(), new_lens=st["new"].data_ptr(),
         fork_from=st["fork"].data_ptr(), free_slots=st["free"].data_ptr(),
@@ -483,8 +482,7 @@ def _own_layout(st):
         seq_lens=st["seq_lens"].data_ptr(), cu_seqlens=st["cu"].data_ptr(),
         token_seq=st["token_seq"].data_ptr(), token_pos=st["token_pos"].data_ptr(),
         slot_map=st["slot_map"].data_ptr(), token_capacity=st["cap"],
-        counts=st["counts"].data_ptr(), workspace=_workspace(nb), workspace_bytes=nb,
-        err_word=st["err"].data_ptr(), stream=_stream()))
+        counts=st["counts"].data_ptr(), err_word=st["err"].data_ptr(), stream=_stream()))
     return {k: st[k] for k in ("table", "seq_lens", "cu", "token_seq", "token_pos", "slot_map",
                                "counts", "err")}
 
