@@ -578,6 +578,111 @@ int kllm_gpu_p2p_merge(struct kllm_gpu_ctx *ctx, const float *m, const float *l,
 		       uint32_t *err_word, int timeout_ms, void *stream);
 void kllm_gpu_p2p_destroy(struct kllm_gpu_ctx *ctx);
 
+/* ------------------------------------------------------------------------ */
+/* Parallel sampling with scored answers (no counterpart in the reference):  */
+/* n continuations of one prompt, each token with its log-probability        */
+/* ------------------------------------------------------------------------ */
+
+/* Lays out one scheduler step on the GPU from the requests' lengths: block
+ * tables, slot maps and token positions, as kllm_gpu_kv_append_v2 and
+ * kllm_gpu_prefill_v2 take them. For row s, with cap = max_blocks_per_seq *
+ * block_size:
+ *   ctx = ctx_lens[s] in [0, cap], new = new_lens[s] in [0, cap - ctx] (a
+ *   negative length counts as 0; a length cut at cap is flagged with
+ *   KLLM_ERR_SEQ_TOO_LONG);
+ *   blocks [0, ceil(ctx / block_size)) are kept, blocks up to ceil((ctx + new)
+ *   / block_size) take the next slots of free_slots, rows in order; entries
+ *   past them are left as they are;
+ *   seq_lens[s] = ctx + new, cu_seqlens[s] = sum of new over the rows before;
+ *   token t = cu_seqlens[s] + i: token_seq = s, token_pos = ctx + i,
+ *   slot_map = slot * block_size + token_pos % block_size (-1: no page).
+ * Tokens in [cu_seqlens[num_seqs], token_capacity) are padding: token_seq -1,
+ * token_pos 0, slot_map -1, so that launches of a fixed size can follow.
+ * A row with fork_from[s] = p >= 0 continues row p: its ctx tokens are p's
+ * first ones and its blocks [0, ctx / block_size) become p's entries. ctx must
+ * be a multiple of block_size and at most ctx_lens[p], and p must not fork
+ * itself in the same call; otherwise the row is laid out empty. That, a
+ * free list that runs out, a slot outside [0, total_slots) (both leave a zero
+ * entry) and more tokens than token_capacity are flagged with
+ * KLLM_ERR_LAYOUT. num_seqs <= 4096. */
+#define KLLM_ERR_LAYOUT         0x80u
+
+struct kllm_gpu_batch_layout_params {
+	uint32_t struct_size;
+	uint32_t flags;              /* 0 */
+	const int *ctx_lens;         /* [num_seqs] tokens already cached */
+	const int *new_lens;         /* [num_seqs] tokens this step adds */
+	const int *fork_from;        /* [num_seqs] row to continue, or -1; NULL: none */
+	const int *free_slots;       /* [num_free] free arena slots, taken from the front */
+	int num_free;
+	int num_seqs;
+	int max_blocks_per_seq;
+	int block_size;              /* tokens per block, >= 1 */
+	uint64_t arena_base;         /* device address of slot 0 */
+	uint64_t slot_bytes;
+	uint64_t total_slots;
+	uint64_t k_offset;           /* K page offset inside a slot */
+	uint64_t v_offset;           /* V page offset inside a slot */
+	void *block_tables;          /* in/out: kllm_block_table_entry [num_seqs][max_blocks_per_seq] */
+	int *seq_lens;               /* out: [num_seqs] */
+	int *cu_seqlens;             /* out: [num_seqs + 1] (sums past INT32_MAX are cut there) */
+	int *token_seq;              /* out: [token_capacity] */
+	int *token_pos;              /* out: [token_capacity] */
+	int64_t *slot_map;           /* out, optional: [token_capacity] */
+	int token_capacity;
+	int *counts;                 /* out, optional: [2] tokens, slots of free_slots wanted */
+	uint32_t *err_word;
+	void *stream;
+};
+
+int kllm_gpu_batch_layout(struct kllm_gpu_ctx *ctx,
+			  const struct kllm_gpu_batch_layout_params *p);
+
+/* Log-probabilities of given tokens with rank, entropy and top alternatives,
+ * from logits, in one pass over them. Row r, with z = l / T (T =
+ * temperature[r]; NULL or T <= 0: 1):
+ *   lse        ln sum exp(z)
+ *   logprob(t) z[t] - lse
+ *   rank(t)    tokens with a larger logit, or an equal one and a lower index
+ *   entropy    -sum p ln p, p = exp(z - lse)
+ *   top        the top_n largest logits in (value desc, index asc) order,
+ *              with their logprob
+ * A target outside [0, vocab) gives logprob -inf and rank -1 (padding). A row
+ * whose logits are all -inf (a mask that leaves nothing) gives lse and every
+ * logprob -inf, entropy 0. A NaN or +inf logit makes the row's lse, logprobs
+ * and entropy NaN; the top order takes a NaN as -inf, ranks do not count it (a
+ * NaN target has rank -1). Sums are fp32 against the row's maximum. */
+enum kllm_logits_dtype {
+	KLLM_LOGITS_F32 = 0,
+	KLLM_LOGITS_BF16 = 1,
+};
+#define KLLM_MAX_TOP_N   32
+#define KLLM_MAX_TARGETS 8
+
+struct kllm_gpu_logprobs_params {
+	uint32_t struct_size;
+	uint32_t flags;              /* 0 */
+	const void *logits;          /* [num_rows] rows of vocab, row_stride elements apart */
+	int logits_dtype;            /* enum kllm_logits_dtype */
+	int num_rows;
+	int64_t row_stride;          /* >= vocab; 0: vocab */
+	int vocab;
+	int num_targets;             /* 0 .. KLLM_MAX_TARGETS per row */
+	const float *temperature;    /* [num_rows], or NULL */
+	const int *targets;          /* [num_rows][num_targets] */
+	float *target_logprobs;      /* out: [num_rows][num_targets] */
+	int *target_ranks;           /* out, optional: [num_rows][num_targets] */
+	float *entropy;              /* out, optional: [num_rows] */
+	float *lse;                  /* out, optional: [num_rows] */
+	int top_n;                   /* 0 .. KLLM_MAX_TOP_N, <= vocab */
+	int reserved;
+	int *top_ids;                /* out: [num_rows][top_n] */
+	float *top_logprobs;         /* out: [num_rows][top_n] */
+	void *stream;
+};
+
+int kllm_gpu_logprobs(struct kllm_gpu_ctx *ctx, const struct kllm_gpu_logprobs_params *p);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,6 +25,7 @@ extern "C" {
 #define KLLM_ERR_TOPK_RANGE_BIT 0x10u /* a row asked for top-k above 1024 */
 #define KLLM_ERR_NONFINITE_BIT 0x20u /* MX payload 0x7F/0xFF not recomputed */
 #define KLLM_ERR_PAGE_RANGE_BIT 0x40u /* a page outside the registered arenas: skipped */
+#define KLLM_ERR_LAYOUT_BIT 0x80u /* batch layout: bad fork, no free slot, too many tokens */
 
 /* Device memory ranges the caller registered as KV arenas; when count > 0
  * every page a kernel reads or writes must lie inside one of them. */
@@ -208,6 +209,45 @@ struct kllm_lm_head_args {
 };
 int kllm_lm_head_tiles(int vocab);
 int kllm_lm_head_launch(const struct kllm_lm_head_args *a, void *stream);
+
+/* One scheduler step's block tables and slot maps (batch_layout.cu). */
+struct kllm_layout_args {
+	const int *ctx_lens, *new_lens;  /* [num_seqs] */
+	const int *fork_from;     /* [num_seqs] or NULL */
+	const int *free_slots;    /* [num_free] */
+	int num_free, num_seqs;   /* num_seqs <= KLLM_MAX_SEQS_LAUNCH */
+	int max_blocks, block_size;
+	unsigned long long arena_base, slot_bytes, total_slots, k_offset, v_offset;
+	void *table;              /* 24-byte entries [num_seqs][max_blocks] */
+	int *seq_lens;            /* [num_seqs] */
+	int *cu_seqlens;          /* [num_seqs + 1] */
+	int *token_seq, *token_pos;  /* [token_capacity] */
+	long long *slot_map;      /* [token_capacity] or NULL */
+	int token_capacity;
+	int *counts;              /* [2] or NULL */
+	uint32_t *err;
+};
+int kllm_layout_launch(const struct kllm_layout_args *a, int num_sms, void *stream);
+
+/* Log-probabilities from logits (logprobs.cu). */
+#define KLLM_MAX_TOP_N_I   32
+#define KLLM_MAX_TARGETS_I 8
+struct kllm_logprobs_args {
+	const void *logits;
+	int bf16;                 /* 0: fp32 logits */
+	int num_rows, vocab;
+	long long row_stride;     /* elements */
+	const float *temperature; /* [num_rows] or NULL */
+	const int *targets;       /* [num_rows][num_targets] */
+	int num_targets;
+	float *target_lp;         /* [num_rows][num_targets] */
+	int *target_rank;         /* or NULL */
+	float *entropy, *lse;     /* [num_rows] or NULL */
+	int top_n;
+	int *top_ids;             /* [num_rows][top_n] */
+	float *top_lp;
+};
+int kllm_logprobs_launch(const struct kllm_logprobs_args *a, int num_sms, void *stream);
 
 /* Block arrival: one chunk of records already copied to device memory at
  * src_dev; record i (bytes[i] at src_dev + off[i], off 16-byte aligned) goes

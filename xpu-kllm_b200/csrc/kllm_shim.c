@@ -987,6 +987,104 @@ int kllm_gpu_lm_head_sample(struct kllm_gpu_ctx *ctx, const struct kllm_gpu_lm_h
 	return KLLM_OK;
 }
 
+/* ---- parallel sampling with scored answers -------------------------------- */
+
+int kllm_gpu_batch_layout(struct kllm_gpu_ctx *ctx,
+			  const struct kllm_gpu_batch_layout_params *p)
+{
+	if (!p || p->struct_size < sizeof(*p) || p->flags)
+		return fail(ctx, KLLM_EINVAL);
+	if (!ready(ctx))
+		return fail(ctx, KLLM_ENODEV);
+	if (p->num_seqs < 0 || p->num_free < 0 || p->token_capacity < 0 ||
+	    p->max_blocks_per_seq <= 0 || p->block_size <= 0 || p->slot_bytes == 0 ||
+	    (int64_t)p->max_blocks_per_seq * p->block_size > (1ll << 30))
+		return fail(ctx, KLLM_EINVAL);
+	if (p->num_seqs > KLLM_MAX_SEQS_LAUNCH)
+		return fail(ctx, KLLM_ENOSYS);
+	if (!p->cu_seqlens || (p->num_free > 0 && !p->free_slots) ||
+	    (p->token_capacity > 0 && (!p->token_seq || !p->token_pos)) ||
+	    (p->num_seqs > 0 && (!p->ctx_lens || !p->new_lens || !p->block_tables || !p->seq_lens)))
+		return fail(ctx, KLLM_EINVAL);
+	if (((uintptr_t)p->block_tables | (uintptr_t)p->slot_map) & 7u)
+		return fail(ctx, KLLM_EINVAL);
+	struct kllm_layout_args a;
+	memset(&a, 0, sizeof(a));
+	a.ctx_lens = p->ctx_lens;
+	a.new_lens = p->new_lens;
+	a.fork_from = p->fork_from;
+	a.free_slots = p->free_slots;
+	a.num_free = p->num_free;
+	a.num_seqs = p->num_seqs;
+	a.max_blocks = p->max_blocks_per_seq;
+	a.block_size = p->block_size;
+	a.arena_base = p->arena_base;
+	a.slot_bytes = p->slot_bytes;
+	a.total_slots = p->total_slots;
+	a.k_offset = p->k_offset;
+	a.v_offset = p->v_offset;
+	a.table = p->block_tables;
+	a.seq_lens = p->seq_lens;
+	a.cu_seqlens = p->cu_seqlens;
+	a.token_seq = p->token_seq;
+	a.token_pos = p->token_pos;
+	a.slot_map = (long long *)p->slot_map;
+	a.token_capacity = p->token_capacity;
+	a.counts = p->counts;
+	a.err = p->err_word;
+	int rc = kllm_layout_launch(&a, ctx->num_sms, pick_stream(ctx, p->stream));
+	if (rc)
+		return cuda_fail(ctx, rc);
+	ctx->stats.launches++;
+	return KLLM_OK;
+}
+
+int kllm_gpu_logprobs(struct kllm_gpu_ctx *ctx, const struct kllm_gpu_logprobs_params *p)
+{
+	if (!p || p->struct_size < sizeof(*p) || p->flags)
+		return fail(ctx, KLLM_EINVAL);
+	if (!ready(ctx))
+		return fail(ctx, KLLM_ENODEV);
+	if (p->logits_dtype != KLLM_LOGITS_F32 && p->logits_dtype != KLLM_LOGITS_BF16)
+		return fail(ctx, KLLM_ENOSYS);
+	int64_t stride = p->row_stride ? p->row_stride : p->vocab;
+	if (p->num_rows < 0 || p->vocab <= 0 || stride < p->vocab || p->num_targets < 0 ||
+	    p->top_n < 0 || p->top_n > p->vocab)
+		return fail(ctx, KLLM_EINVAL);
+	if (p->num_targets > KLLM_MAX_TARGETS || p->top_n > KLLM_MAX_TOP_N ||
+	    p->vocab > (1 << 28) || p->num_rows > (1 << 28))
+		return fail(ctx, KLLM_ENOSYS);
+	if (p->num_rows == 0)
+		return KLLM_OK;
+	if (!p->logits || (p->num_targets > 0 && (!p->targets || !p->target_logprobs)) ||
+	    (p->top_n > 0 && (!p->top_ids || !p->top_logprobs)))
+		return fail(ctx, KLLM_EINVAL);
+	if ((uintptr_t)p->logits & (p->logits_dtype == KLLM_LOGITS_F32 ? 3u : 1u))
+		return fail(ctx, KLLM_EINVAL);
+	struct kllm_logprobs_args a;
+	memset(&a, 0, sizeof(a));
+	a.logits = p->logits;
+	a.bf16 = p->logits_dtype == KLLM_LOGITS_BF16;
+	a.num_rows = p->num_rows;
+	a.vocab = p->vocab;
+	a.row_stride = stride;
+	a.temperature = p->temperature;
+	a.targets = p->targets;
+	a.num_targets = p->num_targets;
+	a.target_lp = p->target_logprobs;
+	a.target_rank = p->target_ranks;
+	a.entropy = p->entropy;
+	a.lse = p->lse;
+	a.top_n = p->top_n;
+	a.top_ids = p->top_ids;
+	a.top_lp = p->top_logprobs;
+	int rc = kllm_logprobs_launch(&a, ctx->num_sms, pick_stream(ctx, p->stream));
+	if (rc)
+		return cuda_fail(ctx, rc);
+	ctx->stats.launches++;
+	return KLLM_OK;
+}
+
 int kllm_gpu_merge_partials(struct kllm_gpu_ctx *ctx, const float *m,
 			    const float *l, const float *o, int num_parts,
 			    int num_rows, int head_dim, void *out, void *stream)

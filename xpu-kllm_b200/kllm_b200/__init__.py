@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import (POINTER, Structure, c_float, c_int, c_uint8, c_uint32,
+from ctypes import (POINTER, Structure, c_float, c_int, c_int64, c_uint8, c_uint32,
                     c_uint64, c_void_p)
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -26,7 +26,7 @@ KV_BF16, KV_MX_FP8, KV_MX_BF16_COMPAT = 0, 1, 2
 # error codes
 OK, EIO, ENOMEM, ENODEV, EINVAL, ENOSPC, ENOSYS, ETIMEDOUT = 0, -5, -12, -19, -22, -28, -38, -110
 ERR_SEQ_TOO_LONG, ERR_MISALIGNED, ERR_APPEND_NOPAGE, ERR_TIMEOUT = 0x1, 0x2, 0x4, 0x8
-ERR_TOPK_RANGE, ERR_NONFINITE, ERR_PAGE_RANGE = 0x10, 0x20, 0x40
+ERR_TOPK_RANGE, ERR_NONFINITE, ERR_PAGE_RANGE, ERR_LAYOUT = 0x10, 0x20, 0x40, 0x80
 TRACE_DECODE, TRACE_APPEND, TRACE_PREFILL = 1, 2, 3
 
 
@@ -109,6 +109,31 @@ class LmHeadParams(Structure):
 SAMPLE_GREEDY, SAMPLE_TOP_K, SAMPLE_TOP_P, SAMPLE_TEMPERATURE = 0, 1, 2, 3
 
 
+class BatchLayoutParams(Structure):
+    _fields_ = [("struct_size", c_uint32), ("flags", c_uint32), ("ctx_lens", c_void_p),
+                ("new_lens", c_void_p), ("fork_from", c_void_p), ("free_slots", c_void_p),
+                ("num_free", c_int), ("num_seqs", c_int), ("max_blocks_per_seq", c_int),
+                ("block_size", c_int), ("arena_base", c_uint64), ("slot_bytes", c_uint64),
+                ("total_slots", c_uint64), ("k_offset", c_uint64), ("v_offset", c_uint64),
+                ("block_tables", c_void_p), ("seq_lens", c_void_p), ("cu_seqlens", c_void_p),
+                ("token_seq", c_void_p), ("token_pos", c_void_p), ("slot_map", c_void_p),
+                ("token_capacity", c_int), ("counts", c_void_p), ("err_word", c_void_p),
+                ("stream", c_void_p)]
+
+
+LOGITS_F32, LOGITS_BF16 = 0, 1      # enum kllm_logits_dtype
+MAX_TOP_N, MAX_TARGETS = 32, 8
+
+
+class LogprobsParams(Structure):
+    _fields_ = [("struct_size", c_uint32), ("flags", c_uint32), ("logits", c_void_p),
+                ("logits_dtype", c_int), ("num_rows", c_int), ("row_stride", c_int64),
+                ("vocab", c_int), ("num_targets", c_int), ("temperature", c_void_p),
+                ("targets", c_void_p), ("target_logprobs", c_void_p), ("target_ranks", c_void_p),
+                ("entropy", c_void_p), ("lse", c_void_p), ("top_n", c_int), ("reserved", c_int),
+                ("top_ids", c_void_p), ("top_logprobs", c_void_p), ("stream", c_void_p)]
+
+
 class WfBlockDesc(Structure):
     """userspace/gpu/nvme_ep_wavefront.h:32-39"""
     _fields_ = [("obj_key", c_uint8 * 32), ("vram_dest_addr", c_uint64), ("block_size", c_uint32),
@@ -159,6 +184,8 @@ _SIGNATURES = [
     ("kllm_gpu_build_block_tables", c_int, [c_void_p, POINTER(TableBuildParams)]),
     ("kllm_gpu_lm_head_workspace_size", c_uint64, [c_int, c_int]),
     ("kllm_gpu_lm_head_sample", c_int, [c_void_p, POINTER(LmHeadParams)]),
+    ("kllm_gpu_batch_layout", c_int, [c_void_p, POINTER(BatchLayoutParams)]),
+    ("kllm_gpu_logprobs", c_int, [c_void_p, POINTER(LogprobsParams)]),
     ("kllm_gpu_merge_partials", c_int,
      [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     ("kllm_gpu_memcpy_d2h", c_int, [c_void_p, c_void_p, c_void_p, c_uint64]),
@@ -312,6 +339,14 @@ class Backend:
         for k, v in kw.items():
             setattr(p, k, v)
         return self.lib.kllm_gpu_lm_head_sample(self.ctx, ctypes.byref(p))
+
+    def batch_layout(self, **kw) -> int:
+        p = BatchLayoutParams(struct_size=ctypes.sizeof(BatchLayoutParams), **kw)
+        return self.lib.kllm_gpu_batch_layout(self.ctx, ctypes.byref(p))
+
+    def logprobs(self, **kw) -> int:
+        p = LogprobsParams(struct_size=ctypes.sizeof(LogprobsParams), **kw)
+        return self.lib.kllm_gpu_logprobs(self.ctx, ctypes.byref(p))
 
     def merge(self, m, l, o, num_parts, num_rows, head_dim, out, stream=None) -> int:
         return self.lib.kllm_gpu_merge_partials(self.ctx, m, l, o, num_parts, num_rows,
