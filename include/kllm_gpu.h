@@ -683,6 +683,43 @@ struct kllm_gpu_logprobs_params {
 
 int kllm_gpu_logprobs(struct kllm_gpu_ctx *ctx, const struct kllm_gpu_logprobs_params *p);
 
+/* Scores of given tokens straight from hidden states: the numbers of
+ * kllm_gpu_logprobs for the logits l[r][v] = sum_k hidden[r][k] *
+ * weight[v][k] (bf16 in, fp32 sums on the tensor cores), which are never
+ * stored, so that a whole prompt can be scored in one call. Ranks are not
+ * given. Rules as kllm_gpu_logprobs, with one difference: a row with fewer
+ * than top_n logits above -inf fills up with id -1 and logprob -inf.
+ * hidden_dim % 64 == 0; hidden, weight and workspace 16-byte aligned. The
+ * workspace (kllm_gpu_score_workspace_size bytes) needs no set-up and holds
+ * nothing between calls. */
+struct kllm_gpu_score_params {
+	uint32_t struct_size;
+	uint32_t flags;              /* 0 */
+	const void *hidden;          /* bf16 [num_rows][hidden_dim] */
+	const void *weight;          /* bf16 [vocab][hidden_dim] */
+	int num_rows;
+	int hidden_dim;
+	int vocab;
+	int num_targets;             /* 0 .. KLLM_MAX_TARGETS per row */
+	const float *temperature;    /* [num_rows], or NULL */
+	const int *targets;          /* [num_rows][num_targets] */
+	float *target_logprobs;      /* out: [num_rows][num_targets] */
+	float *entropy;              /* out, optional: [num_rows] */
+	float *lse;                  /* out, optional: [num_rows] */
+	int top_n;                   /* 0 .. KLLM_MAX_TOP_N, <= vocab */
+	int reserved;
+	int *top_ids;                /* out: [num_rows][top_n] */
+	float *top_logprobs;         /* out: [num_rows][top_n] */
+	void *workspace;
+	uint64_t workspace_bytes;
+	uint32_t *err_word;
+	void *stream;
+};
+
+uint64_t kllm_gpu_score_workspace_size(struct kllm_gpu_ctx *ctx, int num_rows, int vocab,
+				       int num_targets, int top_n);
+int kllm_gpu_score_tokens(struct kllm_gpu_ctx *ctx, const struct kllm_gpu_score_params *p);
+
 #ifdef __cplusplus
 }
 #endif

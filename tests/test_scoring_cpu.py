@@ -16,6 +16,7 @@ import kllm_b200 as kb
 STRUCTS = {
     "kllm_gpu_batch_layout_params": kb.BatchLayoutParams,
     "kllm_gpu_logprobs_params": kb.LogprobsParams,
+    "kllm_gpu_score_params": kb.ScoreParams,
 }
 
 
@@ -55,8 +56,11 @@ def test_no_device_is_refused():
     be = kb.Backend()
     assert be.batch_layout() == kb.ENODEV
     assert be.logprobs() == kb.ENODEV
+    assert be.score_tokens() == kb.ENODEV
+    assert be.score_workspace_size(4, 1000, 1, 5) == 0
     assert be.batch_layout(flags=1) == kb.EINVAL
     assert be.logprobs(flags=1) == kb.EINVAL
+    assert be.score_tokens(flags=1) == kb.EINVAL
     be.close()
 
 

@@ -249,6 +249,32 @@ struct kllm_logprobs_args {
 };
 int kllm_logprobs_launch(const struct kllm_logprobs_args *a, int num_sms, void *stream);
 
+/* Token scores from hidden states (score.cu). */
+struct kllm_score_args {
+	const void *hidden;       /* bf16 [num_rows][hidden_dim] */
+	const void *weight;       /* bf16 [vocab][hidden_dim] */
+	int num_rows, hidden_dim, vocab;
+	const float *temperature; /* [num_rows] or NULL */
+	const int *targets;       /* [num_rows][num_targets] */
+	int num_targets;
+	float *target_lp;         /* [num_rows][num_targets] */
+	float *entropy, *lse;     /* [num_rows] or NULL */
+	int top_n;
+	int *top_ids;             /* [num_rows][top_n] */
+	float *top_lp;
+	uint32_t *err;
+	/* set by kllm_score_plan: row blocks, of which group_rb run side by
+	 * side, each over `splits` ranges of the vocabulary's 64-column units */
+	int row_blocks, group_rb, splits, units;
+	/* set by kllm_score_launch: per range and row, the (m, S, W, threshold)
+	 * quadruples, the list entries (value, index) and their number */
+	void *part, *part_list;
+	int *part_n;
+};
+void kllm_score_plan(int num_rows, int vocab, int num_sms, struct kllm_score_args *a);
+uint64_t kllm_score_workspace(const struct kllm_score_args *a);
+int kllm_score_launch(struct kllm_score_args *a, void *workspace, void *stream);
+
 /* Block arrival: one chunk of records already copied to device memory at
  * src_dev; record i (bytes[i] at src_dev + off[i], off 16-byte aligned) goes
  * to dst[i], a range the host checked lies in device memory of this GPU. */

@@ -1085,6 +1085,66 @@ int kllm_gpu_logprobs(struct kllm_gpu_ctx *ctx, const struct kllm_gpu_logprobs_p
 	return KLLM_OK;
 }
 
+uint64_t kllm_gpu_score_workspace_size(struct kllm_gpu_ctx *ctx, int num_rows, int vocab,
+				       int num_targets, int top_n)
+{
+	if (!ctx || ctx->backend != KLLM_GPU_CUDA || num_rows <= 0 || vocab <= 0 ||
+	    num_targets < 0 || top_n < 0 || top_n > KLLM_MAX_TOP_N)
+		return 0;
+	struct kllm_score_args a;
+	memset(&a, 0, sizeof(a));
+	a.top_n = top_n;
+	kllm_score_plan(num_rows, vocab, ctx->num_sms, &a);
+	return kllm_score_workspace(&a);
+}
+
+int kllm_gpu_score_tokens(struct kllm_gpu_ctx *ctx, const struct kllm_gpu_score_params *p)
+{
+	if (!p || p->struct_size < sizeof(*p) || p->flags)
+		return fail(ctx, KLLM_EINVAL);
+	if (!ready(ctx))
+		return fail(ctx, KLLM_ENODEV);
+	if (p->num_rows < 0 || p->hidden_dim <= 0 || p->vocab <= 0 || p->num_targets < 0 ||
+	    p->top_n < 0 || p->top_n > p->vocab)
+		return fail(ctx, KLLM_EINVAL);
+	if (p->num_targets > KLLM_MAX_TARGETS || p->top_n > KLLM_MAX_TOP_N || p->hidden_dim % 64 ||
+	    p->vocab > (1 << 28) || p->num_rows > (1 << 20))
+		return fail(ctx, KLLM_ENOSYS);
+	if (p->num_rows == 0)
+		return KLLM_OK;
+	if (!p->hidden || !p->weight || !p->workspace ||
+	    (p->num_targets > 0 && (!p->targets || !p->target_logprobs)) ||
+	    (p->top_n > 0 && (!p->top_ids || !p->top_logprobs)))
+		return fail(ctx, KLLM_EINVAL);
+	if (((uintptr_t)p->hidden | (uintptr_t)p->weight | (uintptr_t)p->workspace) & 15u)
+		return fail(ctx, KLLM_EINVAL);
+	struct kllm_score_args a;
+	memset(&a, 0, sizeof(a));
+	a.hidden = p->hidden;
+	a.weight = p->weight;
+	a.num_rows = p->num_rows;
+	a.hidden_dim = p->hidden_dim;
+	a.vocab = p->vocab;
+	a.temperature = p->temperature;
+	a.targets = p->targets;
+	a.num_targets = p->num_targets;
+	a.target_lp = p->target_logprobs;
+	a.entropy = p->entropy;
+	a.lse = p->lse;
+	a.top_n = p->top_n;
+	a.top_ids = p->top_ids;
+	a.top_lp = p->top_logprobs;
+	a.err = p->err_word;
+	kllm_score_plan(p->num_rows, p->vocab, ctx->num_sms, &a);
+	if (p->workspace_bytes < kllm_score_workspace(&a))
+		return fail(ctx, KLLM_ENOSPC);
+	int rc = kllm_score_launch(&a, p->workspace, pick_stream(ctx, p->stream));
+	if (rc)
+		return cuda_fail(ctx, rc);
+	ctx->stats.launches += 2;
+	return KLLM_OK;
+}
+
 int kllm_gpu_merge_partials(struct kllm_gpu_ctx *ctx, const float *m,
 			    const float *l, const float *o, int num_parts,
 			    int num_rows, int head_dim, void *out, void *stream)

@@ -27,9 +27,9 @@
 
 #include "kllm_device.cuh"
 #include "kllm_internal.h"
+#include "kllm_topk.cuh"
 
 #include <cooperative_groups.h>
-#include <math_constants.h>
 
 namespace cg = cooperative_groups;
 
@@ -42,7 +42,6 @@ constexpr int kMaxSeg = 1024;         // segments of a row, over the cluster
 constexpr int kCandCap = 1024;        // candidates sorted by counting
 constexpr int kMaxCluster = 8;
 constexpr int kTgtMax = KLLM_MAX_TARGETS_I;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 struct LpSmem {
 	float wm[kLpWarps], ws[kLpWarps], ww[kLpWarps];
@@ -64,22 +63,6 @@ struct LpSmem {
 	int remain, base_gt;
 	int wcnt[2][kLpWarps];
 };
-
-// Joins two (m, S, W) triples; a triple without elements has m = -inf, S = 0.
-__device__ __forceinline__ void join(float &m, float &s, float &w, float m2, float s2, float w2)
-{
-	const float M = fmaxf(m, m2);
-	if (M == -CUDART_INF_F) {     // nothing finite on either side (NaN sums stay NaN)
-		s += s2;
-		w += w2;
-		return;
-	}
-	const float d1 = m == -CUDART_INF_F ? 0.f : M - m, d2 = m2 == -CUDART_INF_F ? 0.f : M - m2;
-	const float f1 = ex2_approx(-d1), f2 = ex2_approx(-d2);
-	w = f1 * fmaf(-d1, s, w) + f2 * fmaf(-d2, s2, w2);
-	s = f1 * s + f2 * s2;
-	m = M;
-}
 
 template <int BF16>
 struct Elem;
@@ -140,33 +123,7 @@ __device__ __forceinline__ float order_val(float l)
 }
 __device__ __forceinline__ uint32_t order_bits(float l)
 {
-	const uint32_t u = __float_as_uint(order_val(l) + 0.f);      // -0 as +0
-	return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
-
-// 32 values, one a lane, sorted descending over the warp (bitonic network).
-__device__ __forceinline__ float bitonic_step(float x, int lane, int stride, bool keep_max)
-{
-	const float o = __shfl_xor_sync(0xffffffffu, x, stride);
-	return keep_max ? fmaxf(x, o) : fminf(x, o);
-}
-__device__ __forceinline__ float warp_sort_desc(float x, int lane)
-{
-#pragma unroll
-	for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-		for (int stride = size >> 1; stride; stride >>= 1)
-			x = bitonic_step(x, lane, stride, ((lane & stride) == 0) == ((lane & size) == 0));
-	return x;
-}
-// The 32 largest of two descending lists, descending.
-__device__ __forceinline__ float warp_merge_desc(float a, float b, int lane)
-{
-	a = fmaxf(a, __shfl_sync(0xffffffffu, b, 31 - lane));
-#pragma unroll
-	for (int stride = 16; stride; stride >>= 1)
-		a = bitonic_step(a, lane, stride, (lane & stride) == 0);
-	return a;
+	return key_of(order_val(l));
 }
 
 __device__ __forceinline__ float warp_max(float x)

@@ -134,6 +134,16 @@ class LogprobsParams(Structure):
                 ("top_ids", c_void_p), ("top_logprobs", c_void_p), ("stream", c_void_p)]
 
 
+class ScoreParams(Structure):
+    _fields_ = [("struct_size", c_uint32), ("flags", c_uint32), ("hidden", c_void_p),
+                ("weight", c_void_p), ("num_rows", c_int), ("hidden_dim", c_int),
+                ("vocab", c_int), ("num_targets", c_int), ("temperature", c_void_p),
+                ("targets", c_void_p), ("target_logprobs", c_void_p), ("entropy", c_void_p),
+                ("lse", c_void_p), ("top_n", c_int), ("reserved", c_int), ("top_ids", c_void_p),
+                ("top_logprobs", c_void_p), ("workspace", c_void_p),
+                ("workspace_bytes", c_uint64), ("err_word", c_void_p), ("stream", c_void_p)]
+
+
 class WfBlockDesc(Structure):
     """userspace/gpu/nvme_ep_wavefront.h:32-39"""
     _fields_ = [("obj_key", c_uint8 * 32), ("vram_dest_addr", c_uint64), ("block_size", c_uint32),
@@ -186,6 +196,8 @@ _SIGNATURES = [
     ("kllm_gpu_lm_head_sample", c_int, [c_void_p, POINTER(LmHeadParams)]),
     ("kllm_gpu_batch_layout", c_int, [c_void_p, POINTER(BatchLayoutParams)]),
     ("kllm_gpu_logprobs", c_int, [c_void_p, POINTER(LogprobsParams)]),
+    ("kllm_gpu_score_workspace_size", c_uint64, [c_void_p, c_int, c_int, c_int, c_int]),
+    ("kllm_gpu_score_tokens", c_int, [c_void_p, POINTER(ScoreParams)]),
     ("kllm_gpu_merge_partials", c_int,
      [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     ("kllm_gpu_memcpy_d2h", c_int, [c_void_p, c_void_p, c_void_p, c_uint64]),
@@ -347,6 +359,14 @@ class Backend:
     def logprobs(self, **kw) -> int:
         p = LogprobsParams(struct_size=ctypes.sizeof(LogprobsParams), **kw)
         return self.lib.kllm_gpu_logprobs(self.ctx, ctypes.byref(p))
+
+    def score_workspace_size(self, num_rows, vocab, num_targets, top_n) -> int:
+        return self.lib.kllm_gpu_score_workspace_size(self.ctx, num_rows, vocab, num_targets,
+                                                      top_n)
+
+    def score_tokens(self, **kw) -> int:
+        p = ScoreParams(struct_size=ctypes.sizeof(ScoreParams), **kw)
+        return self.lib.kllm_gpu_score_tokens(self.ctx, ctypes.byref(p))
 
     def merge(self, m, l, o, num_parts, num_rows, head_dim, out, stream=None) -> int:
         return self.lib.kllm_gpu_merge_partials(self.ctx, m, l, o, num_parts, num_rows,
