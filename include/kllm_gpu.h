@@ -408,6 +408,7 @@ void kllm_gpu_clear_arenas(struct kllm_gpu_ctx *ctx);
 #define KLLM_TRACE_DECODE  1u
 #define KLLM_TRACE_APPEND  2u
 #define KLLM_TRACE_PREFILL 3u
+#define KLLM_TRACE_SHARED  4u   /* kllm_gpu_shared_prefix_attention */
 #define KLLM_TRACE_MAX     65536
 struct kllm_gpu_trace_record {
 	uint64_t seq;                /* call number since tracing was enabled */
@@ -637,6 +638,53 @@ struct kllm_gpu_batch_layout_params {
 
 int kllm_gpu_batch_layout(struct kllm_gpu_ctx *ctx,
 			  const struct kllm_gpu_batch_layout_params *p);
+
+/* Decode attention of a batch whose groups of sequences share their leading
+ * pages: the same result as kllm_gpu_paged_attention_v2, with each group's
+ * shared pages read and multiplied once for all of its sequences (on the
+ * tcgen05 tensor cores) and the rest of each sequence by the split-KV decode.
+ * Group g is the rows group_starts[g] .. group_starts[g + 1] - 1; in each of
+ * its rows that holds prefix_lens[g] tokens, the first prefix_lens[g] /
+ * block_size block-table entries must be the same (as sequences forked by
+ * kllm_gpu_batch_layout or found by kllm_gpu_build_block_tables have them).
+ * Tokens of the prefix past its last whole block count as the rows' own, a
+ * shorter row is attended on its own, and rows outside every group are too.
+ * Groups that are out of order or out of range are flagged with
+ * KLLM_ERR_LAYOUT and nothing is shared. Shapes, page rules, page formats and
+ * error bits as kllm_gpu_paged_attention_v2. The workspace
+ * (kllm_gpu_shared_prefix_workspace_size bytes, 16-byte aligned) needs no
+ * set-up and holds nothing between calls. */
+struct kllm_gpu_shared_prefix_params {
+	uint32_t struct_size;
+	uint32_t flags;              /* 0 */
+	void *output;                /* bf16 [num_seqs][num_heads][head_dim] */
+	const void *query;           /* bf16 [num_seqs][num_heads][head_dim] */
+	const void *block_tables;    /* kllm_block_table_entry [num_seqs][max_blocks_per_seq] */
+	const int *seq_lens;         /* [num_seqs]: tokens of context (<= 0: empty) */
+	const int *group_starts;     /* [num_groups + 1], ascending, in [0, num_seqs] */
+	const int *prefix_lens;      /* [num_groups] tokens shared */
+	int num_seqs;
+	int num_groups;              /* 0 .. num_seqs */
+	int num_heads;
+	int num_kv_heads;            /* num_heads % num_kv_heads == 0, ratio <= 8 */
+	int head_dim;                /* 64 or 128 */
+	int max_blocks_per_seq;
+	int block_size;              /* 16 .. 128, a multiple of 16 */
+	int kv_dtype;                /* KLLM_KV_BF16 or KLLM_KV_MX_FP8_E4M3 */
+	int layer;
+	float scale;
+	uint64_t layer_stride;       /* multiple of 16 */
+	void *workspace;
+	uint64_t workspace_bytes;
+	uint32_t *err_word;
+	void *stream;
+};
+
+uint64_t kllm_gpu_shared_prefix_workspace_size(struct kllm_gpu_ctx *ctx, int num_seqs,
+					       int num_heads, int num_kv_heads, int head_dim,
+					       int max_blocks_per_seq);
+int kllm_gpu_shared_prefix_attention(struct kllm_gpu_ctx *ctx,
+				     const struct kllm_gpu_shared_prefix_params *p);
 
 /* Log-probabilities of given tokens with rank, entropy and top alternatives,
  * from logits, in one pass over them. Row r, with z = l / T (T =

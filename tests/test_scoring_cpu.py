@@ -17,6 +17,7 @@ STRUCTS = {
     "kllm_gpu_batch_layout_params": kb.BatchLayoutParams,
     "kllm_gpu_logprobs_params": kb.LogprobsParams,
     "kllm_gpu_score_params": kb.ScoreParams,
+    "kllm_gpu_shared_prefix_params": kb.SharedPrefixParams,
 }
 
 
@@ -57,6 +58,8 @@ def test_no_device_is_refused():
     assert be.batch_layout() == kb.ENODEV
     assert be.logprobs() == kb.ENODEV
     assert be.score_tokens() == kb.ENODEV
+    assert be.shared_prefix() == kb.ENODEV and be.shared_prefix(flags=1) == kb.EINVAL
+    assert be.shared_prefix_workspace_size(2, 32, 8, 128, 4) == 0
     assert be.score_workspace_size(4, 1000, 1, 5) == 0
     assert be.batch_layout(flags=1) == kb.EINVAL
     assert be.logprobs(flags=1) == kb.EINVAL

@@ -249,6 +249,38 @@ struct kllm_logprobs_args {
 };
 int kllm_logprobs_launch(const struct kllm_logprobs_args *a, int num_sms, void *stream);
 
+/* Decode attention of groups that share their leading pages
+ * (shared_prefix.cu). */
+struct kllm_prefix_args {
+	void *out;                /* bf16 [num_seqs][num_heads][head_dim] */
+	const void *q;            /* bf16, same shape */
+	const void *table;        /* 24-byte entries [num_seqs][max_blocks] */
+	const int *seq_lens;      /* [num_seqs] */
+	const int *group_starts;  /* [num_groups + 1] */
+	const int *prefix_lens;   /* [num_groups] */
+	int num_seqs, num_groups;
+	int num_heads, num_kv_heads, group, head_dim;
+	int max_blocks, block_size, kv_dtype;
+	int min_share;            /* sequences a group needs for its prefix to be shared */
+	int ctas;                 /* CTAs of the prefix kernel */
+	uint64_t layer_off;
+	float scale_log2;         /* softmax scale * log2(e) */
+	uint32_t *err;
+	struct kllm_arenas arenas;
+	/* set by kllm_prefix_workspace: the plan, each row's group, the suffixes'
+	 * lengths, tables and triples, the prefix pieces' partials */
+	void *header, *groups;
+	int *row_group, *suf_lens;
+	void *suf_table;
+	float *sm, *sl, *so;
+	float *pm, *pl, *po;
+};
+/* Bytes of the workspace; with `a`, sets its pointers into `base` too. */
+uint64_t kllm_prefix_workspace(int num_seqs, int num_heads, int head_dim, int max_blocks,
+			       int ctas, void *base, struct kllm_prefix_args *a);
+int kllm_prefix_launch(const struct kllm_prefix_args *a, void *stream);
+int kllm_prefix_join_launch(const struct kllm_prefix_args *a, void *stream);
+
 /* Token scores from hidden states (score.cu). */
 struct kllm_score_args {
 	const void *hidden;       /* bf16 [num_rows][hidden_dim] */

@@ -1039,6 +1039,105 @@ int kllm_gpu_batch_layout(struct kllm_gpu_ctx *ctx,
 	return KLLM_OK;
 }
 
+/* A group of fewer sequences is attended row by row. */
+#define KLLM_SHARED_MIN_SEQS 2
+
+uint64_t kllm_gpu_shared_prefix_workspace_size(struct kllm_gpu_ctx *ctx, int num_seqs,
+					       int num_heads, int num_kv_heads, int head_dim,
+					       int max_blocks_per_seq)
+{
+	if (!ctx || ctx->backend != KLLM_GPU_CUDA || num_seqs <= 0 || num_heads <= 0 ||
+	    num_kv_heads <= 0 || head_dim <= 0 || max_blocks_per_seq <= 0)
+		return 0;
+	return kllm_prefix_workspace(num_seqs, num_heads, head_dim, max_blocks_per_seq,
+				     ctx->num_sms, NULL, NULL);
+}
+
+int kllm_gpu_shared_prefix_attention(struct kllm_gpu_ctx *ctx,
+				     const struct kllm_gpu_shared_prefix_params *p)
+{
+	if (!p || p->struct_size < sizeof(*p) || p->flags)
+		return fail(ctx, KLLM_EINVAL);
+	if (!ready(ctx))
+		return fail(ctx, KLLM_ENODEV);
+	int rc = check_decode_shape(p->num_seqs, p->num_heads, p->num_kv_heads, p->head_dim,
+				    p->max_blocks_per_seq, p->block_size, p->kv_dtype);
+	if (rc)
+		return fail(ctx, rc);
+	if (p->num_groups < 0 || p->num_groups > p->num_seqs)
+		return fail(ctx, KLLM_EINVAL);
+	if (p->num_seqs == 0)
+		return KLLM_OK;
+	if (!p->output || !p->query || !p->block_tables || !p->seq_lens || !p->workspace ||
+	    (p->num_groups > 0 && (!p->group_starts || !p->prefix_lens)))
+		return fail(ctx, KLLM_EINVAL);
+	if ((p->layer_stride & 15u) || p->layer < 0 || ((uintptr_t)p->block_tables & 7u) ||
+	    (((uintptr_t)p->query | (uintptr_t)p->output | (uintptr_t)p->workspace) & 15u))
+		return fail(ctx, KLLM_EINVAL);
+	if (p->workspace_bytes <
+	    kllm_prefix_workspace(p->num_seqs, p->num_heads, p->head_dim, p->max_blocks_per_seq,
+				  ctx->num_sms, NULL, NULL))
+		return fail(ctx, KLLM_ENOSPC);
+	const uint64_t layer_off = (uint64_t)p->layer * p->layer_stride;
+	struct kllm_prefix_args a;
+	memset(&a, 0, sizeof(a));
+	a.out = p->output;
+	a.q = p->query;
+	a.table = p->block_tables;
+	a.seq_lens = p->seq_lens;
+	a.group_starts = p->group_starts;
+	a.prefix_lens = p->prefix_lens;
+	a.num_seqs = p->num_seqs;
+	a.num_groups = p->num_groups;
+	a.num_heads = p->num_heads;
+	a.num_kv_heads = p->num_kv_heads;
+	a.group = p->num_heads / p->num_kv_heads;
+	a.head_dim = p->head_dim;
+	a.max_blocks = p->max_blocks_per_seq;
+	a.block_size = p->block_size;
+	a.kv_dtype = p->kv_dtype;
+	a.min_share = KLLM_SHARED_MIN_SEQS;
+	a.ctas = ctx->num_sms;
+	a.layer_off = layer_off;
+	a.scale_log2 = p->scale * 1.4426950408889634f;
+	a.err = p->err_word;
+	a.arenas = ctx->arenas;
+	kllm_prefix_workspace(p->num_seqs, p->num_heads, p->head_dim, p->max_blocks_per_seq,
+			      ctx->num_sms, p->workspace, &a);
+	/* the suffixes: an ordinary split-KV decode into triples. Its set-up reads
+	 * the suffix lengths and tables, which the plan kernel wrote before the
+	 * prefix kernel let it start (KLLM_DECODE_OVERLAP_PREV's condition) */
+	struct kllm_decode_args d;
+	fill_args(&d, NULL, p->query, a.suf_table, a.suf_lens, p->num_seqs, p->num_heads,
+		  p->num_kv_heads, p->head_dim, p->max_blocks_per_seq, p->block_size, p->kv_dtype,
+		  layer_off, p->scale);
+	d.pm = a.sm;
+	d.pl = a.sl;
+	d.po = a.so;
+	d.err = p->err_word;
+	d.overlap = 1;
+	d.arenas = ctx->arenas;
+	cudaStream_t st = pick_stream(ctx, p->stream);
+	int tr = trace_begin(ctx, st, KLLM_TRACE_SHARED);
+	rc = kllm_prefix_launch(&a, st);
+	if (!rc) {
+		ctx->stats.launches += 2;
+		rc = decode_common(ctx, &d, 1, ctx->ws_part, ctx->ws_part_bytes, ctx->ws_cnt,
+				   KLLM_CNT_CAP, ctx->num_sms, st);
+		if (rc) {
+			trace_end(ctx, st, tr);
+			return rc == KLLM_EIO ? cuda_fail(ctx, cudaErrorLaunchFailure)
+					      : fail(ctx, rc);
+		}
+		rc = kllm_prefix_join_launch(&a, st);
+		ctx->stats.launches++;
+	}
+	trace_end(ctx, st, tr);
+	if (rc)
+		return cuda_fail(ctx, rc);
+	return KLLM_OK;
+}
+
 int kllm_gpu_logprobs(struct kllm_gpu_ctx *ctx, const struct kllm_gpu_logprobs_params *p)
 {
 	if (!p || p->struct_size < sizeof(*p) || p->flags)

@@ -27,7 +27,7 @@ KV_BF16, KV_MX_FP8, KV_MX_BF16_COMPAT = 0, 1, 2
 OK, EIO, ENOMEM, ENODEV, EINVAL, ENOSPC, ENOSYS, ETIMEDOUT = 0, -5, -12, -19, -22, -28, -38, -110
 ERR_SEQ_TOO_LONG, ERR_MISALIGNED, ERR_APPEND_NOPAGE, ERR_TIMEOUT = 0x1, 0x2, 0x4, 0x8
 ERR_TOPK_RANGE, ERR_NONFINITE, ERR_PAGE_RANGE, ERR_LAYOUT = 0x10, 0x20, 0x40, 0x80
-TRACE_DECODE, TRACE_APPEND, TRACE_PREFILL = 1, 2, 3
+TRACE_DECODE, TRACE_APPEND, TRACE_PREFILL, TRACE_SHARED = 1, 2, 3, 4
 
 
 class TraceRecord(Structure):
@@ -121,6 +121,17 @@ class BatchLayoutParams(Structure):
                 ("stream", c_void_p)]
 
 
+class SharedPrefixParams(Structure):
+    _fields_ = [("struct_size", c_uint32), ("flags", c_uint32), ("output", c_void_p),
+                ("query", c_void_p), ("block_tables", c_void_p), ("seq_lens", c_void_p),
+                ("group_starts", c_void_p), ("prefix_lens", c_void_p), ("num_seqs", c_int),
+                ("num_groups", c_int), ("num_heads", c_int), ("num_kv_heads", c_int),
+                ("head_dim", c_int), ("max_blocks_per_seq", c_int), ("block_size", c_int),
+                ("kv_dtype", c_int), ("layer", c_int), ("scale", c_float),
+                ("layer_stride", c_uint64), ("workspace", c_void_p),
+                ("workspace_bytes", c_uint64), ("err_word", c_void_p), ("stream", c_void_p)]
+
+
 LOGITS_F32, LOGITS_BF16 = 0, 1      # enum kllm_logits_dtype
 MAX_TOP_N, MAX_TARGETS = 32, 8
 
@@ -195,6 +206,9 @@ _SIGNATURES = [
     ("kllm_gpu_lm_head_workspace_size", c_uint64, [c_int, c_int]),
     ("kllm_gpu_lm_head_sample", c_int, [c_void_p, POINTER(LmHeadParams)]),
     ("kllm_gpu_batch_layout", c_int, [c_void_p, POINTER(BatchLayoutParams)]),
+    ("kllm_gpu_shared_prefix_workspace_size", c_uint64,
+     [c_void_p, c_int, c_int, c_int, c_int, c_int]),
+    ("kllm_gpu_shared_prefix_attention", c_int, [c_void_p, POINTER(SharedPrefixParams)]),
     ("kllm_gpu_logprobs", c_int, [c_void_p, POINTER(LogprobsParams)]),
     ("kllm_gpu_score_workspace_size", c_uint64, [c_void_p, c_int, c_int, c_int, c_int]),
     ("kllm_gpu_score_tokens", c_int, [c_void_p, POINTER(ScoreParams)]),
@@ -355,6 +369,15 @@ class Backend:
     def batch_layout(self, **kw) -> int:
         p = BatchLayoutParams(struct_size=ctypes.sizeof(BatchLayoutParams), **kw)
         return self.lib.kllm_gpu_batch_layout(self.ctx, ctypes.byref(p))
+
+    def shared_prefix_workspace_size(self, num_seqs, num_heads, num_kv_heads, head_dim,
+                                     max_blocks_per_seq) -> int:
+        return self.lib.kllm_gpu_shared_prefix_workspace_size(
+            self.ctx, num_seqs, num_heads, num_kv_heads, head_dim, max_blocks_per_seq)
+
+    def shared_prefix(self, **kw) -> int:
+        p = SharedPrefixParams(struct_size=ctypes.sizeof(SharedPrefixParams), **kw)
+        return self.lib.kllm_gpu_shared_prefix_attention(self.ctx, ctypes.byref(p))
 
     def logprobs(self, **kw) -> int:
         p = LogprobsParams(struct_size=ctypes.sizeof(LogprobsParams), **kw)
