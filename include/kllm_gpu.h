@@ -664,7 +664,7 @@ struct kllm_gpu_shared_prefix_params {
 	const int *group_starts;     /* [num_groups + 1], ascending, in [0, num_seqs] */
 	const int *prefix_lens;      /* [num_groups] tokens shared */
 	int num_seqs;
-	int num_groups;              /* 0 .. num_seqs */
+	int num_groups;              /* 0 .. num_seqs, at most 4096 */
 	int num_heads;
 	int num_kv_heads;            /* num_heads % num_kv_heads == 0, ratio <= 8 */
 	int head_dim;                /* 64 or 128 */

@@ -267,19 +267,19 @@ struct kllm_prefix_args {
 	float scale_log2;         /* softmax scale * log2(e) */
 	uint32_t *err;
 	struct kllm_arenas arenas;
-	/* set by kllm_prefix_workspace: the plan, each row's group, the suffixes'
-	 * lengths, tables and triples, the prefix pieces' partials */
+	int suf_warps;            /* warps of a suffix CTA, set by kllm_prefix_launch */
+	/* set by kllm_prefix_workspace: the plan, each row's group and suffix
+	 * (first block, tokens, exclusive sums of 16-token tiles), the partials of
+	 * the suffixes' and the prefixes' pieces */
 	void *header, *groups;
-	int *row_group, *suf_lens;
-	void *suf_table;
-	float *sm, *sl, *so;
+	int *row_group, *suf_start, *suf_lens, *tile_pre;
+	float *xm, *xl, *xo;
 	float *pm, *pl, *po;
 };
 /* Bytes of the workspace; with `a`, sets its pointers into `base` too. */
-uint64_t kllm_prefix_workspace(int num_seqs, int num_heads, int head_dim, int max_blocks,
+uint64_t kllm_prefix_workspace(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
 			       int ctas, void *base, struct kllm_prefix_args *a);
-int kllm_prefix_launch(const struct kllm_prefix_args *a, void *stream);
-int kllm_prefix_join_launch(const struct kllm_prefix_args *a, void *stream);
+int kllm_prefix_launch(struct kllm_prefix_args *a, void *stream);
 
 /* Token scores from hidden states (score.cu). */
 struct kllm_score_args {

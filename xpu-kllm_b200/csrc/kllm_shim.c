@@ -1047,10 +1047,11 @@ uint64_t kllm_gpu_shared_prefix_workspace_size(struct kllm_gpu_ctx *ctx, int num
 					       int max_blocks_per_seq)
 {
 	if (!ctx || ctx->backend != KLLM_GPU_CUDA || num_seqs <= 0 || num_heads <= 0 ||
-	    num_kv_heads <= 0 || head_dim <= 0 || max_blocks_per_seq <= 0)
+	    num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
+	    max_blocks_per_seq <= 0)
 		return 0;
-	return kllm_prefix_workspace(num_seqs, num_heads, head_dim, max_blocks_per_seq,
-				     ctx->num_sms, NULL, NULL);
+	return kllm_prefix_workspace(num_seqs, num_heads, num_kv_heads, head_dim, ctx->num_sms,
+				     NULL, NULL);
 }
 
 int kllm_gpu_shared_prefix_attention(struct kllm_gpu_ctx *ctx,
@@ -1074,11 +1075,12 @@ int kllm_gpu_shared_prefix_attention(struct kllm_gpu_ctx *ctx,
 	if ((p->layer_stride & 15u) || p->layer < 0 || ((uintptr_t)p->block_tables & 7u) ||
 	    (((uintptr_t)p->query | (uintptr_t)p->output | (uintptr_t)p->workspace) & 15u))
 		return fail(ctx, KLLM_EINVAL);
+	if (p->num_groups > KLLM_MAX_SEQS_LAUNCH)
+		return fail(ctx, KLLM_ENOSYS);
 	if (p->workspace_bytes <
-	    kllm_prefix_workspace(p->num_seqs, p->num_heads, p->head_dim, p->max_blocks_per_seq,
+	    kllm_prefix_workspace(p->num_seqs, p->num_heads, p->num_kv_heads, p->head_dim,
 				  ctx->num_sms, NULL, NULL))
 		return fail(ctx, KLLM_ENOSPC);
-	const uint64_t layer_off = (uint64_t)p->layer * p->layer_stride;
 	struct kllm_prefix_args a;
 	memset(&a, 0, sizeof(a));
 	a.out = p->output;
@@ -1098,43 +1100,19 @@ int kllm_gpu_shared_prefix_attention(struct kllm_gpu_ctx *ctx,
 	a.kv_dtype = p->kv_dtype;
 	a.min_share = KLLM_SHARED_MIN_SEQS;
 	a.ctas = ctx->num_sms;
-	a.layer_off = layer_off;
+	a.layer_off = (uint64_t)p->layer * p->layer_stride;
 	a.scale_log2 = p->scale * 1.4426950408889634f;
 	a.err = p->err_word;
 	a.arenas = ctx->arenas;
-	kllm_prefix_workspace(p->num_seqs, p->num_heads, p->head_dim, p->max_blocks_per_seq,
+	kllm_prefix_workspace(p->num_seqs, p->num_heads, p->num_kv_heads, p->head_dim,
 			      ctx->num_sms, p->workspace, &a);
-	/* the suffixes: an ordinary split-KV decode into triples. Its set-up reads
-	 * the suffix lengths and tables, which the plan kernel wrote before the
-	 * prefix kernel let it start (KLLM_DECODE_OVERLAP_PREV's condition) */
-	struct kllm_decode_args d;
-	fill_args(&d, NULL, p->query, a.suf_table, a.suf_lens, p->num_seqs, p->num_heads,
-		  p->num_kv_heads, p->head_dim, p->max_blocks_per_seq, p->block_size, p->kv_dtype,
-		  layer_off, p->scale);
-	d.pm = a.sm;
-	d.pl = a.sl;
-	d.po = a.so;
-	d.err = p->err_word;
-	d.overlap = 1;
-	d.arenas = ctx->arenas;
 	cudaStream_t st = pick_stream(ctx, p->stream);
 	int tr = trace_begin(ctx, st, KLLM_TRACE_SHARED);
 	rc = kllm_prefix_launch(&a, st);
-	if (!rc) {
-		ctx->stats.launches += 2;
-		rc = decode_common(ctx, &d, 1, ctx->ws_part, ctx->ws_part_bytes, ctx->ws_cnt,
-				   KLLM_CNT_CAP, ctx->num_sms, st);
-		if (rc) {
-			trace_end(ctx, st, tr);
-			return rc == KLLM_EIO ? cuda_fail(ctx, cudaErrorLaunchFailure)
-					      : fail(ctx, rc);
-		}
-		rc = kllm_prefix_join_launch(&a, st);
-		ctx->stats.launches++;
-	}
 	trace_end(ctx, st, tr);
 	if (rc)
 		return cuda_fail(ctx, rc);
+	ctx->stats.launches += 3;
 	return KLLM_OK;
 }
 

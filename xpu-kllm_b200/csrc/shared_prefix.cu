@@ -10,36 +10,44 @@
 // group's prefix of P tokens (whole pages) and the row's own suffix:
 //   o = (sum_prefix 2^(x_i - M) v_i + sum_suffix 2^(x_i - M) v_i) / (same sums of 1)
 // with x = scale log2(e) q.k, so (max, sum, o) triples of the two parts, and of
-// any pieces of the prefix, join exactly. Four steps per call:
+// any pieces of either, join exactly. Three launches per call:
 //
-// plan_kernel     per row: its group, suffix length and suffix block table; per
-//                 group: the row whose table names the prefix pages, the work.
-// prefix_kernel   the prefix. All rows of a group that use one kv head (G
-//                 query heads x its sequences) are the M dimension of the
-//                 products: S = Q K^T and O += P V on tcgen05, 128 keys at a
-//                 time. Below.
-// decode kernels  the suffixes, by the split-KV decode over the suffix tables.
+// plan_kernel     per row: its group and suffix; per group: the row whose table
+//                 names the prefix pages, the work; how many CTAs take which part.
+// attend_kernel   one CTA per SM. The first ones take the prefixes
+//                 (prefix_role, bound by the tensor core and the exponential),
+//                 the others the suffixes (suffix_role, bound by HBM), so that
+//                 the two run at the same time instead of one after the other.
 // join_kernel     both parts' triples -> the output rows.
 //
-// prefix_kernel. A unit is (group, kv head, up to 256 rows). Its key blocks are
-// laid end to end over all units, and each of one CTA per SM takes an equal
+// prefix_role. All rows of a group that use one kv head (G query heads x its
+// sequences) are the M dimension of the products: S = Q K^T and O += P V on
+// tcgen05, 128 keys at a time. A unit is (group, kv head, up to 256 rows). Its
+// key blocks are laid end to end over all units, and each CTA takes an equal
 // contiguous share (pieces leave fp32 partials). A unit of more than 128 rows
 // runs as two query tiles that share every K/V block; a smaller one as two
 // streams of one query tile that take alternate blocks, so that in both shapes
 // one stream's products run under the other's softmax. Warps:
-//   0-3 / 4-7  softmax of stream 0 / 1 (one row a thread)
-//   8-11       producers: queries, then K and V blocks into the swizzled
-//              operand layout (MX: dequantised to f16 from staged raw pages;
-//              BF16: copied by cp.async)
-//   12         TMEM allocation and MMA issue
-//   13         page lookup and bulk copies of raw pages (three stages)
+//   0-3 / 4-7  one row a thread: queries into the operand tile, softmax of
+//              stream 0 / 1, the piece's partial
+//   8-15       producers: K and V blocks into the swizzled operand layout (MX:
+//              dequantised to f16 from staged raw pages; BF16: copied by
+//              cp.async)
+//   16         TMEM allocation and MMA issue
+//   17         page lookup and bulk copies of raw pages (three stages)
 // MX computes in f16 like the decode: K and V are payload x scale / 4, the
 // query row times a power of two; P is one f16 (11 bits; its 2^-12 stays under
 // the output's 2^-9) built 2^7 larger, so that what underflows is below 2^-32
 // of the row's largest. BF16 pages keep P as bf16 hi + lo: one bf16 P would add
 // as much error as the output's own rounding.
+//
+// suffix_role. The decode's tiles (16 tokens of one sequence and kv head, all G
+// query heads, m16n8k16) laid end to end; each warp takes an equal contiguous
+// range, as the split-KV decode does, but leaves every piece as a partial for
+// the join, which reads them anyway: no counters, no last-arriver merge.
 // Every wait is bounded in wall time; a timeout sets KLLM_ERR_TIMEOUT.
 
+#include "kllm_decode_tile.cuh"
 #include "kllm_device.cuh"
 #include "kllm_internal.h"
 #include "kllm_umma.cuh"
@@ -51,13 +59,17 @@ namespace {
 
 constexpr int kPRows = 128, kPKeys = 128;
 constexpr int kUnitRows = 256;
-constexpr int kPThreads = 14 * 32;
-constexpr int kWarpProd = 8, kWarpMma = 12;
+constexpr int kPThreads = 20 * 32;
+constexpr int kWarpProd = 8, kWarpMma = 16, kWarpLoad = 17;
+constexpr int kProd = 256;                    // producer threads
+// Registers: 640 threads launch with 96 each, and the CTA hands them to the
+// warps that need them: a softmax thread holds 64 scores (256 x 112 + 384 x 80
+// of 640 x 96), a suffix warp its tile's fragments (MX: 384 x 144 + 256 x 24;
+// BF16: 256 x 184 + 384 x 32).
 constexpr int kRaw = 3;                       // raw stages (MX) / page-address stages (BF16)
 constexpr float kRaise = 8.f;                 // slack of the lazy reference maximum, log2
 constexpr float kPShift = 7.f;                // f16 P is built 2^7 larger
 constexpr uint64_t kPWaitNs = 200000000ull;
-constexpr float kPLog2e = 1.4426950408889634f;
 
 struct PGroup {
 	long long x0;         // first work step of the group's units
@@ -71,21 +83,27 @@ struct PGroup {
 	int alloc;            // partial rows per kv head
 };
 struct PHeader {
-	long long T;          // work steps of the call
-	int W;                // CTAs that share them
-	int pad[13];
+	long long T;          // work steps of the prefixes
+	long long N;          // suffix tiles, kv heads counted
+	int W;                // CTAs that share the steps
+	int n_prefix;         // CTAs set aside for them; the rest take suffixes
+	int WS;               // warps that share the tiles
+	int pad[9];
 };
 static_assert(sizeof(PHeader) == 64 && sizeof(PGroup) == 48, "workspace layout");
 
-struct DevEntry {
-	unsigned long long k, v;
-	int valid;
-	int pad;
-};
-
 // ---- plan ------------------------------------------------------------------------
 
-constexpr int kPlanThreads = 256;
+constexpr int kPlanThreads = 1024;
+// A CTA's time for n steps or for n tiles a warp, in ns, as measured on the
+// whole chip: set-up, then the rate. They only balance the two parts.
+constexpr float kStepSetNs = 7000.f, kStepNs = 1400.f, kTileSetNs = 4500.f, kTileNs = 1200.f;
+
+struct PlanSmem {
+	long long w0[32], w1[32];
+	int leader[KLLM_MAX_SEQS_LAUNCH];
+	unsigned long long best;
+};
 
 // Tokens of group g's prefix that are whole pages inside the table.
 __device__ __forceinline__ int prefix_tokens(const kllm_prefix_args &a, int g)
@@ -94,149 +112,165 @@ __device__ __forceinline__ int prefix_tokens(const kllm_prefix_args &a, int g)
 	return min(max(a.prefix_lens[g], 0), cap) / a.block_size * a.block_size;
 }
 
-__device__ __forceinline__ int row_length(const kllm_prefix_args &a, int s, bool &too_long)
+// Exclusive sums of x and y over the block's threads, on top of run_x, run_y,
+// which advance by the totals.
+__device__ __forceinline__ void block_scan2(PlanSmem &sm, long long x, long long y, long long &ex,
+					    long long &ey, long long &run_x, long long &run_y)
 {
-	const int cap = a.max_blocks * a.block_size, L = a.seq_lens[s];
-	too_long |= L > cap;
-	return min(max(L, 0), cap);
+	const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+	long long ix = x, iy = y;
+#pragma unroll
+	for (int o = 1; o < 32; o <<= 1) {
+		const long long nx = __shfl_up_sync(0xffffffffu, ix, o);
+		const long long ny = __shfl_up_sync(0xffffffffu, iy, o);
+		if (lane >= o) {
+			ix += nx;
+			iy += ny;
+		}
+	}
+	__syncthreads();
+	if (lane == 31) {
+		sm.w0[warp] = ix;
+		sm.w1[warp] = iy;
+	}
+	__syncthreads();
+	long long bx = lane < kPlanThreads / 32 ? sm.w0[lane] : 0, by = lane < kPlanThreads / 32 ? sm.w1[lane] : 0;
+#pragma unroll
+	for (int o = 1; o < 32; o <<= 1) {
+		const long long nx = __shfl_up_sync(0xffffffffu, bx, o);
+		const long long ny = __shfl_up_sync(0xffffffffu, by, o);
+		if (lane >= o) {
+			bx += nx;
+			by += ny;
+		}
+	}
+	const long long px = __shfl_sync(0xffffffffu, bx, max(warp - 1, 0));
+	const long long py = __shfl_sync(0xffffffffu, by, max(warp - 1, 0));
+	ex = run_x + (warp ? px : 0) + ix - x;
+	ey = run_y + (warp ? py : 0) + iy - y;
+	run_x += __shfl_sync(0xffffffffu, bx, 31);
+	run_y += __shfl_sync(0xffffffffu, by, 31);
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
 plan_kernel(const kllm_prefix_args a)
 {
-	__shared__ int leader[kPlanThreads];
-	__shared__ long long sx[kPlanThreads / 32], sr[kPlanThreads / 32];
-	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-	const int S = a.num_seqs, NG = a.num_groups;
+	__shared__ PlanSmem sm;
+	const int tid = threadIdx.x;
+	const int S = a.num_seqs, NG = a.num_groups, bs = a.block_size;
 	grid_launch_dependents();
+	// groups out of order or out of range: nothing is shared (the result stays
+	// right) and the call is flagged
 	bool bad = false, too_long = false;
 	for (int g = tid; g < NG; g += kPlanThreads) {
 		const int b = a.group_starts[g], e = a.group_starts[g + 1];
 		bad |= b < 0 || e < b || e > S;
+		sm.leader[g] = 0x7fffffff;
 	}
-	// groups out of order or out of range: nothing is shared (the result stays
-	// right) and the call is flagged
 	bad = __syncthreads_or(bad);
 
-	if (blockIdx.x == 0) {
-		PHeader *hd = static_cast<PHeader *>(a.header);
-		PGroup *gr = static_cast<PGroup *>(a.groups);
-		long long run_x = 0, run_r = 0;
-		for (int base = 0; base < NG; base += kPlanThreads) {
-			// the first row of each group that holds the whole prefix
-			for (int i = warp; i < kPlanThreads && base + i < NG; i += kPlanThreads / 32) {
-				const int g = base + i, b = a.group_starts[g], e = a.group_starts[g + 1];
-				int who = -1;
-				if (!bad && e - b >= a.min_share) {
-					const int P = prefix_tokens(a, g);
-					for (int s0 = b; P > 0 && s0 < e && who < 0; s0 += 32) {
-						const unsigned m = __ballot_sync(
-						    0xffffffffu, s0 + lane < e && a.seq_lens[min(s0 + lane, e - 1)] >= P);
-						if (m)
-							who = s0 + __ffs(m) - 1;
+	// ---- rows: group, suffix, exclusive sums of the suffixes' tiles --------------
+	const int cap = a.max_blocks * bs;
+	long long tiles = 0, none = 0;
+	for (int base = 0; base < S; base += kPlanThreads) {
+		const int s = base + tid;
+		int n_tiles = 0;
+		if (s < S) {
+			const int len = a.seq_lens[s], L = min(max(len, 0), cap);
+			too_long |= len > cap;
+			int g = -1, P = 0;
+			if (!bad && NG > 0) {
+				int lo = 0, hi = NG - 1;        // the last group that starts at or before s
+				while (lo < hi) {
+					const int mid = (lo + hi + 1) >> 1;
+					if (a.group_starts[mid] <= s)
+						lo = mid;
+					else
+						hi = mid - 1;
+				}
+				const int b = a.group_starts[lo], e = a.group_starts[lo + 1];
+				if (b <= s && s < e && e - b >= a.min_share) {
+					P = prefix_tokens(a, lo);
+					if (P > 0 && L >= P) {
+						g = lo;
+						atomicMin(&sm.leader[lo], s);
+					} else {
+						P = 0;          // too short a row: all of it is suffix
 					}
 				}
-				if (lane == 0)
-					leader[i] = who;
 			}
-			__syncthreads();
-			const int g = base + tid;
-			PGroup p = {};
-			long long x = 0, r = 0;
-			if (g < NG) {
-				p.row0 = a.group_starts[g];
-				p.nseq = bad ? 0 : a.group_starts[g + 1] - p.row0;
-				p.leader = leader[tid];
-				const int rows = p.nseq * a.group;
-				p.tiles = (rows + kUnitRows - 1) / kUnitRows;
-				p.wgt = rows > kPRows ? 2 : 1;
-				p.alloc = rows > kPRows ? rows : 2 * rows;
-				if (p.leader >= 0) {
-					p.npages = prefix_tokens(a, g) / a.block_size;
-					const int ppb = kPKeys / a.block_size;
-					p.nblk = (p.npages + ppb - 1) / ppb;
-					x = (long long)a.num_kv_heads * p.tiles * p.nblk * p.wgt;
-					r = (long long)a.num_kv_heads * p.alloc;
-				}
-			}
-			// exclusive sums of x and r over the groups
-			long long ix = x, ir = r;
-#pragma unroll
-			for (int o = 1; o < 32; o <<= 1) {
-				const long long nx = __shfl_up_sync(0xffffffffu, ix, o);
-				const long long nr = __shfl_up_sync(0xffffffffu, ir, o);
-				if (lane >= o) {
-					ix += nx;
-					ir += nr;
-				}
-			}
-			if (lane == 31) {
-				sx[warp] = ix;
-				sr[warp] = ir;
-			}
-			__syncthreads();
-			long long bx = run_x, br = run_r;
-			for (int w = 0; w < kPlanThreads / 32; ++w) {
-				if (w < warp) {
-					bx += sx[w];
-					br += sr[w];
-				}
-				run_x += sx[w];
-				run_r += sr[w];
-			}
-			if (g < NG) {
-				p.x0 = bx + ix - x;
-				p.r0 = br + ir - r;
-				gr[g] = p;
-			}
-			__syncthreads();
-		}
-		if (tid == 0) {
-			hd->T = run_x;
-			hd->W = (int)(run_x < a.ctas ? run_x : a.ctas);
-			if (bad && a.err)
-				atomicOr(a.err, KLLM_ERR_LAYOUT_BIT);
-		}
-		return;
-	}
-
-	// one warp per row
-	for (int s = (blockIdx.x - 1) * (kPlanThreads / 32) + warp; s < S;
-	     s += (gridDim.x - 1) * (kPlanThreads / 32)) {
-		const int L = row_length(a, s, too_long);
-		int g = -1, P = 0;
-		if (!bad && NG > 0) {
-			int lo = 0, hi = NG - 1;            // the last group that starts at or before s
-			while (lo < hi) {
-				const int mid = (lo + hi + 1) >> 1;
-				if (a.group_starts[mid] <= s)
-					lo = mid;
-				else
-					hi = mid - 1;
-			}
-			const int b = a.group_starts[lo], e = a.group_starts[lo + 1];
-			if (b <= s && s < e && e - b >= a.min_share) {
-				P = prefix_tokens(a, lo);
-				if (P > 0 && L >= P)
-					g = lo;
-				else
-					P = 0;                  // too short a row: all of it is suffix
-			}
-		}
-		const int j0 = P / a.block_size;
-		const int n = (L - P + a.block_size - 1) / a.block_size;
-		if (lane == 0) {
+			n_tiles = (L - P + kTile - 1) / kTile;
 			a.row_group[s] = g;
+			a.suf_start[s] = P / bs;
 			a.suf_lens[s] = L - P;
 		}
-		const unsigned long long *src = reinterpret_cast<const unsigned long long *>(
-		    static_cast<const DevEntry *>(a.table) + (size_t)s * a.max_blocks + j0);
-		unsigned long long *dst = reinterpret_cast<unsigned long long *>(
-		    static_cast<DevEntry *>(a.suf_table) + (size_t)s * a.max_blocks);
-		for (int w = lane; w < 3 * n; w += 32)
-			dst[w] = src[w];
+		long long et, en;
+		block_scan2(sm, n_tiles, 0, et, en, tiles, none);
+		if (s < S)
+			a.tile_pre[s] = (int)et;
 	}
-	if (too_long && lane == 0 && a.err)
+	__syncthreads();                           // sm.leader is complete
+
+	// ---- groups: exclusive sums of steps and partial rows ---------------------------
+	PGroup *gr = static_cast<PGroup *>(a.groups);
+	long long run_x = 0, run_r = 0;
+	for (int base = 0; base < NG; base += kPlanThreads) {
+		const int g = base + tid;
+		PGroup p = {};
+		long long x = 0, r = 0;
+		if (g < NG) {
+			p.row0 = a.group_starts[g];
+			p.nseq = bad ? 0 : a.group_starts[g + 1] - p.row0;
+			p.leader = sm.leader[g];
+			const int rows = p.nseq * a.group;
+			p.tiles = (rows + kUnitRows - 1) / kUnitRows;
+			p.wgt = rows > kPRows ? 2 : 1;
+			p.alloc = rows > kPRows ? rows : 2 * rows;
+			if (p.leader != 0x7fffffff) {
+				p.npages = prefix_tokens(a, g) / bs;
+				const int ppb = kPKeys / bs;
+				p.nblk = (p.npages + ppb - 1) / ppb;
+				x = (long long)a.num_kv_heads * p.tiles * p.nblk * p.wgt;
+				r = (long long)a.num_kv_heads * p.alloc;
+			}
+		}
+		block_scan2(sm, x, r, p.x0, p.r0, run_x, run_r);
+		if (g < NG)
+			gr[g] = p;
+	}
+
+	// ---- CTAs for each part: the split whose slower part is fastest -----------------
+	const long long T = run_x, N = tiles * a.num_kv_heads;
+	if (tid == 0)
+		sm.best = ~0ull;
+	__syncthreads();
+	if (tid <= a.ctas) {
+		const int n = tid;                         // CTAs for the prefixes
+		const bool possible = (T > 0) == (n > 0) && (N == 0 || n < a.ctas);
+		if (possible) {
+			float t = 0.f;
+			if (n > 0)
+				t = kStepSetNs + kStepNs * ceilf((float)T / (float)n);
+			if (N > 0)
+				t = fmaxf(t, kTileSetNs + kTileNs * ceilf((float)N / (float)((a.ctas - n) * a.suf_warps)));
+			atomicMin(&sm.best, ((unsigned long long)__float_as_uint(t) << 32) | (unsigned)n);
+		}
+	}
+	__syncthreads();
+	if (tid == 0) {
+		PHeader *hd = static_cast<PHeader *>(a.header);
+		const int n = (int)(sm.best & 0xffffffffull);
+		const long long ws = (long long)(a.ctas - n) * a.suf_warps;
+		hd->T = T;
+		hd->N = N;
+		hd->n_prefix = n;
+		hd->W = (int)(T < n ? T : n);
+		hd->WS = (int)(N < ws ? N : ws);
+		a.tile_pre[S] = (int)tiles;
+		if (bad && a.err)
+			atomicOr(a.err, KLLM_ERR_LAYOUT_BIT);
+	}
+	if (too_long && a.err)
 		atomicOr(a.err, KLLM_ERR_SEQ_TOO_LONG_BIT);
 }
 
@@ -249,8 +283,9 @@ struct PG {
 	static constexpr int HALF = kPRows * 128;             // bytes of one half tile
 	static constexpr int TILE = NH * HALF;
 	static constexpr int KB = MX ? 1 : 2;                 // K operand buffers
-	static constexpr int RAW = MX ? kPKeys * D * 9 / 8 : 16;
-	static constexpr int LPR = D / 8;                     // producer lanes per row
+	static constexpr int RAW = MX ? kPKeys * D : 16;      // payload of a block
+	static constexpr int RAWS = MX ? kPKeys * D / 8 : 16; // its scales
+	static constexpr int LPR = D / 8;                     // 16-byte chunks of a bf16 row
 };
 
 template <int D, int KVT>
@@ -259,8 +294,9 @@ struct PrefixSmem {
 	uint8_t q[2][G::TILE];
 	uint8_t k[G::KB][G::TILE];
 	uint8_t v[2][G::TILE];
-	uint8_t raw[kRaw][G::RAW];
-	float qf[2][2][kPRows];               // 2^-e of each query row (MX), by piece parity
+	uint8_t raw[kRaw][G::RAW];            // [128 keys][D] payload
+	uint8_t raws[kRaw][G::RAWS];          // [128 keys][D / 8] scales
+	float qf[2][kPRows];                  // 2^-e of a solo piece's query rows, by piece parity
 	unsigned long long pg[kRaw][2][8];    // page addresses of a block (BF16)
 	uint32_t slot_ok[kRaw];               // pages present, one bit each
 	uint32_t key_ok[4][4];                // key masks of the last four blocks
@@ -316,6 +352,13 @@ __device__ __forceinline__ int group_of_step(const PGroup *gr, int ng, long long
 	return lo;
 }
 
+// a / b, in 32 bits where the values allow (a 64-bit division costs several
+// times as much, and the pieces are found before the first load)
+__device__ __forceinline__ long long div_steps(long long x, long long y)
+{
+	return (unsigned long long)(x | y) >> 32 ? x / y : (long long)((uint32_t)x / (uint32_t)y);
+}
+
 // The piece that starts at step x < xe; advances x to its end.
 __device__ __forceinline__ Piece next_piece(const kllm_prefix_args &a, long long &x, long long xe,
 					    int cta)
@@ -325,13 +368,13 @@ __device__ __forceinline__ Piece next_piece(const kllm_prefix_args &a, long long
 	p.g = group_of_step(gr, a.num_groups, x);
 	const PGroup G = gr[p.g];
 	const long long cost = (long long)G.nblk * G.wgt;
-	const long long u = (x - G.x0) / cost;
+	const long long u = div_steps(x - G.x0, cost);
 	const long long ux = G.x0 + u * cost;
 	const long long end = min(xe, ux + cost);
-	p.h = (int)(u / G.tiles);
+	p.h = (int)div_steps(u, G.tiles);
 	p.tile = (int)(u - (long long)p.h * G.tiles);
-	p.b0 = (int)((x - ux) / G.wgt);
-	p.nb = (int)((end - ux) / G.wgt) - p.b0;
+	p.b0 = (int)((x - ux) >> (G.wgt - 1));
+	p.nb = (int)((end - ux) >> (G.wgt - 1)) - p.b0;
 	const int all = G.nseq * a.group;
 	p.rows = min(kUnitRows, all - p.tile * kUnitRows);
 	p.solo = G.wgt == 1;
@@ -357,63 +400,79 @@ __device__ __forceinline__ uint32_t swz(int row, int chunk16)
 	return (uint32_t)row * 128u + (uint32_t)((chunk16 ^ (row & 7)) << 4);
 }
 
-// Two words (8 codes) of an MX block and its scale -> 8 f16 values payload x
-// scale / 4. The hardware conversion reads codes 0x7F / 0xFF as NaN; the
-// format's decoder reads them as +-480 (userspace/compute/mx_dequant.h:30-55),
-// so a word that holds one is converted by placing the bits: s.eeee.mmm as
-// s.0eeee.mmm0000000 is the value x 2^-8 for every code.
-__device__ __forceinline__ uint4 mx8_to_f16(uint2 w, uint32_t sc)
+// Two E4M3 codes in bytes 0 and 2 -> f16x2 of value x 2^-8: the bits s.eeee.mmm
+// placed as s.0eeee.mmm0000000, exact for every code (subnormals land on f16
+// subnormals, 0x7F / 0xFF give +-480 as the format's decoder has it,
+// userspace/compute/mx_dequant.h:30-55). Shifted by 7 the sign sits in bit 14;
+// adding that bit moves it to bit 15. Integer instructions, because the hardware
+// conversion shares its unit with the softmax's exponentials.
+__device__ __forceinline__ uint32_t place_pair(uint32_t x)
 {
-	const uint32_t bits = ((sc & 0x80u) << 8) | ((sc & 0x7Fu) << 7);
-	const uint32_t s = f16x2_mul(bits | (bits << 16), 0x54005400u);     // x 64: scale / 4
-	uint4 o;
-	o.x = e4m3x2_lo_to_f16x2(w.x);
-	o.y = e4m3x2_hi_to_f16x2(w.x);
-	o.z = e4m3x2_lo_to_f16x2(w.y);
-	o.w = e4m3x2_hi_to_f16x2(w.y);
-	const uint32_t t0 = (w.x & 0x7F7F7F7Fu) + 0x01010101u, t1 = (w.y & 0x7F7F7F7Fu) + 0x01010101u;
-	if ((t0 | t1) & 0x80808080u) {
-		const uint32_t ww[2] = {w.x, w.y};
-		uint32_t r[4];
-#pragma unroll
-		for (int i = 0; i < 4; ++i) {
-			const uint32_t x = __byte_perm(ww[i >> 1], 0u, (i & 1) ? 0x4342u : 0x4140u);
-			const uint32_t p = ((x & 0x007F007Fu) << 7) | ((x & 0x00800080u) << 8);
-			r[i] = f16x2_mul(p, 0x5C005C00u);                           // x 2^8: exact
-		}
-		o = make_uint4(r[0], r[1], r[2], r[3]);
-	}
-	o.x = f16x2_mul(o.x, s);
-	o.y = f16x2_mul(o.y, s);
-	o.z = f16x2_mul(o.z, s);
-	o.w = f16x2_mul(o.w, s);
-	return o;
+	const uint32_t h = x << 7;
+	return h + (h & 0x40004000u);
 }
 
-// One raw block (pages of bs tokens: payload rows, then scale rows) -> the
-// operand tile [128 keys][D] f16, 128-byte swizzle. Absent pages give zeros.
-template <int D>
-__device__ __forceinline__ void dequant_block(uint8_t *dst, const uint8_t *raw, uint32_t ok, int bs,
-					      int pt)
+// Sixteen codes (two scale blocks) of a row -> 16 f16 values payload x scale /
+// 4, the second block's eight in `hi`: the scale is placed and multiplied by
+// 2^14, which makes it x 64, and x 64 x 2^-8 is / 4.
+__device__ __forceinline__ void mx16_to_f16(uint2 wl, uint2 wh, uint32_t scl, uint32_t sch, uint4 &lo,
+					    uint4 &hi)
 {
-	constexpr int LPR = D / 8, RPP = 128 / LPR;      // rows per pass of 128 threads
-	const int l = pt % LPR, sec = bs * D * 9 / 8;
-	int row = pt / LPR, page = 0, tok = row;         // row < 16 <= bs
-	uint8_t *out = dst + (l >> 3) * (kPRows * 128);
-#pragma unroll 4
-	for (int i = 0; i < kPKeys / RPP; ++i) {
-		uint4 o = make_uint4(0u, 0u, 0u, 0u);
-		if ((ok >> page) & 1u) {
-			const uint8_t *p = raw + page * sec;
-			const uint2 w = *reinterpret_cast<const uint2 *>(p + tok * D + l * 8);
-			o = mx8_to_f16(w, p[bs * D + tok * LPR + l]);
+	const uint32_t s = f16x2_mul(place_pair(scl | (sch << 16)), 0x74007400u);
+	const uint32_t s0 = __byte_perm(s, 0u, 0x1010u), s1 = __byte_perm(s, 0u, 0x3232u);
+	lo.x = f16x2_mul(place_pair(__byte_perm(wl.x, 0u, 0x4140u)), s0);
+	lo.y = f16x2_mul(place_pair(__byte_perm(wl.x, 0u, 0x4342u)), s0);
+	lo.z = f16x2_mul(place_pair(__byte_perm(wl.y, 0u, 0x4140u)), s0);
+	lo.w = f16x2_mul(place_pair(__byte_perm(wl.y, 0u, 0x4342u)), s0);
+	hi.x = f16x2_mul(place_pair(__byte_perm(wh.x, 0u, 0x4140u)), s1);
+	hi.y = f16x2_mul(place_pair(__byte_perm(wh.x, 0u, 0x4342u)), s1);
+	hi.z = f16x2_mul(place_pair(__byte_perm(wh.y, 0u, 0x4140u)), s1);
+	hi.w = f16x2_mul(place_pair(__byte_perm(wh.y, 0u, 0x4342u)), s1);
+}
+
+// One raw block -> the operand tile [128 keys][D] f16, 128-byte swizzle, by the
+// producers; rows of absent pages are zeros. A lane takes 16 codes as two
+// 8-byte chunks; lanes of the upper 64 columns take them in the other order, so
+// that the eight lanes of a row never store to one bank. Loads of kFly rows
+// come before their stores: the compiler cannot tell that the tiles do not
+// overlap.
+template <int D>
+__device__ __forceinline__ void dequant_block(uint8_t *dst, const uint8_t *raw, const uint8_t *rs,
+					      const uint32_t *mask, bool full, int pt)
+{
+	constexpr int LPR = D / 16, RPP = kProd / LPR, kFly = kPKeys / RPP;
+	const int l = pt % LPR, row0 = pt / LPR;
+	const int first = l >= 4 ? 1 : 0;
+	const int c0 = (2 * l) & 7;
+	// RPP is a multiple of 8, so the swizzle of a lane's rows is the same
+	uint8_t *o0 = dst + (l >> 2) * (kPRows * 128) + swz(row0, c0 + first);
+	uint8_t *o1 = dst + (l >> 2) * (kPRows * 128) + swz(row0, c0 + 1 - first);
+	const uint8_t *pl = raw + row0 * D + l * 16 + 8 * first, *ph = raw + row0 * D + l * 16 + 8 * (1 - first);
+	const uint8_t *sl = rs + row0 * (D / 8) + l * 2 + first, *sh = rs + row0 * (D / 8) + l * 2 + 1 - first;
+#pragma unroll
+	for (int i0 = 0; i0 < kPKeys / RPP; i0 += kFly) {
+		uint2 wl[kFly], wh[kFly];
+		uint32_t a[kFly], b[kFly];
+#pragma unroll
+		for (int u = 0; u < kFly; ++u) {
+			wl[u] = *reinterpret_cast<const uint2 *>(pl + (i0 + u) * RPP * D);
+			wh[u] = *reinterpret_cast<const uint2 *>(ph + (i0 + u) * RPP * D);
+			a[u] = sl[(i0 + u) * RPP * (D / 8)];
+			b[u] = sh[(i0 + u) * RPP * (D / 8)];
 		}
-		*reinterpret_cast<uint4 *>(out + swz(row, l & 7)) = o;
-		row += RPP;
-		tok += RPP;
-		if (tok >= bs) {
-			tok -= bs;
-			++page;
+		if (!full)
+#pragma unroll
+			for (int u = 0; u < kFly; ++u) {
+				const int row = row0 + (i0 + u) * RPP;
+				if (!((mask[row >> 5] >> (row & 31)) & 1u))
+					wl[u] = wh[u] = make_uint2(0u, 0u);
+			}
+#pragma unroll
+		for (int u = 0; u < kFly; ++u) {
+			uint4 lo, hi;
+			mx16_to_f16(wl[u], wh[u], a[u], b[u], lo, hi);
+			*reinterpret_cast<uint4 *>(o0 + (i0 + u) * RPP * 128) = lo;
+			*reinterpret_cast<uint4 *>(o1 + (i0 + u) * RPP * 128) = hi;
 		}
 	}
 }
@@ -433,42 +492,37 @@ __device__ __forceinline__ void cp_async_wait()
 	asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory");
 }
 
-// Loads two 32-column chunks of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64])
+// 64 scores of this thread's TMEM lane, all loads in flight; keys whose bit in
+// (m0, m1) is clear read as -inf.
+__device__ __forceinline__ void load_scores(uint32_t taddr, bool full, uint32_t m0, uint32_t m1,
+					    uint32_t (&r)[4][16])
 {
-	uint32_t r[64];
 #pragma unroll
 	for (int q = 0; q < 4; ++q)
-		tmem_ld16_nowait(taddr + 16 * q, *reinterpret_cast<uint32_t (*)[16]>(&r[16 * q]));
+		tmem_ld16_nowait(taddr + 16 * q, r[q]);
 #pragma unroll
 	for (int q = 0; q < 4; ++q)
 		asm volatile("tcgen05.wait::ld.sync.aligned;"
-			     : "+r"(r[16 * q]), "+r"(r[16 * q + 1]), "+r"(r[16 * q + 2]),
-			       "+r"(r[16 * q + 3]), "+r"(r[16 * q + 4]), "+r"(r[16 * q + 5]),
-			       "+r"(r[16 * q + 6]), "+r"(r[16 * q + 7]), "+r"(r[16 * q + 8]),
-			       "+r"(r[16 * q + 9]), "+r"(r[16 * q + 10]), "+r"(r[16 * q + 11]),
-			       "+r"(r[16 * q + 12]), "+r"(r[16 * q + 13]), "+r"(r[16 * q + 14]),
-			       "+r"(r[16 * q + 15])
+			     : "+r"(r[q][0]), "+r"(r[q][1]), "+r"(r[q][2]), "+r"(r[q][3]),
+			       "+r"(r[q][4]), "+r"(r[q][5]), "+r"(r[q][6]), "+r"(r[q][7]),
+			       "+r"(r[q][8]), "+r"(r[q][9]), "+r"(r[q][10]), "+r"(r[q][11]),
+			       "+r"(r[q][12]), "+r"(r[q][13]), "+r"(r[q][14]), "+r"(r[q][15])
 			     :: "memory");
+	if (!full)
 #pragma unroll
-	for (int i = 0; i < 64; ++i)
-		v[i] = __uint_as_float(r[i]);
-}
-
-// Masked scores of half `half` of a block: absent keys are -inf.
-__device__ __forceinline__ void mask64(float (&v)[64], uint32_t m0, uint32_t m1)
-{
-#pragma unroll
-	for (int i = 0; i < 64; ++i)
-		if (!(((i < 32 ? m0 : m1) >> (i & 31)) & 1u))
-			v[i] = -CUDART_INF_F;
+		for (int i = 0; i < 64; ++i)
+			if (!(((i < 32 ? m0 : m1) >> (i & 31)) & 1u))
+				r[i >> 4][i & 15] = 0xFF800000u;
 }
 
 // One 128-key block of one row: S in the TMEM columns of tS -> P over them
 // (f16 pairs in columns 0-63, or bf16 groups of 8 hi + 8 lo). The row's block
 // maximum is known before any P is written, so raising the reference rescales
 // only O and l. Warp-collective; branches around TMEM accesses are
-// warp-uniform. Returns through m_ref and l_sum.
+// warp-uniform. Returns through m_ref and l_sum. Keys 0-63 are announced on
+// p_half as soon as they are written, so their products can start. Two passes
+// over the scores, 64 at a time and rolled: holding all 128 took registers that
+// the other roles then spilled for, and its code thrashed the instruction cache.
 template <int D, int KVT>
 __device__ __forceinline__ void softmax_rows(uint32_t tS, uint32_t tO, const uint32_t *mask,
 					     float sl2, bool o_live, float &m_ref, float &l_sum,
@@ -476,19 +530,19 @@ __device__ __forceinline__ void softmax_rows(uint32_t tS, uint32_t tO, const uin
 {
 	constexpr bool MX = KVT == 1;
 	constexpr float shift = MX ? kPShift : 0.f;
-	const uint32_t k0 = mask[0], k1 = mask[1], k2 = mask[2], k3 = mask[3];
-	const bool full = (k0 & k1 & k2 & k3) == 0xFFFFFFFFu;   // the same for every lane
-	float v[64];
+	const bool full = (mask[0] & mask[1] & mask[2] & mask[3]) == 0xFFFFFFFFu;  // same in all lanes
 	float mx = -CUDART_INF_F;
-#pragma unroll
+#pragma unroll 1
 	for (int half = 0; half < 2; ++half) {
-		tmem_ld64(tS + 64 * half, v);
-		if (!full)
-			mask64(v, half ? k2 : k0, half ? k3 : k1);
-		float m4[4] = {v[0], v[1], v[2], v[3]};
+		uint32_t r[4][16];
+		load_scores(tS + 64 * half, full, mask[2 * half], mask[2 * half + 1], r);
+		float m4[4];
 #pragma unroll
-		for (int i = 4; i < 64; ++i)
-			m4[i & 3] = fmaxf(m4[i & 3], v[i]);
+		for (int i = 0; i < 4; ++i)
+			m4[i] = __uint_as_float(r[0][i]);
+#pragma unroll
+		for (int k = 4; k < 64; ++k)
+			m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(r[k >> 4][k & 15]));
 		mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
 	}
 	const float gl = mx * sl2;
@@ -513,19 +567,20 @@ __device__ __forceinline__ void softmax_rows(uint32_t tS, uint32_t tO, const uin
 	// no key present yet (m_ref = -inf): every p is 0, not exp2(-inf + inf)
 	const float moff = m_ref == -CUDART_INF_F ? -CUDART_INF_F : shift - m_ref;
 	float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 1
 	for (int half = 0; half < 2; ++half) {
-		tmem_ld64(tS + 64 * half, v);
-		if (!full)
-			mask64(v, half ? k2 : k0, half ? k3 : k1);
+		uint32_t r[4][16];
+		load_scores(tS + 64 * half, full, mask[2 * half], mask[2 * half + 1], r);
 #pragma unroll
 		for (int c = 0; c < 64; c += MX ? 32 : 16) {
 			float w[16];
 			if constexpr (MX) {
 #pragma unroll
 				for (int i = 0; i < 16; ++i) {
-					const float p0 = ex2_approx(fmaf(v[c + 2 * i], sl2, moff));
-					const float p1 = ex2_approx(fmaf(v[c + 2 * i + 1], sl2, moff));
+					const int k = c + 2 * i;
+					const float p0 = ex2_approx(fmaf(__uint_as_float(r[k >> 4][k & 15]), sl2, moff));
+					const float p1 =
+					    ex2_approx(fmaf(__uint_as_float(r[k >> 4][(k & 15) + 1]), sl2, moff));
 					sum[i & 3] += p0 + p1;
 					w[i] = __uint_as_float(pack_f16x2(p0, p1));
 				}
@@ -533,14 +588,15 @@ __device__ __forceinline__ void softmax_rows(uint32_t tS, uint32_t tO, const uin
 			} else {
 #pragma unroll
 				for (int i = 0; i < 8; ++i) {
-					const float p0 = ex2_approx(fmaf(v[c + 2 * i], sl2, moff));
-					const float p1 = ex2_approx(fmaf(v[c + 2 * i + 1], sl2, moff));
+					const int k = c + 2 * i;
+					const float p0 = ex2_approx(fmaf(__uint_as_float(r[k >> 4][k & 15]), sl2, moff));
+					const float p1 =
+					    ex2_approx(fmaf(__uint_as_float(r[k >> 4][(k & 15) + 1]), sl2, moff));
 					sum[i & 3] += p0 + p1;
 					const uint32_t hi = pack_bf16x2(p0, p1);
 					w[i] = __uint_as_float(hi);
-					w[8 + i] = __uint_as_float(
-					    pack_bf16x2(p0 - __uint_as_float(hi << 16),
-							p1 - __uint_as_float(hi & 0xFFFF0000u)));
+					w[8 + i] = __uint_as_float(pack_bf16x2(p0 - __uint_as_float(hi << 16),
+									       p1 - __uint_as_float(hi & 0xFFFF0000u)));
 				}
 				tmem_st16_nowait(tS + 64 * half + c, w);
 			}
@@ -554,46 +610,92 @@ __device__ __forceinline__ void softmax_rows(uint32_t tS, uint32_t tO, const uin
 	l_sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
+// A warp's 32 query rows into the operand tile: bf16 as they are, or for MX f16
+// after a power of two that puts a row's largest element in [2^14, 2^15);
+// returns the inverse of that factor for row `lane`. off: where row `lane`
+// starts in q, in elements (-1: a row of zeros). Copied in by whole lines, then
+// converted in place, a row a lane (the swizzle spreads eight rows over all
+// banks). The loops stay rolled: this code runs once a piece, and unrolled it
+// spent 10k cycles on instruction fetches alone.
 template <int D, int KVT>
-__global__ void __launch_bounds__(kPThreads, 1)
-prefix_kernel(const kllm_prefix_args a)
+__device__ __forceinline__ float load_queries(uint8_t *tile, int r0, int lane, const void *q,
+					      long long off)
+{
+	constexpr int LPR = D / 8, RPP = 32 / LPR;
+	const int l = lane % LPR, sub = lane / LPR;
+#pragma unroll 2
+	for (int i = 0; i < 32; i += RPP) {
+		const long long o = __shfl_sync(0xffffffffu, off, i + sub);
+		uint8_t *dst = tile + (l >> 3) * (kPRows * 128) + swz(r0 + i + sub, l & 7);
+		if (o >= 0)
+			cp_async16(dst, static_cast<const uint8_t *>(q) + o * 2 + l * 16);
+		else
+			*reinterpret_cast<uint4 *>(dst) = make_uint4(0u, 0u, 0u, 0u);
+	}
+	cp_async_commit();
+	cp_async_wait<0>();
+	__syncwarp();
+	if constexpr (KVT == 0)
+		return 1.f;
+	const int r = r0 + lane;
+	uint32_t mb = 0u;                                // bf16 magnitudes order as integers
+#pragma unroll 4
+	for (int c = 0; c < LPR; ++c) {
+		const uint4 w = *reinterpret_cast<const uint4 *>(tile + (c >> 3) * (kPRows * 128) + swz(r, c & 7));
+		const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+		for (int i = 0; i < 4; ++i)
+			mb = max(mb, max((ww[i] << 16) & 0x7FFF0000u, ww[i] & 0x7FFF0000u));
+	}
+	const int E = mb ? (int)(mb >> 23) - 127 : 0;
+	const int e = min(max(14 - E, -100), 100);
+	const float f = __uint_as_float((uint32_t)(e + 127) << 23);
+#pragma unroll 2
+	for (int c = 0; c < LPR; ++c) {
+		uint4 *p = reinterpret_cast<uint4 *>(tile + (c >> 3) * (kPRows * 128) + swz(r, c & 7));
+		const uint4 w = *p;
+		uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+		for (int i = 0; i < 4; ++i)
+			ww[i] = pack_f16x2(__uint_as_float(ww[i] << 16) * f,
+					   __uint_as_float(ww[i] & 0xFFFF0000u) * f);
+		*p = make_uint4(ww[0], ww[1], ww[2], ww[3]);
+	}
+	return __uint_as_float((uint32_t)(127 - e) << 23);
+}
+
+template <int D, int KVT>
+__device__ __forceinline__ void init_prefix(PrefixSmem<D, KVT> &sm)
+{
+	mbar_init(&sm.q_full, 256);
+	mbar_init(&sm.q_empty, 1);
+	for (int i = 0; i < 2; ++i) {
+		mbar_init(&sm.k_full[i], kProd);
+		mbar_init(&sm.k_empty[i], 1);
+		mbar_init(&sm.v_full[i], kProd);
+		mbar_init(&sm.v_empty[i], 1);
+		mbar_init(&sm.s_full[i], 1);
+		mbar_init(&sm.p_half[i], 128);
+		mbar_init(&sm.p_full[i], 128);
+		mbar_init(&sm.o_full[i], 1);
+	}
+	for (int i = 0; i < kRaw; ++i) {
+		mbar_init(&sm.raw_full[i], 1);
+		mbar_init(&sm.raw_empty[i], kProd);
+	}
+	mbar_init(&sm.drain, 1);
+	sm.abort = 0;
+	fence_mbar_init();
+}
+
+// CTA `cta` of the W that share the T steps of the prefixes. The barriers are
+// initialised; every thread of the CTA calls it.
+template <int D, int KVT>
+__device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSmem<D, KVT> &sm, int cta,
+					    long long T, int W)
 {
 	using G = PG<D, KVT>;
-	using Sm = PrefixSmem<D, KVT>;
-	extern __shared__ __align__(1024) uint8_t smem_raw[];
-	Sm &sm = *reinterpret_cast<Sm *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-					 ~(uintptr_t)1023);
 	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-	if (tid == 0) {
-		mbar_init(&sm.q_full, 128);
-		mbar_init(&sm.q_empty, 1);
-		for (int i = 0; i < 2; ++i) {
-			mbar_init(&sm.k_full[i], 128);
-			mbar_init(&sm.k_empty[i], 1);
-			mbar_init(&sm.v_full[i], 128);
-			mbar_init(&sm.v_empty[i], 1);
-			mbar_init(&sm.s_full[i], 1);
-			mbar_init(&sm.p_half[i], 128);
-			mbar_init(&sm.p_full[i], 128);
-			mbar_init(&sm.o_full[i], 1);
-		}
-		for (int i = 0; i < kRaw; ++i) {
-			mbar_init(&sm.raw_full[i], 1);
-			mbar_init(&sm.raw_empty[i], 128);
-		}
-		mbar_init(&sm.drain, 1);
-		sm.abort = 0;
-		fence_mbar_init();
-	}
-	// the plan this launch reads is written by the kernel before it
-	grid_dependency_wait();
-	grid_launch_dependents();
-	const PHeader *hd = static_cast<const PHeader *>(a.header);
-	const long long T = hd->T;
-	const int W = hd->W, cta = blockIdx.x;
-	if (cta >= W)
-		return;                            // uniform: no barrier has been used yet
 	if (warp == kWarpMma) {
 		asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
 			     :: "r"(smem_u32(&sm.tmem_base)), "r"(512u));
@@ -605,14 +707,15 @@ prefix_kernel(const kllm_prefix_args a)
 	const uint32_t tmem = sm.tmem_base;
 	auto col_s = [](int t) { return (uint32_t)(t * 128); };
 	auto col_o = [](int t) { return (uint32_t)(256 + t * 128); };
-	long long x = cta * T / W;
-	const long long xe = (cta + 1) * T / W;
+	long long x = div_steps(cta * T, W);
+	const long long xe = div_steps((cta + 1) * T, W);
 	const int bs = a.block_size, ppb = kPKeys / bs;
 	const int sec = bs * (G::MX ? D * 9 / 8 : D * 2);
 	auto wait = [&](uint64_t *bar, uint32_t parity) { return p_wait(&sm.abort, bar, parity, a.err); };
 
 	if (warp < kWarpProd) {
 		// ================= softmax of stream t ========================================
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
 		const int t = warp >> 2, rr = (warp & 3) * 32 + lane;
 		const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
 		const uint32_t tS = lane_base + col_s(t), tO = lane_base + col_o(t);
@@ -620,11 +723,36 @@ prefix_kernel(const kllm_prefix_args a)
 		bool ok = true;
 		while (x < xe && ok) {
 			const Piece p = next_piece(a, x, xe, cta);
-			if (p.nb <= 0)
-				continue;
 			const int qt = p.solo ? 0 : t;
 			const int row = qt * kPRows + rr;            // row of the unit
+			if (p.nb <= 0) {                             // a share without a whole block
+				if (row < p.rows) {
+					const long long e = p.slot + (p.solo && t == 1 ? p.rows : 0) + row;
+					a.pm[e] = -CUDART_INF_F;
+					a.pl[e] = 0.f;
+				}
+				continue;
+			}
 			const bool warp_live = qt * kPRows + (warp & 3) * 32 < p.rows;
+			// ---- this row's query (a solo piece has one tile: stream 0 loads it) -------
+			// Rows of sequences that do not take part are computed too; nothing
+			// reads them.
+			if (np > 0 && !__all_sync(0xffffffffu, wait(&sm.q_empty, (uint32_t)((np - 1) & 1)))) {
+				ok = false;
+				break;
+			}
+			float qf = 1.f;
+			if (!p.solo || t == 0) {
+				const int rh = p.tile * kUnitRows + row;         // row of the kv head
+				const int seq = p.row0 + rh / a.group, hh = rh % a.group;
+				const long long off = row < p.rows
+				    ? ((long long)seq * a.num_heads + (long long)p.h * a.group + hh) * D : -1;
+				qf = load_queries<D, KVT>(sm.q[qt], (warp & 3) * 32, lane, a.q, off);
+				if (G::MX && p.solo)
+					sm.qf[np & 1][rr] = qf;
+				fence_async_smem();
+			}
+			mbar_arrive(&sm.q_full);
 			float m_ref = -CUDART_INF_F, l_sum = 0.f, sl2 = 0.f;
 			bool first = true;
 			for (int j = p.solo ? t : 0; j < p.nb; j += p.solo ? 2 : 1, ++n_s) {
@@ -634,7 +762,9 @@ prefix_kernel(const kllm_prefix_args a)
 				}
 				tc_fence_after();
 				if (first)
-					sl2 = a.scale_log2 * (G::MX ? sm.qf[np & 1][qt][rr] * KLLM_MX_DEC_UNBIAS : 1.f);
+					sl2 = a.scale_log2 *
+					      (G::MX ? (p.solo && t ? sm.qf[np & 1][rr] : qf) * KLLM_MX_DEC_UNBIAS
+						     : 1.f);
 				if (warp_live)
 					softmax_rows<D, KVT>(tS, tO, sm.key_ok[(kf + j) & 3], sl2, !first, m_ref,
 							     l_sum, &sm.p_half[t]);
@@ -681,10 +811,10 @@ prefix_kernel(const kllm_prefix_args a)
 		}
 	} else if (warp < kWarpMma) {
 		// ================= producers ====================================================
+		asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
 		const int pt = tid - kWarpProd * 32;
-		int np = 0, kf = 0, vf = 0, rf = 0;              // pieces, K fills, V fills, raw stages
+		int kf = 0, vf = 0, rf = 0;                  // K fills, V fills, raw stages
 		bool ok = true;
-		// a warp leaves as a whole: the query loads shuffle across it
 		auto wait_warp = [&](uint64_t *bar, uint32_t parity) {
 			return __all_sync(0xffffffffu, wait(bar, parity));
 		};
@@ -692,64 +822,18 @@ prefix_kernel(const kllm_prefix_args a)
 			const Piece p = next_piece(a, x, xe, cta);
 			if (p.nb <= 0)
 				continue;
-			// ---- queries ------------------------------------------------------------
-			if (np > 0 && !wait_warp(&sm.q_empty, (uint32_t)((np - 1) & 1)))
-				break;
-			{
-				const int l = pt % G::LPR;
-				const int all = p.rows;
-				for (int t = 0; t < (p.solo ? 1 : 2); ++t)
-					for (int r = pt / G::LPR; r < kPRows; r += 128 / G::LPR) {
-						const int ru = t * kPRows + r;               // row of the unit
-						const int rh = p.tile * kUnitRows + ru;      // row of the head
-						const int seq = p.row0 + rh / a.group, hh = rh % a.group;
-						uint4 w = make_uint4(0u, 0u, 0u, 0u);
-						if (ru < all && a.row_group[seq] == p.g)
-							w = __ldg(reinterpret_cast<const uint4 *>(
-								static_cast<const uint8_t *>(a.q) +
-								(((size_t)seq * a.num_heads + (size_t)p.h * a.group + hh) * D +
-								 l * 8) * 2));
-						if constexpr (G::MX) {
-							// the row times 2^e, its largest in [2^14, 2^15)
-							const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-							float mx = 0.f;
-#pragma unroll
-							for (int i = 0; i < 4; ++i)
-								mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(ww[i] << 16)),
-										     fabsf(__uint_as_float(ww[i] & 0xFFFF0000u))));
-#pragma unroll
-							for (int o = 1; o < G::LPR; o <<= 1)
-								mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-							const int E = mx > 0.f ? (int)((__float_as_uint(mx) >> 23) & 0xFFu) - 127 : 0;
-							const int e = min(max(14 - E, -100), 100);
-							const float f = __uint_as_float((uint32_t)(e + 127) << 23);
-							uint32_t o4[4];
-#pragma unroll
-							for (int i = 0; i < 4; ++i)
-								o4[i] = pack_f16x2(__uint_as_float(ww[i] << 16) * f,
-										   __uint_as_float(ww[i] & 0xFFFF0000u) * f);
-							w = make_uint4(o4[0], o4[1], o4[2], o4[3]);
-							if (l == 0)
-								sm.qf[np & 1][t][r] = __uint_as_float((uint32_t)(127 - e) << 23);
-						}
-						*reinterpret_cast<uint4 *>(sm.q[t] + (l >> 3) * G::HALF + swz(r, l & 7)) = w;
-					}
-			}
-			fence_async_smem();
-			mbar_arrive(&sm.q_full);
-			++np;
 			// ---- K and V blocks ---------------------------------------------------------
-			auto write_mask = [&](uint32_t okm) {
-				if (pt < 4) {
-					uint32_t m = 0;
+			const uint32_t all_pages = (1u << ppb) - 1u;
+			// key bits of word w of a block whose pages present are okm
+			auto key_mask = [&](uint32_t okm, int w) {
+				uint32_t m = 0;
 #pragma unroll
-					for (int i = 0; i < 2; ++i) {
-						const int page = (32 * pt + 16 * i) / bs;
-						if (page < ppb && ((okm >> page) & 1u))
-							m |= 0xFFFFu << (16 * i);
-					}
-					sm.key_ok[kf & 3][pt] = m;
+				for (int i = 0; i < 2; ++i) {
+					const int page = (32 * w + 16 * i) / bs;
+					if (page < ppb && ((okm >> page) & 1u))
+						m |= 0xFFFFu << (16 * i);
 				}
+				return m;
 			};
 			if constexpr (G::MX) {
 				for (int j = 0; j < p.nb && ok; ++j)
@@ -764,9 +848,19 @@ prefix_kernel(const kllm_prefix_args a)
 						if (!ok)
 							break;
 						const uint32_t okm = sm.slot_ok[st];
-						dequant_block<D>(which ? sm.v[vf & 1] : sm.k[0], sm.raw[st], okm, bs, pt);
-						if (which == 0)
-							write_mask(okm);
+						// all pages present and no key past the last one
+						const bool full = okm == all_pages && ppb * bs == kPKeys;
+						uint32_t mk[4] = {~0u, ~0u, ~0u, ~0u};
+						if (!full)
+#pragma unroll
+							for (int w = 0; w < 4; ++w)
+								mk[w] = key_mask(okm, w);
+						dequant_block<D>(which ? sm.v[vf & 1] : sm.k[0], sm.raw[st], sm.raws[st], mk,
+								 full, pt);
+						if (which == 0 && pt == 0)
+#pragma unroll
+							for (int w = 0; w < 4; ++w)
+								sm.key_ok[kf & 3][w] = mk[w];
 						fence_async_smem();
 						mbar_arrive(&sm.raw_empty[st]);
 						if (which == 0) {
@@ -781,6 +875,9 @@ prefix_kernel(const kllm_prefix_args a)
 				// fills run two ahead of their arrival: K0 V0 K1 V1 ...
 				const int l = pt % G::LPR;
 				const int kf0 = kf, n_fill = 2 * p.nb;
+				// (row / 16) x inv16 / 256 = row / bs for rows below 128 and the block
+				// sizes 16, 32 .. 128
+				const int inv16 = 256 / (bs >> 4) + 1;
 				auto arrive_fill = [&](int f) {
 					const int b = (kf0 + (f >> 1)) & 1;
 					mbar_arrive((f & 1) ? &sm.v_full[b] : &sm.k_full[b]);
@@ -796,25 +893,24 @@ prefix_kernel(const kllm_prefix_args a)
 						break;
 					const uint32_t okm = sm.slot_ok[st];
 					uint8_t *dst = (which ? sm.v[cnt & 1] : sm.k[cnt & 1]) + (l >> 3) * G::HALF;
-					int row = pt / G::LPR, page = 0, tok = row;
-					for (int i = 0; i < kPKeys * G::LPR / 128; ++i) {
-						uint8_t *o = dst + swz(row, l & 7);
-						if ((okm >> page) & 1u)
+					// a lane's rows are multiples of 8 apart, so their swizzle is the same
+					constexpr int RPP = kProd / G::LPR;
+					const int row0 = pt / G::LPR;
+					uint8_t *o = dst + swz(row0, l & 7);
+#pragma unroll 4
+					for (int row = row0; row < kPKeys; row += RPP, o += RPP * 128) {
+						const int page = ((row >> 4) * inv16) >> 8;        // row / bs
+						if ((okm >> page) & 1u)                            // never past the last page
 							cp_async16(o, reinterpret_cast<const uint8_t *>(sm.pg[st][which][page]) +
-									  (size_t)tok * D * 2 + l * 16);
+									  (row - page * bs) * (D * 2) + l * 16);
 						else
 							*reinterpret_cast<uint4 *>(o) = make_uint4(0u, 0u, 0u, 0u);
-						row += 128 / G::LPR;
-						tok += 128 / G::LPR;
-						if (tok >= bs) {
-							tok -= bs;
-							++page;
-						}
 					}
 					cp_async_commit();
-					if (which == 0)
-						write_mask(okm);
-					else {
+					if (which == 0) {
+						if (pt < 4)
+							sm.key_ok[kf & 3][pt] = key_mask(okm, pt);
+					} else {
 						mbar_arrive(&sm.raw_empty[st]);
 						++rf;
 					}
@@ -835,7 +931,9 @@ prefix_kernel(const kllm_prefix_args a)
 				}
 			}
 		}
-	} else if (warp == kWarpMma) {
+	} else {
+	asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+	if (warp == kWarpMma) {
 		// ================= MMA issue =======================================================
 		// The whole warp runs this role (descriptors stay warp-uniform); one
 		// elected lane issues.
@@ -983,7 +1081,7 @@ prefix_kernel(const kllm_prefix_args a)
 		// every MMA issued completes before TMEM is freed
 		commit(&sm.drain);
 		mbar_wait_ns(&sm.drain, 0u, kPWaitNs);
-	} else {
+	} else if (warp == kWarpLoad) {
 		// ================= page lookup and raw copies ========================================
 		int rf = 0;
 		uint32_t armed[kRaw] = {0, 0, 0};
@@ -1039,10 +1137,14 @@ prefix_kernel(const kllm_prefix_args a)
 						for (int i = 0; i < kRaw; ++i)
 							armed[i] += i == st ? 1u : 0u;
 						__syncwarp();
-						if (here)
-							bulk_g2s(sm.raw[st] + lane * sec,
-								 reinterpret_cast<const void *>((which ? e.v : e.k) + off),
-								 (uint32_t)sec, &sm.raw_full[st]);
+						// payload and scales of a page to the rows of its keys
+						if (here) {
+							const uint8_t *src = reinterpret_cast<const uint8_t *>((which ? e.v : e.k) + off);
+							bulk_g2s(sm.raw[st] + lane * bs * D, src, (uint32_t)(bs * D),
+								 &sm.raw_full[st]);
+							bulk_g2s(sm.raws[st] + lane * bs * (D / 8), src + bs * D,
+								 (uint32_t)(bs * (D / 8)), &sm.raw_full[st]);
+						}
 					} else {
 						if (lane < 8) {
 							sm.pg[st][0][lane] = e.k + off;
@@ -1064,6 +1166,7 @@ prefix_kernel(const kllm_prefix_args a)
 				if (armed[i] > 0)
 					mbar_wait_ns(&sm.raw_full[i], (armed[i] - 1) & 1u, kPWaitNs);
 	}
+	}
 
 	tc_fence_before();
 	__syncthreads();
@@ -1075,38 +1178,418 @@ prefix_kernel(const kllm_prefix_args a)
 	}
 }
 
+// ---- suffixes --------------------------------------------------------------------------
+
+// Warps of a suffix CTA that work (the BF16 tile needs more registers).
+template <int KVT>
+struct SW {
+	static constexpr int N = KVT == 1 ? 12 : 8;
+};
+
+struct SufSeg {
+	int s, h, j, ts;      // sequence, kv head, tile of its suffix, tiles of it
+};
+
+// The sequence, head and tile of step x of the tiles laid end to end
+// (sequence-major, then kv head); pre: exclusive sums of tiles per sequence.
+__device__ __forceinline__ SufSeg locate_suffix(const int *pre, int S, int H, long long x)
+{
+	int lo = 0, hi = S - 1;
+	while (lo < hi) {
+		const int mid = (lo + hi + 1) >> 1;
+		if ((long long)pre[mid] * H <= x)
+			lo = mid;
+		else
+			hi = mid - 1;
+	}
+	SufSeg c;
+	c.s = lo;
+	c.ts = pre[lo + 1] - pre[lo];
+	const int rel = (int)(x - (long long)pre[lo] * H);   // below ts x H: 32 bits
+	c.h = rel / c.ts;
+	c.j = rel - c.h * c.ts;
+	return c;
+}
+
+// Tiles j0 .. j1 - 1 of one (sequence, kv head) by a warp, exactly, in fp32
+// with plain loads: for pieces whose tile loop was not finite because a page
+// holds payload 0x7F / 0xFF (which the hardware conversion reads as NaN). No
+// writer emits those codes, but pages that arrive from a store are raw bytes.
+template <int D>
+__device__ __noinline__ void suffix_exact(const kllm_prefix_args &a, int s, int h, int j0, int j1,
+					  float sl2, float *xm, float *xl, float *xo)
+{
+	constexpr int NV = D / 32;
+	const int lane = threadIdx.x & 31, bs = a.block_size;
+	const size_t sec = (size_t)bs * D * 9 / 8;
+	for (int hh = 0; hh < a.group; ++hh) {
+		const uint16_t *qp = static_cast<const uint16_t *>(a.q) +
+				     ((size_t)s * a.num_heads + (size_t)h * a.group + hh) * D + lane * NV;
+		float q[NV], o[NV], m = -CUDART_INF_F, l = 0.f;
+#pragma unroll
+		for (int i = 0; i < NV; ++i) {
+			q[i] = __uint_as_float((uint32_t)qp[i] << 16);
+			o[i] = 0.f;
+		}
+		const int t1 = min(j1 * kTile, a.suf_lens[s]);
+		for (int t = j0 * kTile; t < t1; ++t) {
+			const int page = a.suf_start[s] + t / bs, r = t % bs;
+			const DevEntry *e = static_cast<const DevEntry *>(a.table) + (size_t)s * a.max_blocks + page;
+			const unsigned long long off = a.layer_off + (unsigned long long)h * sec;
+			if (!e->valid || !e->k || ((e->k | e->v) & 15ull) ||
+			    !(in_arenas(a.arenas, e->k + off, sec) && in_arenas(a.arenas, e->v + off, sec)))
+				continue;                        // skipped by the tile loop as well
+			const uint8_t *kb = reinterpret_cast<const uint8_t *>(e->k + off);
+			const uint8_t *vb = reinterpret_cast<const uint8_t *>(e->v + off);
+			const size_t so = (size_t)bs * D + (size_t)r * (D / 8) + lane * NV / 8;
+			const float ksc = e4m3_ref_to_f32(kb[so]), vsc = e4m3_ref_to_f32(vb[so]);
+			float dot = 0.f;
+#pragma unroll
+			for (int i = 0; i < NV; ++i)
+				dot = fmaf(q[i], e4m3_ref_to_f32(kb[(size_t)r * D + lane * NV + i]) * ksc, dot);
+#pragma unroll
+			for (int w = 16; w; w >>= 1)
+				dot += __shfl_xor_sync(0xffffffffu, dot, w);
+			const float x = dot * sl2, mn = fmaxf(m, x);
+			const float f = exp2f(m - mn), pw = exp2f(x - mn);
+			l = fmaf(l, f, pw);
+#pragma unroll
+			for (int i = 0; i < NV; ++i)
+				o[i] = fmaf(o[i], f, pw * e4m3_ref_to_f32(vb[(size_t)r * D + lane * NV + i]) * vsc);
+			m = mn;
+		}
+		// the join multiplies MX values by what the tile loop leaves off
+#pragma unroll
+		for (int i = 0; i < NV; ++i)
+			xo[(size_t)hh * D + lane * NV + i] = o[i] * (1.f / KLLM_MX_DEC_UNBIAS);
+		if (lane == 0) {
+			xm[hh] = m;
+			xl[hh] = l;
+		}
+	}
+}
+
+template <int D, int KVT>
+struct SufLayout {
+	using Gm = Geom<D, KVT>;
+	static constexpr int NW = SW<KVT>::N, NST = 3;
+	static constexpr size_t ring = 0, bar = (size_t)NW * NST * Gm::STAGE, meta = bar + 8 * NW * NST;
+	static constexpr size_t lut = meta + 4 * NW * NST, pre = lut + 4 * 256;
+	static constexpr size_t total = pre + 4 * (KLLM_MAX_SEQS_LAUNCH + 1);
+};
+
+// CTA `cta` of those that share the N tiles of the suffixes among WS warps.
+// smem: SufLayout bytes, 128-byte aligned; its barriers are initialised here.
+template <int D, int KVT>
+__device__ __forceinline__ void suffix_role(const kllm_prefix_args &a, uint8_t *smem, int cta, long long N,
+					    int WS)
+{
+	using Gm = Geom<D, KVT>;
+	using Lay = SufLayout<D, KVT>;
+	constexpr int NW = Lay::NW, NST = Lay::NST;
+	const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+	const int S = a.num_seqs, H = a.num_kv_heads, tpp = a.block_size / kTile;
+	uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Lay::bar);
+	int *meta = reinterpret_cast<int *>(smem + Lay::meta);
+	uint32_t *lut = reinterpret_cast<uint32_t *>(smem + Lay::lut);
+	int *spre = reinterpret_cast<int *>(smem + Lay::pre);
+	if (cta * NW >= WS)
+		return;                                    // uniform over the CTA
+	const bool local = S <= KLLM_MAX_SEQS_LAUNCH;
+	if (local)
+		for (int i = tid; i <= S; i += kPThreads)
+			spre[i] = a.tile_pre[i];
+	if constexpr (Gm::MX)
+		for (int i = tid; i < 256; i += kPThreads)
+			lut[i] = mx_scale_lut_entry_f16((uint32_t)i);
+	if (warp < NW && lane == 0) {
+		for (int i = 0; i < NST; ++i)
+			mbar_init(&bars[warp * NST + i], 1);
+		fence_mbar_init();
+	}
+	__syncthreads();
+	if (warp >= NW) {
+		if constexpr (Gm::MX)
+			asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+		else
+			asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+		return;
+	}
+	if constexpr (Gm::MX)
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+	else
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+	const int *pre = local ? spre : a.tile_pre;
+	const int w = cta * NW + warp;
+	if (w >= WS)
+		return;
+	const long long xa = div_steps(w * N, WS), xb = div_steps((w + 1) * N, WS);
+	const int n = (int)(xb - xa);
+	uint8_t *ring = smem + Lay::ring + (size_t)warp * NST * Gm::STAGE;
+	uint64_t *bar = bars + warp * NST;
+	int *ntoks = meta + warp * NST;
+	const uint64_t policy = l2_evict_first_policy();
+	const size_t sec = Gm::MX ? (size_t)a.block_size * D * 9 / 8 : (size_t)a.block_size * D * 2;
+
+	// block-table entries of 32 consecutive tiles, one a lane: loaded a batch
+	// ahead (raw), turned into section addresses when their turn comes
+	unsigned long long ck = 0, cv = 0, nk, nv;
+	int cvalid = 0, cpack = 0, nvalid, npack;
+	auto load = [&](int base, unsigned long long &ek, unsigned long long &ev, int &valid, int &pack) {
+		const int pos = base + lane;
+		ek = ev = 0ull;
+		valid = pack = 0;
+		if (pos < n) {
+			const SufSeg c = locate_suffix(pre, S, H, xa + pos);
+			const int ntok = min(a.suf_lens[c.s] - c.j * kTile, kTile);
+			const int page = c.j / tpp, sub = c.j - page * tpp;
+			const DevEntry *e = static_cast<const DevEntry *>(a.table) +
+					    (size_t)c.s * a.max_blocks + a.suf_start[c.s] + page;
+			ek = __ldg(&e->k);
+			ev = __ldg(&e->v);
+			valid = __ldg(&e->valid);
+			pack = ntok | (sub << 8) | (c.h << 16);
+		}
+	};
+	auto finish = [&]() {
+		const int ntok = cpack & 0xFF, sub = (cpack >> 8) & 0xFF, h = cpack >> 16;
+		const bool present = cvalid && ck != 0ull, aligned = ((ck | cv) & 15ull) == 0ull;
+		if (present && !aligned && a.err)
+			atomicOr(a.err, 0x2u);
+		bool ok = present && aligned && ntok > 0;
+		const unsigned long long off = a.layer_off + (unsigned long long)h * sec;
+		if (ok && !(in_arenas(a.arenas, ck + off, sec) && in_arenas(a.arenas, cv + off, sec))) {
+			ok = false;
+			if (a.err)
+				atomicOr(a.err, KLLM_ERR_PAGE_RANGE_BIT);
+		}
+		ck += off;
+		cv += off;
+		cpack = (ok ? ntok : 0) | (sub << 8);
+	};
+	load(0, ck, cv, cvalid, cpack);
+	load(32, nk, nv, nvalid, npack);
+	finish();
+	int pb = 0;
+	auto issue = [&](int pos) {
+		int bi = pos - pb;
+		if (bi >= 32) {
+			ck = nk;
+			cv = nv;
+			cvalid = nvalid;
+			cpack = npack;
+			finish();
+			pb += 32;
+			bi -= 32;
+			load(pb + 32, nk, nv, nvalid, npack);
+		}
+		const unsigned long long ek = __shfl_sync(0xffffffffu, ck, bi);
+		const unsigned long long ev = __shfl_sync(0xffffffffu, cv, bi);
+		const int pack = __shfl_sync(0xffffffffu, cpack, bi);
+		if (lane == 0) {
+			const int st = pos % NST, ntok = pack & 0xFF, sub = pack >> 8;
+			ntoks[st] = ntok;
+			if (ntok) {
+				mbar_arrive_expect_tx(&bar[st], Gm::STAGE);
+				uint8_t *dK = ring + (size_t)st * Gm::STAGE, *dV = dK + Gm::KV;
+				const uint8_t *sK = reinterpret_cast<const uint8_t *>(ek);
+				const uint8_t *sV = reinterpret_cast<const uint8_t *>(ev);
+				if (Gm::MX && tpp == 1) {       // payload and scales in one run
+					bulk_g2s_stream(dK, sK, Gm::KV, &bar[st], policy);
+					bulk_g2s_stream(dV, sV, Gm::KV, &bar[st], policy);
+				} else {
+					bulk_g2s_stream(dK, sK + (size_t)sub * Gm::PAY, Gm::PAY, &bar[st], policy);
+					bulk_g2s_stream(dV, sV + (size_t)sub * Gm::PAY, Gm::PAY, &bar[st], policy);
+				}
+				if (Gm::MX && tpp > 1) {
+					const size_t so = (size_t)a.block_size * D + (size_t)sub * Gm::SCL;
+					bulk_g2s_stream(dK + Gm::PAY, sK + so, Gm::SCL, &bar[st], policy);
+					bulk_g2s_stream(dV + Gm::PAY, sV + so, Gm::SCL, &bar[st], policy);
+				}
+			} else {
+				mbar_arrive(&bar[st]);
+			}
+		}
+	};
+	int p = 0;
+	for (; p < n && p < NST - 1; ++p)
+		issue(p);
+
+	SufSeg cc = locate_suffix(pre, S, H, xa);
+	bool redo = false;
+	uint32_t q[D / 8];
+	load_q<D>(q, a, cc.s, cc.h, lane);
+	const float scale = a.scale_log2 * (Gm::MX ? KLLM_MX_DEC_UNBIAS : 1.f);
+	float sl2 = scale;
+	if constexpr (Gm::MX)
+		sl2 = scale * q_to_f16<D>(q);
+	float o[D / 16][4];
+#pragma unroll
+	for (int mt = 0; mt < D / 16; ++mt)
+		o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
+	float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
+	float mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F;
+	const int g = lane >> 2, c = lane & 3;
+
+#pragma unroll 1
+	for (int i = 0; i < n; ++i) {
+		if (p < n) {
+			issue(p);
+			++p;
+		}
+		const int st = i % NST;
+		if (!__all_sync(0xffffffffu, mbar_wait_ns(&bar[st], (uint32_t)((i / NST) & 1), kPWaitNs))) {
+			if (lane == 0 && a.err)
+				atomicOr(a.err, KLLM_ERR_TIMEOUT_BIT);
+			return;
+		}
+		const int ntok = *reinterpret_cast<volatile int *>(&ntoks[st]);
+		if (ntok > 0) {
+			const uint8_t *sK = ring + (size_t)st * Gm::STAGE;
+			tile_compute<D, KVT>(sK, sK + Gm::KV, lut, ntok, q, o, m0, m1, l0, l1, mx0, mx1, sl2,
+					     lane);
+		}
+		__syncwarp();
+		const bool seg_end = cc.j + 1 == cc.ts, last = i + 1 == n;
+		if (!(seg_end || last)) {
+			++cc.j;
+			continue;
+		}
+		// ---- piece finished: its partial, against its exact maximum ----------------
+#pragma unroll
+		for (int off = 4; off < 32; off <<= 1) {
+			mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
+			mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
+		}
+		const float f0 = mx0 > m0 ? exp2f(m0 - mx0) : 1.f, f1 = mx1 > m1 ? exp2f(m1 - mx1) : 1.f;
+		m0 = fmaxf(m0, mx0);
+		m1 = fmaxf(m1, mx1);
+		float L0 = l0 * f0, L1 = l1 * f1;
+#pragma unroll
+		for (int off = 4; off < 32; off <<= 1) {
+			L0 += __shfl_xor_sync(0xffffffffu, L0, off);
+			L1 += __shfl_xor_sync(0xffffffffu, L1, off);
+		}
+		// (sequence, head) + warp numbers the pieces without gaps or clashes
+		const size_t slot = (size_t)cc.s * H + cc.h + w;
+		float *xm = a.xm + slot * a.group, *xl = a.xl + slot * a.group, *xo = a.xo + slot * a.group * D;
+		if constexpr (Gm::MX) {
+			// not finite: the piece is marked by its sum and done again at the end
+			bool bad = !isfinite(L0) || !isfinite(L1);
+#pragma unroll
+			for (int mt = 0; mt < D / 16; ++mt)
+				bad |= !isfinite(o[mt][0] + o[mt][1] + o[mt][2] + o[mt][3]);
+			if (__any_sync(0xffffffffu, bad)) {
+				L0 = L1 = CUDART_INF_F;
+				redo = true;
+			}
+		}
+#pragma unroll
+		for (int hp = 0; hp < 2; ++hp) {
+			const int hh = 2 * c + hp;
+			if (hh < a.group) {
+				const float f = hp ? f1 : f0;
+				float *dst = xo + (size_t)hh * D + g * (D / 8);
+#pragma unroll
+				for (int mt = 0; mt < D / 16; mt += 2)
+					*reinterpret_cast<float4 *>(dst + 2 * mt) =
+					    make_float4(o[mt][hp] * f, o[mt][2 + hp] * f,
+							o[mt + 1][hp] * f, o[mt + 1][2 + hp] * f);
+				if (g == 0) {
+					xm[hh] = hp ? m1 : m0;
+					xl[hh] = hp ? L1 : L0;
+				}
+			}
+		}
+		if (last)
+			break;
+		cc.j = 0;
+		if (++cc.h == H) {
+			cc.h = 0;
+			do {
+				++cc.s;
+			} while (pre[cc.s + 1] == pre[cc.s]);
+			cc.ts = pre[cc.s + 1] - pre[cc.s];
+		}
+		load_q<D>(q, a, cc.s, cc.h, lane);
+		if constexpr (Gm::MX)
+			sl2 = scale * q_to_f16<D>(q);
+#pragma unroll
+		for (int mt = 0; mt < D / 16; ++mt)
+			o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
+		m0 = m1 = mx0 = mx1 = -CUDART_INF_F;
+		l0 = l1 = 0.f;
+	}
+	if constexpr (Gm::MX) {
+		if (redo) {                    // rare: the marked pieces of this warp, exactly
+			__syncwarp();
+			for (long long x = xa; x < xb;) {
+				const SufSeg e = locate_suffix(pre, S, H, x);
+				const int nt = (int)min((long long)(e.ts - e.j), xb - x);
+				const size_t slot = ((size_t)e.s * H + e.h + w) * a.group;
+				if (__ldcg(a.xl + slot) == CUDART_INF_F)
+					suffix_exact<D>(a, e.s, e.h, e.j, e.j + nt, a.scale_log2, a.xm + slot,
+							a.xl + slot, a.xo + slot * D);
+				x += nt;
+			}
+		}
+	}
+}
+
+template <int D, int KVT>
+__global__ void __launch_bounds__(kPThreads, 1)
+attend_kernel(const kllm_prefix_args a)
+{
+	extern __shared__ __align__(1024) uint8_t smem_raw[];
+	uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+						   ~(uintptr_t)1023);
+	// the plan this launch reads is written by the kernel before it
+	grid_dependency_wait();
+	grid_launch_dependents();
+	const PHeader *hd = static_cast<const PHeader *>(a.header);
+	const int cta = blockIdx.x, n_prefix = hd->n_prefix;
+	if (cta < n_prefix) {
+		const long long T = hd->T;
+		const int W = hd->W;
+		if (cta >= W)
+			return;
+		PrefixSmem<D, KVT> &sm = *reinterpret_cast<PrefixSmem<D, KVT> *>(smem);
+		if (threadIdx.x == 0)
+			init_prefix(sm);
+		prefix_role<D, KVT>(a, sm, cta, T, W);
+	} else {
+		suffix_role<D, KVT>(a, smem, cta - n_prefix, hd->N, hd->WS);
+	}
+}
+
 // ---- join -----------------------------------------------------------------------------
 
-constexpr int kJThreads = 256;
 constexpr int kJRows = 32;
 
 // One CTA: 32 consecutive rows (sequence-major) of one kv head. Phase 1: a lane
-// per row, a warp per chunk of 4 dims: the prefix pieces' sums against their
-// maximum (the partials hold [D / 4][rows][4], so a warp reads 512 contiguous
-// bytes). Phase 2: eight threads per row add the suffix triple and store.
+// per row, a warp per two chunks of 4 dims: the prefix pieces folded into a
+// running (max, sum, o), six pieces' loads in flight (the partials hold [D /
+// 4][rows][4], so a warp reads 512 contiguous bytes). Phase 2: D / 8 threads
+// per row fold the suffix pieces (rows of D) and store.
 template <int D>
-__global__ void __launch_bounds__(kJThreads)
+__global__ void __launch_bounds__(4 * D)
 join_kernel(const kllm_prefix_args a, float unbias)
 {
+	constexpr int kFly = 6, kFlyS = 4;
 	__shared__ float acc_s[kJRows][D + 4];
 	__shared__ float m_s[kJRows], l_s[kJRows];
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-	const int h = blockIdx.y, rows = a.num_seqs * a.group;
+	const int h = blockIdx.y, H = a.num_kv_heads, rows = a.num_seqs * a.group;
 	grid_dependency_wait();
 	const PHeader *hd = static_cast<const PHeader *>(a.header);
-	const long long T = hd->T, W = hd->W;
 	const int i = blockIdx.x * kJRows + lane;
 	{
 		const int seq = i / a.group;
 		const int g = i < rows ? a.row_group[seq] : -1;
 		float M = -CUDART_INF_F, L = 0.f;
-		float acc[D / 32][4];
-#pragma unroll
-		for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-			for (int q = 0; q < 4; ++q)
-				acc[c][q] = 0.f;
+		float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 		if (g >= 0) {
+			const long long T = hd->T, W = hd->W;
 			const PGroup G = static_cast<const PGroup *>(a.groups)[g];
 			const int lr = (seq - G.row0) * a.group + i % a.group;
 			const bool solo = G.wgt == 1;
@@ -1114,71 +1597,129 @@ join_kernel(const kllm_prefix_args a, float unbias)
 			const int urows = min(kUnitRows, G.nseq * a.group - tile * kUnitRows);
 			const long long cost = (long long)G.nblk * G.wgt;
 			const long long ux = G.x0 + ((long long)h * G.tiles + tile) * cost;
-			const long long c0 = ((ux + 1) * W - 1) / T, c1 = ((ux + cost) * W - 1) / T;
-			const long long base = G.r0 + (long long)h * G.alloc + tile * kUnitRows;
-			for (int pass = 0; pass < 2; ++pass)
-				for (long long c = c0; c <= c1; ++c) {
-					const long long lo = max(c * T / W, ux), hi = min((c + 1) * T / W, ux + cost);
-					if ((hi - ux) / G.wgt <= (lo - ux) / G.wgt)
-						continue;              // no whole block in this share
-					for (int st = 0; st < (solo ? 2 : 1); ++st) {
-						const long long at = base + (long long)kUnitRows * c + st * urows;
-						const float l = __ldcg(a.pl + at + r), m = __ldcg(a.pm + at + r);
-						if (!(l != 0.f))
-							continue;
-						if (pass == 0) {
-							M = fmaxf(M, m);
-							continue;
-						}
-						const float e = exp2f(m - M);
-						L = fmaf(l, e, L);
-						const float *po = a.po + at * D + (size_t)r * 4;
+			// the shares that overlap the unit; solo pieces are two streams
+			const long long c0 = div_steps((ux + 1) * W - 1, T), c1 = div_steps((ux + cost) * W - 1, T);
+			const long long base = G.r0 + (long long)h * G.alloc + tile * kUnitRows + kUnitRows * c0;
+			const int sh = solo ? 1 : 0, np = (int)(c1 - c0 + 1) << sh;
+			for (int p0 = 0; p0 < np; p0 += kFly) {
+				float l[kFly], m[kFly];
+				float4 o[kFly][2];
 #pragma unroll
-						for (int q = 0; q < D / 32; ++q) {
-							const float4 o = __ldcg(reinterpret_cast<const float4 *>(
-							    po + (size_t)(warp + 8 * q) * urows * 4));
-							acc[q][0] = fmaf(o.x, e, acc[q][0]);
-							acc[q][1] = fmaf(o.y, e, acc[q][1]);
-							acc[q][2] = fmaf(o.z, e, acc[q][2]);
-							acc[q][3] = fmaf(o.w, e, acc[q][3]);
-						}
+				for (int u = 0; u < kFly; ++u) {
+					const int p = p0 + u;
+					l[u] = 0.f;
+					m[u] = -CUDART_INF_F;
+					if (p < np) {
+						const long long at = base + (long long)kUnitRows * (p >> sh) +
+								     (solo && (p & 1) ? urows : 0);
+						l[u] = __ldcg(a.pl + at + r);
+						m[u] = __ldcg(a.pm + at + r);
+						const float *po = a.po + at * D + ((size_t)2 * warp * urows + r) * 4;
+						o[u][0] = __ldcg(reinterpret_cast<const float4 *>(po));
+						o[u][1] = __ldcg(reinterpret_cast<const float4 *>(po + 4 * urows));
 					}
 				}
+				float mb = M;
+#pragma unroll
+				for (int u = 0; u < kFly; ++u)
+					if (l[u] != 0.f)
+						mb = fmaxf(mb, m[u]);
+				if (mb > M) {
+					const float f = exp2f(M - mb);       // 0 while M is -inf
+					L *= f;
+#pragma unroll
+					for (int q = 0; q < 8; ++q)
+						acc[q] *= f;
+					M = mb;
+				}
+#pragma unroll
+				for (int u = 0; u < kFly; ++u)
+					if (l[u] != 0.f) {                   // o of an empty piece is not written
+						const float e = exp2f(m[u] - M);
+						L = fmaf(l[u], e, L);
+#pragma unroll
+						for (int q = 0; q < 2; ++q) {
+							acc[4 * q] = fmaf(o[u][q].x, e, acc[4 * q]);
+							acc[4 * q + 1] = fmaf(o[u][q].y, e, acc[4 * q + 1]);
+							acc[4 * q + 2] = fmaf(o[u][q].z, e, acc[4 * q + 2]);
+							acc[4 * q + 3] = fmaf(o[u][q].w, e, acc[4 * q + 3]);
+						}
+					}
+			}
 		}
 #pragma unroll
-		for (int q = 0; q < D / 32; ++q)
-			*reinterpret_cast<float4 *>(&acc_s[lane][4 * (warp + 8 * q)]) =
-			    make_float4(acc[q][0], acc[q][1], acc[q][2], acc[q][3]);
+		for (int q = 0; q < 2; ++q)
+			*reinterpret_cast<float4 *>(&acc_s[lane][8 * warp + 4 * q]) =
+			    make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
 		if (warp == 0) {
 			m_s[lane] = M;
 			l_s[lane] = L;
 		}
 	}
 	__syncthreads();
-	const int r = tid >> 3, part = tid & 7, ii = blockIdx.x * kJRows + r;
+	const int r = tid / (D / 8), part = tid % (D / 8), ii = blockIdx.x * kJRows + r;
 	if (ii >= rows)
 		return;
-	const size_t row = (size_t)(ii / a.group) * a.num_heads + (size_t)h * a.group + ii % a.group;
-	const float Ms = a.sm[row] * kPLog2e, Ls = a.sl[row], Mp = m_s[r], Lp = l_s[r];
-	const float M = fmaxf(Ls > 0.f ? Ms : -CUDART_INF_F, Lp > 0.f ? Mp : -CUDART_INF_F);
-	const float wp = Lp > 0.f ? exp2f(Mp - M) : 0.f;
-	const float ws = Ls > 0.f ? Ls * exp2f(Ms - M) : 0.f;
-	const float den = fmaf(Lp, wp, ws);
-	const float fp = den > 0.f ? wp * unbias / den : 0.f, fs = den > 0.f ? ws / den : 0.f;
-	constexpr int N = D / 8;                      // dims per thread
-	const float *so = a.so + row * D + part * N;
-	uint32_t o[N / 2];
+	const int seq = ii / a.group, hh = ii - seq * a.group;
+	float M = m_s[r], L = l_s[r], acc[8];
 #pragma unroll
-	for (int c = 0; c < N; c += 4) {
-		const float4 s = *reinterpret_cast<const float4 *>(so + c);
-		const float4 p = *reinterpret_cast<const float4 *>(&acc_s[r][part * N + c]);
-		o[c / 2] = pack_bf16x2(fmaf(p.x, fp, s.x * fs), fmaf(p.y, fp, s.y * fs));
-		o[c / 2 + 1] = pack_bf16x2(fmaf(p.z, fp, s.z * fs), fmaf(p.w, fp, s.w * fs));
+	for (int q = 0; q < 8; ++q)
+		acc[q] = acc_s[r][part * 8 + q];
+	const int t0 = a.tile_pre[seq], ts = a.tile_pre[seq + 1] - t0;
+	if (ts > 0) {
+		const long long N = hd->N, WS = hd->WS, x0 = (long long)t0 * H + (long long)h * ts;
+		const long long w0 = div_steps((x0 + 1) * WS - 1, N), w1 = div_steps((x0 + ts) * WS - 1, N);
+		const size_t slot = (size_t)seq * H + h + w0;
+		const int np = (int)(w1 - w0 + 1);
+		for (int p0 = 0; p0 < np; p0 += kFlyS) {
+			float l[kFlyS], m[kFlyS];
+			float4 o[kFlyS][2];
+#pragma unroll
+			for (int u = 0; u < kFlyS; ++u) {
+				l[u] = 0.f;
+				m[u] = -CUDART_INF_F;
+				if (p0 + u < np) {
+					const size_t at = (slot + p0 + u) * a.group + hh;
+					l[u] = __ldcg(a.xl + at);
+					m[u] = __ldcg(a.xm + at);
+					const float4 *xo = reinterpret_cast<const float4 *>(a.xo + at * D + part * 8);
+					o[u][0] = __ldcg(xo);
+					o[u][1] = __ldcg(xo + 1);
+				}
+			}
+			float mb = M;
+#pragma unroll
+			for (int u = 0; u < kFlyS; ++u)
+				if (l[u] != 0.f)
+					mb = fmaxf(mb, m[u]);
+			if (mb > M) {
+				const float f = exp2f(M - mb);
+				L *= f;
+#pragma unroll
+				for (int q = 0; q < 8; ++q)
+					acc[q] *= f;
+				M = mb;
+			}
+#pragma unroll
+			for (int u = 0; u < kFlyS; ++u)
+				if (l[u] != 0.f) {               // o of a piece without tokens counts nothing
+					const float e = exp2f(m[u] - M);
+					L = fmaf(l[u], e, L);
+#pragma unroll
+					for (int q = 0; q < 2; ++q) {
+						acc[4 * q] = fmaf(o[u][q].x, e, acc[4 * q]);
+						acc[4 * q + 1] = fmaf(o[u][q].y, e, acc[4 * q + 1]);
+						acc[4 * q + 2] = fmaf(o[u][q].z, e, acc[4 * q + 2]);
+						acc[4 * q + 3] = fmaf(o[u][q].w, e, acc[4 * q + 3]);
+					}
+				}
+		}
 	}
-	uint4 *out = reinterpret_cast<uint4 *>(static_cast<uint8_t *>(a.out) + (row * D + part * N) * 2);
-#pragma unroll
-	for (int c = 0; c < N / 8; ++c)
-		out[c] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+	const float inv = L != 0.f ? unbias / L : 0.f;    // an empty row gives zeros
+	const size_t row = (size_t)seq * a.num_heads + (size_t)h * a.group + hh;
+	*reinterpret_cast<uint4 *>(static_cast<uint8_t *>(a.out) + (row * D + part * 8) * 2) =
+	    make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
+		       pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
 }
 
 template <typename... KArgs, typename... Args>
@@ -1199,17 +1740,20 @@ cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, int block, siz
 }
 
 template <int D, int KVT>
-cudaError_t launch_prefix(const kllm_prefix_args &a, cudaStream_t st)
+cudaError_t launch_attend(const kllm_prefix_args &a, cudaStream_t st)
 {
-	// more than half an SM's shared memory, so that one CTA has the SM's TMEM
-	size_t smem = sizeof(PrefixSmem<D, KVT>) + 1024;
+	// at least half an SM's shared memory, so that one CTA has the SM's TMEM
+	size_t smem = sizeof(PrefixSmem<D, KVT>);
+	if (smem < SufLayout<D, KVT>::total)
+		smem = SufLayout<D, KVT>::total;
+	smem += 1024;
 	if (smem < 120u * 1024u)
 		smem = 120u * 1024u;
 	const cudaError_t e = cudaFuncSetAttribute(
-	    prefix_kernel<D, KVT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+	    attend_kernel<D, KVT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
 	if (e != cudaSuccess)
 		return e;
-	return launch_dependent(prefix_kernel<D, KVT>, dim3((unsigned)a.ctas), kPThreads, smem, st, 1, a);
+	return launch_dependent(attend_kernel<D, KVT>, dim3((unsigned)a.ctas), kPThreads, smem, st, 1, a);
 }
 
 }  // namespace
@@ -1219,12 +1763,15 @@ using namespace kllm;
 
 static uint64_t up256(uint64_t x) { return (x + 255u) & ~(uint64_t)255u; }
 
-extern "C" uint64_t kllm_prefix_workspace(int num_seqs, int num_heads, int head_dim, int max_blocks,
+extern "C" uint64_t kllm_prefix_workspace(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
 					  int ctas, void *base, struct kllm_prefix_args *a)
 {
 	uint8_t *p = static_cast<uint8_t *>(base);
-	const uint64_t S = (uint64_t)num_seqs, rows = S * num_heads;
-	const uint64_t part = 2u * rows + (uint64_t)kUnitRows * ctas;
+	const uint64_t S = (uint64_t)num_seqs, G = (uint64_t)(num_heads / num_kv_heads);
+	// prefix partials: two streams of a row, and a unit's rows for every CTA
+	// boundary; suffix partials: one per (sequence, kv head) and one per warp
+	const uint64_t part = 2u * S * num_heads + (uint64_t)kUnitRows * ctas;
+	const uint64_t suf = (S * num_kv_heads + (uint64_t)ctas * 16u) * G;
 	uint64_t at = 0;
 	auto take = [&](uint64_t bytes) {
 		uint8_t *q = p + at;
@@ -1232,18 +1779,19 @@ extern "C" uint64_t kllm_prefix_workspace(int num_seqs, int num_heads, int head_
 		return q;
 	};
 	uint8_t *header = take(sizeof(PHeader)), *groups = take(S * sizeof(PGroup));
-	uint8_t *rg = take(S * 4), *sl = take(S * 4), *stb = take(S * max_blocks * 24);
-	uint8_t *sm = take(rows * 4), *sll = take(rows * 4), *so = take(rows * head_dim * 4);
+	uint8_t *rg = take(S * 4), *ss = take(S * 4), *sl = take(S * 4), *tp = take((S + 1) * 4);
+	uint8_t *xm = take(suf * 4), *xl = take(suf * 4), *xo = take(suf * head_dim * 4);
 	uint8_t *pm = take(part * 4), *pl = take(part * 4), *po = take(part * head_dim * 4);
 	if (a) {
 		a->header = header;
 		a->groups = groups;
 		a->row_group = reinterpret_cast<int *>(rg);
+		a->suf_start = reinterpret_cast<int *>(ss);
 		a->suf_lens = reinterpret_cast<int *>(sl);
-		a->suf_table = stb;
-		a->sm = reinterpret_cast<float *>(sm);
-		a->sl = reinterpret_cast<float *>(sll);
-		a->so = reinterpret_cast<float *>(so);
+		a->tile_pre = reinterpret_cast<int *>(tp);
+		a->xm = reinterpret_cast<float *>(xm);
+		a->xl = reinterpret_cast<float *>(xl);
+		a->xo = reinterpret_cast<float *>(xo);
 		a->pm = reinterpret_cast<float *>(pm);
 		a->pl = reinterpret_cast<float *>(pl);
 		a->po = reinterpret_cast<float *>(po);
@@ -1251,29 +1799,24 @@ extern "C" uint64_t kllm_prefix_workspace(int num_seqs, int num_heads, int head_
 	return at;
 }
 
-extern "C" int kllm_prefix_launch(const struct kllm_prefix_args *a, void *stream)
+extern "C" int kllm_prefix_launch(struct kllm_prefix_args *a, void *stream)
 {
 	cudaStream_t st = static_cast<cudaStream_t>(stream);
-	const int wpb = kPlanThreads / 32;
-	const int row_ctas = (a->num_seqs + wpb - 1) / wpb;
-	plan_kernel<<<1 + (row_ctas < 512 ? row_ctas : 512), kPlanThreads, 0, st>>>(*a);
+	a->suf_warps = a->kv_dtype ? SW<1>::N : SW<0>::N;
+	plan_kernel<<<1, kPlanThreads, 0, st>>>(*a);
 	cudaError_t e = cudaGetLastError();
 	if (e != cudaSuccess)
 		return (int)e;
 	if (a->head_dim == 128)
-		e = a->kv_dtype ? launch_prefix<128, 1>(*a, st) : launch_prefix<128, 0>(*a, st);
+		e = a->kv_dtype ? launch_attend<128, 1>(*a, st) : launch_attend<128, 0>(*a, st);
 	else
-		e = a->kv_dtype ? launch_prefix<64, 1>(*a, st) : launch_prefix<64, 0>(*a, st);
-	return (int)e;
-}
-
-extern "C" int kllm_prefix_join_launch(const struct kllm_prefix_args *a, void *stream)
-{
-	cudaStream_t st = static_cast<cudaStream_t>(stream);
+		e = a->kv_dtype ? launch_attend<64, 1>(*a, st) : launch_attend<64, 0>(*a, st);
+	if (e != cudaSuccess)
+		return (int)e;
 	const dim3 grid((unsigned)(((long long)a->num_seqs * a->group + kJRows - 1) / kJRows),
 			(unsigned)a->num_kv_heads);
 	const float unbias = a->kv_dtype ? KLLM_MX_DEC_UNBIAS : 1.f;
 	if (a->head_dim == 128)
-		return (int)launch_dependent(join_kernel<128>, grid, kJThreads, 0, st, 1, *a, unbias);
-	return (int)launch_dependent(join_kernel<64>, grid, kJThreads, 0, st, 1, *a, unbias);
+		return (int)launch_dependent(join_kernel<128>, grid, 4 * 128, 0, st, 1, *a, unbias);
+	return (int)launch_dependent(join_kernel<64>, grid, 4 * 64, 0, st, 1, *a, unbias);
 }
