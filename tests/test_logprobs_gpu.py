@@ -212,3 +212,10 @@ def test_refusals(be):
     short = kb.LogprobsParams(struct_size=8)
     import ctypes
     assert be.lib.kllm_gpu_logprobs(be.ctx, ctypes.byref(short)) == kb.EINVAL
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_a_vocabulary_past_the_segment_table(be, bf16):
+    """More than 1,024 segments of four vectors: segments grow with the row."""
+    V = 1300007
+    check(be, normal(2, V, 21), some_targets(2, V, 3, 5), 32, bf16=bf16, shift=1)

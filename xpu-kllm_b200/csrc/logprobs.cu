@@ -11,19 +11,23 @@
 // W' = 2^-d (W - d S). Triples of threads, warps and CTAs join by the same
 // rule; then lse = (m + log2 S) ln 2 and the entropy is (log2 S - W / S) ln 2.
 //
-// Top alternatives. The row is cut into segments; the pass also leaves each
-// segment's maximum. The k-th largest of those, tau, is an element, so at
-// least k elements are >= tau and all of the k largest are; only segments
-// whose maximum reaches tau (about k of up to 1,024) hold any. A second look
-// at those segments, which are still in the L2, collects the elements >= tau,
-// and each finds its place by counting the better ones. Rows whose candidates
-// do not fit (long runs of equal logits) are selected exactly by radix.
+// Top alternatives, in the same pass. The elements fall into 32 groups by lane,
+// and each group's maximum so far is kept; the k-th largest of those, tau, is
+// an element that k elements reach, so all of the k largest are >= tau at any
+// time. A batch's elements >= tau are collected (some 30 of the first batches'
+// 16 thousand for k = 20, fewer as tau rises, a hundred or two in all), and at
+// the end those that reach the k-th largest of 32 group maxima among them are
+// ordered by counting the better ones. When too many are collected (long runs
+// of equal logits, masks of the type's lowest value) the row is read again with
+// the last tau, and selected exactly by radix if that is too many as well.
+// (Segment maxima in the pass and a second look at the best segments took 9 us
+// of 37 on 256 rows of 128,256: the second look waits behind other rows' loads.)
 //
 // A row is one thread-block cluster of 1, 2, 4 or 8 CTAs, chosen so that few
 // rows still cover the GPU; the CTAs share maxima, sums and candidates through
 // distributed shared memory, so no workspace and no atomic on global memory is
 // needed and the result does not depend on the order in which CTAs finish.
-// Bound: HBM, each logit read once (the segments looked at twice come from L2).
+// Bound: HBM, each logit read once.
 
 #include "kllm_device.cuh"
 #include "kllm_internal.h"
@@ -36,41 +40,81 @@ namespace cg = cooperative_groups;
 namespace kllm {
 namespace {
 
-constexpr int kLpThreads = 512;
-constexpr int kLpWarps = kLpThreads / 32;
-constexpr int kMaxSeg = 1024;         // segments of a row, over the cluster
-constexpr int kCandCap = 1024;        // candidates sorted by counting
+constexpr int kCandCap = 1024;        // candidates ordered by counting
 constexpr int kMaxCluster = 8;
 constexpr int kTgtMax = KLLM_MAX_TARGETS_I;
 
 struct LpSmem {
-	float wm[kLpWarps], ws[kLpWarps], ww[kLpWarps];
-	int wr[kLpWarps][kTgtMax];
+	float wm[16], ws[16], ww[16];         // per warp
+	int wr[16][kTgtMax];
 	// rank 0 of the cluster gathers here; each CTA writes its own slot
 	float cm[kMaxCluster], cs[kMaxCluster], cw[kMaxCluster];
 	int cr[kMaxCluster][kTgtMax];
-	float segmax[kMaxSeg];                // rank 0's: every segment of the row
+	uint32_t gkey[32];                    // group maxima of this CTA's part, as ordered keys
+	uint32_t all_key[32];                 // rank 0's: of the whole row
 	float cand_v[kCandCap];               // rank 0's
 	int cand_i[kCandCap];
 	int n_cand;                           // rank 0's
-	int seg_list[kMaxSeg];                // own segments to look at again
-	int n_list;
-	float merge[kLpWarps / 2][32];
+	int short_list[kCandCap];             // candidates that reach the last threshold
+	int n_short;
+	float tl[kTgtMax];                    // the targets' logits
 	float tau;
-	float fin[3];                         // lse, floor (lse, or 0 in an empty row), 1 / T
+	float sub;                            // what logprobs subtract: lse, 0 in an empty row
 	uint32_t hist[256];
 	uint32_t prefix;
-	int remain, base_gt;
-	int wcnt[2][kLpWarps];
+	int remain, base_eq;
+	int wcnt[16];
 };
+
+// Two fp32 values as one operand of the packed instructions.
+__device__ __forceinline__ uint64_t pack2(float a, float b)
+{
+	uint64_t r;
+	asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+	return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b)
+{
+	asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+	uint64_t r;
+	asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+	return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+	uint64_t r;
+	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+	return r;
+}
 
 template <int BF16>
 struct Elem;
 template <>
 struct Elem<0> {
 	static constexpr int kVec = 4;       // elements per 16 bytes
+	static constexpr int kFly = 8;       // vectors of a batch: 32 elements a lane
 	using T = float;
 	static __device__ __forceinline__ float get(const T *p) { return __ldcg(p); }
+	// elements of a batch that are > t, or >= t
+	static __device__ __forceinline__ int count(const uint4 (&raw)[kFly], float t, bool equal)
+	{
+		int n = 0;
+		if (equal) {
+#pragma unroll
+			for (int q = 0; q < kFly; ++q)
+				n += (__uint_as_float(raw[q].x) >= t) + (__uint_as_float(raw[q].y) >= t) +
+				     (__uint_as_float(raw[q].z) >= t) + (__uint_as_float(raw[q].w) >= t);
+		} else {
+#pragma unroll
+			for (int q = 0; q < kFly; ++q)
+				n += (__uint_as_float(raw[q].x) > t) + (__uint_as_float(raw[q].y) > t) +
+				     (__uint_as_float(raw[q].z) > t) + (__uint_as_float(raw[q].w) > t);
+		}
+		return n;
+	}
 	static __device__ __forceinline__ void unpack(uint4 v, float (&x)[4])
 	{
 		x[0] = __uint_as_float(v.x);
@@ -81,11 +125,28 @@ struct Elem<0> {
 };
 template <>
 struct Elem<1> {
-	static constexpr int kVec = 8;
+	static constexpr int kVec = 8, kFly = 4;
 	using T = uint16_t;
 	static __device__ __forceinline__ float get(const T *p)
 	{
 		return __uint_as_float((uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(p)) << 16);
+	}
+	// The comparisons of two elements give two bf16 ones or zeros, whose sums
+	// (at most 16 each) are exact.
+	static __device__ __forceinline__ int count(const uint4 (&raw)[kFly], float t, bool equal)
+	{
+		const __nv_bfloat162 t2 = __float2bfloat162_rn(t);       // t is a bf16 value
+		__nv_bfloat162 n = __float2bfloat162_rn(0.f);
+#pragma unroll
+		for (int q = 0; q < kFly; ++q) {
+			const uint32_t w[4] = {raw[q].x, raw[q].y, raw[q].z, raw[q].w};
+#pragma unroll
+			for (int i = 0; i < 4; ++i) {
+				const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(&w[i]);
+				n = __hadd2(n, equal ? __hge2(v, t2) : __hgt2(v, t2));
+			}
+		}
+		return (int)(__low2float(n) + __high2float(n));
 	}
 	static __device__ __forceinline__ void unpack(uint4 v, float (&x)[8])
 	{
@@ -98,22 +159,35 @@ struct Elem<1> {
 	}
 };
 
-// Elements u .. u + kVec - 1 of the row in aligned coordinates: element index
-// i = u - mis. One 16-byte load when all are inside the row, single loads of
-// those that are otherwise; the rest read as -inf.
+// Elements u .. u + kVec - 1 of the row in aligned coordinates (element index
+// i = u - mis), as 16 raw bytes: one load when all are inside the row, single
+// loads of those that are otherwise; the rest read as -inf.
 template <int BF16>
-__device__ __forceinline__ void load_vec(const typename Elem<BF16>::T *row, int mis, int V, int u,
-					 float (&x)[Elem<BF16>::kVec])
+__device__ __forceinline__ uint4 load_raw(const typename Elem<BF16>::T *row, int mis, int V, int u)
 {
 	constexpr int kVec = Elem<BF16>::kVec;
 	const int i = u - mis;
-	if (i >= 0 && i + kVec <= V) {
-		Elem<BF16>::unpack(__ldcg(reinterpret_cast<const uint4 *>(row + i)), x);
-	} else {
+	if (i >= 0 && i + kVec <= V)
+		return __ldcg(reinterpret_cast<const uint4 *>(row + i));
+	uint32_t w[4];
 #pragma unroll
-		for (int q = 0; q < kVec; ++q)
-			x[q] = (i + q >= 0 && i + q < V) ? Elem<BF16>::get(row + i + q) : -CUDART_INF_F;
+	for (int q = 0; q < 4; ++q) {
+		if constexpr (BF16) {
+			uint32_t h[2];
+#pragma unroll
+			for (int z = 0; z < 2; ++z) {
+				const int j = i + 2 * q + z;
+				h[z] = (j >= 0 && j < V)
+				    ? (uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(row + j)) : 0xFF80u;
+			}
+			w[q] = h[0] | (h[1] << 16);
+		} else {
+			const int j = i + q;
+			w[q] = (j >= 0 && j < V) ? __float_as_uint(__ldcg(reinterpret_cast<const float *>(row) + j))
+						 : 0xFF800000u;
+		}
 	}
+	return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // The order of the top list and of ranks: value descending, NaN as -inf.
@@ -126,19 +200,11 @@ __device__ __forceinline__ uint32_t order_bits(float l)
 	return key_of(order_val(l));
 }
 
-__device__ __forceinline__ float warp_max(float x)
-{
-#pragma unroll
-	for (int o = 16; o; o >>= 1)
-		x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-	return x;
-}
-
 // Exact selection by one CTA over the whole row: the k-th largest order key by
 // four 8-bit radix passes, then the elements above it and the first of its
 // equals in index order. Leaves k candidates. Rare: runs of equal logits.
-template <int BF16>
-__device__ void radix_candidates(const typename Elem<BF16>::T *row, int V, int k, LpSmem &sm)
+template <int BF16, int TH>
+__device__ __noinline__ void radix_candidates(const typename Elem<BF16>::T *row, int V, int k, LpSmem &sm)
 {
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	if (tid == 0) {
@@ -149,11 +215,11 @@ __device__ void radix_candidates(const typename Elem<BF16>::T *row, int V, int k
 	for (int pass = 0; pass < 4; ++pass) {
 		const int shift = 24 - 8 * pass;
 		const uint32_t mask = pass ? 0xFFFFFFFFu << (32 - 8 * pass) : 0u;
-		for (int i = tid; i < 256; i += kLpThreads)
+		for (int i = tid; i < 256; i += TH)
 			sm.hist[i] = 0u;
 		__syncthreads();
 		const uint32_t prefix = sm.prefix;
-		for (int base = 0; base < V; base += kLpThreads) {
+		for (int base = 0; base < V; base += TH) {
 			const int i = base + tid;
 			const uint32_t key = i < V ? order_bits(Elem<BF16>::get(row + i)) : 0u;
 			const bool hit = i < V && (key & mask) == prefix;
@@ -179,11 +245,11 @@ __device__ void radix_candidates(const typename Elem<BF16>::T *row, int V, int k
 	const int need_eq = sm.remain, n_gt = k - need_eq;
 	if (tid == 0) {
 		sm.n_cand = 0;
-		sm.base_gt = 0;               // equals taken so far
+		sm.base_eq = 0;               // equals taken so far
 	}
 	__syncthreads();
 	// in index order, 512 elements at a time: equals keep their order
-	for (int base = 0; base < V; base += kLpThreads) {
+	for (int base = 0; base < V; base += TH) {
 		const int i = base + tid;
 		const float l = i < V ? Elem<BF16>::get(row + i) : 0.f;
 		const uint32_t key = i < V ? order_bits(l) : 0u;
@@ -195,14 +261,14 @@ __device__ void radix_candidates(const typename Elem<BF16>::T *row, int V, int k
 		}
 		const unsigned be = __ballot_sync(0xffffffffu, eq);
 		if (lane == 0)
-			sm.wcnt[0][warp] = __popc(be);
+			sm.wcnt[warp] = __popc(be);
 		__syncthreads();
-		int before = sm.base_gt, all = 0;
+		int before = sm.base_eq, all = 0;
 #pragma unroll
-		for (int w = 0; w < kLpWarps; ++w) {
+		for (int w = 0; w < (TH / 32); ++w) {
 			if (w < warp)
-				before += sm.wcnt[0][w];
-			all += sm.wcnt[0][w];
+				before += sm.wcnt[w];
+			all += sm.wcnt[w];
 		}
 		const int at = before + __popc(be & ((1u << lane) - 1u));
 		if (eq && at < need_eq) {
@@ -211,9 +277,9 @@ __device__ void radix_candidates(const typename Elem<BF16>::T *row, int V, int k
 		}
 		__syncthreads();
 		if (tid == 0)
-			sm.base_gt += all;
+			sm.base_eq += all;
 		__syncthreads();
-		if (sm.base_gt >= need_eq && sm.n_cand >= n_gt)
+		if (sm.base_eq >= need_eq && sm.n_cand >= n_gt)
 			break;
 	}
 	if (tid == 0)
@@ -221,13 +287,51 @@ __device__ void radix_candidates(const typename Elem<BF16>::T *row, int V, int k
 	__syncthreads();
 }
 
-// NT: targets counted in the pass (0, 1, or up to kTgtMax).
-template <int BF16, int NT>
-__global__ void __launch_bounds__(kLpThreads, 2)
-logprobs_kernel(const kllm_logprobs_args a, int seg_len)
+// The k-th largest of 32 group maxima (every lane gets it).
+__device__ __forceinline__ float group_tau(const uint32_t *gkey, int k, int lane)
+{
+	const uint32_t key = *reinterpret_cast<const volatile uint32_t *>(gkey + lane);
+	const float top = warp_sort_desc(key ? value_of(key) : -CUDART_INF_F, lane);
+	return __shfl_sync(0xffffffffu, top, k - 1);
+}
+
+// Too many candidates: the row once more, by one CTA, with the tau of all its
+// elements; radix selection when that leaves too many as well.
+template <int BF16, int TH>
+__device__ __noinline__ void recollect(const typename Elem<BF16>::T *row, int V, int mis, int k, LpSmem &sm)
 {
 	constexpr int kVec = Elem<BF16>::kVec;
+	__syncthreads();
+	const float tau = group_tau(sm.all_key, k, threadIdx.x & 31);
+	if (threadIdx.x == 0)
+		sm.n_cand = 0;
+	__syncthreads();
+	for (int u = threadIdx.x * kVec; u < V + mis; u += TH * kVec) {
+		float x[kVec];
+		Elem<BF16>::unpack(load_raw<BF16>(row, mis, V, u), x);
+#pragma unroll
+		for (int z = 0; z < kVec; ++z)
+			if (x[z] >= tau && x[z] > -CUDART_INF_F) {
+				const int at = atomicAdd(&sm.n_cand, 1);
+				if (at < kCandCap) {
+					sm.cand_v[at] = x[z];
+					sm.cand_i[at] = u - mis + z;
+				}
+			}
+	}
+	__syncthreads();
+	if (sm.n_cand > kCandCap)
+		radix_candidates<BF16, TH>(row, V, k, sm);
+}
+
+// NT: targets counted in the pass (0, 1, up to 4, up to kTgtMax). TH threads.
+template <int BF16, int NT, int TH>
+__global__ void __launch_bounds__(TH, 1024 / TH)
+logprobs_kernel(const kllm_logprobs_args a)
+{
+	constexpr int kVec = Elem<BF16>::kVec, kFly = Elem<BF16>::kFly, kWarps = TH / 32;
 	constexpr int kStep = 32 * kVec;              // elements a warp loads at once
+	constexpr int kBatch = kFly * kStep;          // elements of a batch of loads
 	using T = typename Elem<BF16>::T;
 	__shared__ LpSmem sm;
 	cg::cluster_group cl = cg::this_cluster();
@@ -238,15 +342,25 @@ logprobs_kernel(const kllm_logprobs_args a, int seg_len)
 	const T *row = static_cast<const T *>(a.logits) + (long long)r * a.row_stride;
 	const int mis = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
 	const int U = V + mis;
-	const int n_seg = (U + seg_len - 1) / seg_len;
 	LpSmem *lead = cl.map_shared_rank(&sm, 0);
-
+	if (tid < 32)
+		sm.gkey[tid] = sm.all_key[tid] = 0u;  // below every number's key
+	if (tid == 0)
+		sm.n_cand = sm.n_short = 0;
+	// every CTA of the cluster runs, its memory set, before another writes to it
 	if (CL > 1)
-		cl.sync();                  // every CTA of the cluster runs before its memory is written
+		cl.sync();
+	else
+		__syncthreads();
+
+	const int stride = CL * kWarps * kBatch, b0 = (rank * kWarps + warp) * kBatch;
 	const float temp = a.temperature ? a.temperature[r] : 1.f;
 	const float inv_t = temp > 0.f ? 1.f / temp : 1.f;
 	const float c = kLog2e * inv_t;
 
+	// A target counts the elements above it, and its equals at lower indices: >=
+	// in the batches before the one it lies in, > in those after it, and one by
+	// one in that one.
 	constexpr int NTA = NT > 0 ? NT : 1;
 	float tl[NTA];
 	int ti[NTA], cnt[NTA];
@@ -257,50 +371,112 @@ logprobs_kernel(const kllm_logprobs_args a, int seg_len)
 			ti[j] = (t >= 0 && t < V) ? t : -1;
 			tl[j] = ti[j] >= 0 ? Elem<BF16>::get(row + ti[j]) : CUDART_INF_F;
 			cnt[j] = 0;
+			if (tid == 0)
+				sm.tl[j] = tl[j];
 		}
 	}
 
 	// ---- one pass: this thread's (m, S, W), ranks, segment maxima --------------
-	float m = -CUDART_INF_F, S = 0.f, W = 0.f;
-	for (int sg = rank * kLpWarps + warp; sg < n_seg; sg += CL * kLpWarps) {
-		float smax = -CUDART_INF_F;
-		for (int u0 = sg * seg_len; u0 < min((sg + 1) * seg_len, U); u0 += kStep) {
-			float x[kVec];
-			const int u = u0 + lane * kVec;
-			load_vec<BF16>(row, mis, V, u, x);
-			float bm = x[0];
+	// A batch at a time: one maximum, one look at the reference and one at each
+	// target's place for its 32 elements (a vector at a time these took 35
+	// instructions an element, and the pass was bound by them). Its loads are in
+	// flight together; the 32 warps of an SM hide each other's.
+	float m = -CUDART_INF_F, S = 0.f, W = 0.f, tau = -CUDART_INF_F;
+#pragma unroll 1
+	for (int it = 0, here = b0; it == 0 || here < U; ++it, here += stride) {
+		float x[kFly][kVec];
+		uint4 raw[kFly];
+		if (here >= mis && here + kBatch <= U) {               // the same for the whole warp
+			const uint4 *p = reinterpret_cast<const uint4 *>(row + (here - mis)) + lane;
 #pragma unroll
-			for (int q = 1; q < kVec; ++q)
-				bm = fmaxf(bm, x[q]);
-			smax = fmaxf(smax, bm);
-			const float ym = bm * c;
-			if (ym > m) {
-				if (m > -CUDART_INF_F) {
-					const float d = ym - m, f = ex2_approx(-d);
-					W = f * fmaf(-d, S, W);
-					S *= f;
-				}
-				m = ym;
+			for (int q = 0; q < kFly; ++q)
+				raw[q] = __ldcg(p + q * 32);
+		} else {
+#pragma unroll
+			for (int q = 0; q < kFly; ++q)
+				raw[q] = load_raw<BF16>(row, mis, V, here + q * kStep + lane * kVec);
+		}                                                      // past the end: all -inf
+#pragma unroll
+		for (int q = 0; q < kFly; ++q)
+			Elem<BF16>::unpack(raw[q], x[q]);
+		float vm[kFly], bm = -CUDART_INF_F;        // maxima of the vectors, of all
+#pragma unroll
+		for (int q = 0; q < kFly; ++q) {
+			vm[q] = x[q][0];
+#pragma unroll
+			for (int z = 1; z < kVec; ++z)
+				vm[q] = fmaxf(vm[q], x[q][z]);
+			bm = fmaxf(bm, vm[q]);
+		}
+		const float ym = bm * c;
+		if (ym > m) {
+			if (m > -CUDART_INF_F) {
+				const float d = ym - m, f = ex2_approx(-d);
+				W = f * fmaf(-d, S, W);
+				S *= f;
 			}
-			const float ref = m == -CUDART_INF_F ? 0.f : m;
+			m = ym;
+		}
+		const float ref = m == -CUDART_INF_F ? 0.f : m;
+		// two elements an instruction where the hardware has it
+		const uint64_t c2 = pack2(c, c), r2 = pack2(-ref, -ref);
+		uint64_t s2 = 0ull, w2 = 0ull;
 #pragma unroll
-			for (int q = 0; q < kVec; ++q) {
-				const float d = fmaf(x[q], c, -ref);
-				const float e = ex2_approx(d);
-				S += e;
-				W = fmaf(e, fmaxf(d, -1000.f), W);      // 0 x -inf counts 0
-				if constexpr (NT > 0) {
+		for (int q = 0; q < kFly; ++q)
 #pragma unroll
-					for (int j = 0; j < NT; ++j)
-						cnt[j] += (x[q] > tl[j] ||
-							   (x[q] == tl[j] && u - mis + q < ti[j])) ? 1 : 0;
-				}
+			for (int z = 0; z < kVec; z += 2) {
+				float d0, d1;
+				unpack2(fma2(pack2(x[q][z], x[q][z + 1]), c2, r2), d0, d1);
+				const uint64_t e2 = pack2(ex2_approx(d0), ex2_approx(d1));
+				s2 = add2(s2, e2);
+				w2 = fma2(e2, pack2(fmaxf(d0, -1000.f), fmaxf(d1, -1000.f)), w2);  // 0 x -inf counts 0
 			}
+		float sa, sb, wa, wb;
+		unpack2(s2, sa, sb);
+		unpack2(w2, wa, wb);
+		S += sa + sb;
+		W += wa + wb;
+		if constexpr (NT > 0) {
+#pragma unroll
+			for (int j = 0; j < NT; ++j)
+				if (j < nt) {
+					const int rel = ti[j] + mis - here;        // place in the batch
+					const float t = tl[j];
+					if (rel >= kBatch)                         // the same for the whole warp
+						cnt[j] += Elem<BF16>::count(raw, t, true);
+					else if (rel < 0)
+						cnt[j] += Elem<BF16>::count(raw, t, false);
+					else {
+#pragma unroll
+						for (int q = 0; q < kFly; ++q)
+#pragma unroll
+							for (int z = 0; z < kVec; ++z)
+								cnt[j] += (int)(x[q][z] > t) |
+									  ((int)(x[q][z] == t) &
+									   (int)(q * kStep + lane * kVec + z < rel));
+					}
+				}
 		}
 		if (k > 0) {
-			smax = warp_max(smax);
-			if (lane == 0)
-				lead->segmax[sg] = smax;
+			atomicMax(&sm.gkey[lane], key_of(bm));
+			if (it == 0)
+				__syncthreads();          // all warps' first batches are in the groups
+			if ((it & (it + 1)) == 0)         // after 1, 2, 4, 8 .. batches
+				tau = group_tau(sm.gkey, k, lane);
+			if (__any_sync(0xffffffffu, bm >= tau && bm > -CUDART_INF_F)) {
+#pragma unroll
+				for (int q = 0; q < kFly; ++q)
+					if (vm[q] >= tau && vm[q] > -CUDART_INF_F)
+#pragma unroll
+						for (int z = 0; z < kVec; ++z)
+							if (x[q][z] >= tau && x[q][z] > -CUDART_INF_F) {
+								const int at = atomicAdd(&lead->n_cand, 1);
+								if (at < kCandCap) {
+									lead->cand_v[at] = x[q][z];
+									lead->cand_i[at] = here + q * kStep + lane * kVec + z - mis;
+								}
+							}
+			}
 		}
 	}
 
@@ -311,11 +487,11 @@ logprobs_kernel(const kllm_logprobs_args a, int seg_len)
 		const float s2 = __shfl_xor_sync(0xffffffffu, S, o);
 		const float w2 = __shfl_xor_sync(0xffffffffu, W, o);
 		join(m, S, W, m2, s2, w2);
-		if constexpr (NT > 0) {
+	}
+	if constexpr (NT > 0) {
 #pragma unroll
-			for (int j = 0; j < NT; ++j)
-				cnt[j] += __shfl_xor_sync(0xffffffffu, cnt[j], o);
-		}
+		for (int j = 0; j < NT; ++j)
+			cnt[j] = __reduce_add_sync(0xffffffffu, cnt[j]);
 	}
 	if (lane == 0) {
 		sm.wm[warp] = m;
@@ -327,126 +503,100 @@ logprobs_kernel(const kllm_logprobs_args a, int seg_len)
 				sm.wr[warp][j] = cnt[j];
 		}
 	}
-	if (tid == 0)
-		sm.n_list = sm.n_cand = 0;
 	__syncthreads();
-	if (tid == 0) {
-		float M = sm.wm[0], s = sm.ws[0], w = sm.ww[0];
-#pragma unroll 1
-		for (int i = 1; i < kLpWarps; ++i)
-			join(M, s, w, sm.wm[i], sm.ws[i], sm.ww[i]);
-		lead->cm[rank] = M;
-		lead->cs[rank] = s;
-		lead->cw[rank] = w;
-	}
-	if constexpr (NT > 0) {
-		if (tid < NT) {
-			int n = 0;
-#pragma unroll 1
-			for (int i = 0; i < kLpWarps; ++i)
-				n += sm.wr[i][tid];
-			lead->cr[rank][tid] = n;
+	if (warp == 0) {
+		float M = -CUDART_INF_F, s = 0.f, w = 0.f;
+		if (lane < kWarps) {
+			M = sm.wm[lane];
+			s = sm.ws[lane];
+			w = sm.ww[lane];
+		}
+#pragma unroll
+		for (int o = kWarps / 2; o; o >>= 1) {
+			const float m2 = __shfl_xor_sync(0xffffffffu, M, o);
+			const float s2 = __shfl_xor_sync(0xffffffffu, s, o);
+			const float w2 = __shfl_xor_sync(0xffffffffu, w, o);
+			join(M, s, w, m2, s2, w2);
+		}
+		if (k > 0)
+			atomicMax(&lead->all_key[lane], sm.gkey[lane]);
+		if (lane == 0) {
+			lead->cm[rank] = M;
+			lead->cs[rank] = s;
+			lead->cw[rank] = w;
+		}
+		if constexpr (NT > 0) {
+			if (lane < NT) {
+				int n = 0;
+#pragma unroll
+				for (int i = 0; i < kWarps; ++i)
+					n += sm.wr[i][lane];
+				lead->cr[rank][lane] = n;
+			}
 		}
 	}
-	cl.sync();
+	if (CL > 1)
+		cl.sync();
+	else
+		__syncthreads();
 
-	// ---- rank 0: the row's numbers, and tau -------------------------------------------
-	if (rank == 0) {
-		if (tid == 0) {
-			float M = sm.cm[0], s = sm.cs[0], w = sm.cw[0];
-			for (int i = 1; i < CL; ++i)
-				join(M, s, w, sm.cm[i], sm.cs[i], sm.cw[i]);
-			const float l2 = log2f(s);
-			const bool dead = M == -CUDART_INF_F && s == 0.f;
-			const float lse = dead ? -CUDART_INF_F : (M + l2) * kLn2;
-			sm.fin[0] = lse;
-			sm.fin[1] = dead ? 0.f : lse;
+	// ---- rank 0: the row's numbers ------------------------------------------------------
+	if (rank != 0)
+		return;
+	if (warp == 0) {
+		float M = -CUDART_INF_F, s = 0.f, w = 0.f;
+		if (lane < CL) {
+			M = sm.cm[lane];
+			s = sm.cs[lane];
+			w = sm.cw[lane];
+		}
+#pragma unroll
+		for (int o = kMaxCluster / 2; o; o >>= 1) {
+			const float m2 = __shfl_xor_sync(0xffffffffu, M, o);
+			const float s2 = __shfl_xor_sync(0xffffffffu, s, o);
+			const float w2 = __shfl_xor_sync(0xffffffffu, w, o);
+			join(M, s, w, m2, s2, w2);
+		}
+		const float l2 = log2f(s);
+		const bool dead = M == -CUDART_INF_F && s == 0.f;
+		const float lse = dead ? -CUDART_INF_F : (M + l2) * kLn2;
+		const float sub = dead ? 0.f : lse;
+		if (lane == 0) {
+			sm.sub = sub;
 			if (a.lse)
 				a.lse[r] = lse;
 			if (a.entropy)
 				a.entropy[r] = dead ? 0.f : (l2 - w / s) * kLn2;
-			sm.tau = -CUDART_INF_F;
 		}
-		__syncthreads();
 		if constexpr (NT > 0) {
-			if (tid < nt) {
-				const int t = a.targets[(size_t)r * nt + tid];
+			if (lane < nt) {
+				const int t = a.targets[(size_t)r * nt + lane];
 				const bool in = t >= 0 && t < V;
-				const float l = in ? Elem<BF16>::get(row + t) : -CUDART_INF_F;
-				a.target_lp[(size_t)r * nt + tid] = in ? l * inv_t - sm.fin[1] : -CUDART_INF_F;
+				const float l = in ? sm.tl[lane] : -CUDART_INF_F;
+				a.target_lp[(size_t)r * nt + lane] = in ? l * inv_t - sub : -CUDART_INF_F;
 				if (a.target_rank) {
 					int n = 0;
 					for (int i = 0; i < CL; ++i)
-						n += sm.cr[i][tid];
+						n += sm.cr[i][lane];
 					if (l == -CUDART_INF_F)
-						n -= mis;       // the padding before the row read as -inf
-					a.target_rank[(size_t)r * nt + tid] = in && l == l ? n : -1;
+						n -= mis;               // the padding before the row read as -inf
+					a.target_rank[(size_t)r * nt + lane] = in && l == l ? n : -1;
 				}
 			}
-		}
-		// the k-th largest segment maximum: each warp sorts its share, then the
-		// warps' 32 largest are merged pair by pair
-		if (k > 0 && k <= n_seg) {
-			float top = -CUDART_INF_F;
-			for (int i = tid; i - lane < n_seg; i += kLpThreads) {
-				const float x = warp_sort_desc(i < n_seg ? sm.segmax[i] : -CUDART_INF_F, lane);
-				top = i == tid ? x : warp_merge_desc(top, x, lane);
-			}
-			for (int half = kLpWarps / 2; half; half >>= 1) {
-				if (warp >= half && warp < 2 * half)
-					sm.merge[warp - half][lane] = top;
-				__syncthreads();
-				if (warp < half)
-					top = warp_merge_desc(top, sm.merge[warp][lane], lane);
-				__syncthreads();
-			}
-			if (warp == 0 && lane == k - 1)
-				sm.tau = top;
 		}
 	}
 	if (k == 0)
 		return;
-	cl.sync();
 
-	// ---- candidates: every element >= tau (above -inf when that is all tau says) --------
-	const float tau = lead->tau;
-	for (int sg = tid; sg < n_seg; sg += kLpThreads) {
-		if (sg % (CL * kLpWarps) / kLpWarps != rank)
-			continue;
-		const float v = lead->segmax[sg];
-		if (v >= tau && v > -CUDART_INF_F)
-			sm.seg_list[atomicAdd(&sm.n_list, 1)] = sg;
-	}
-	__syncthreads();
-	const int n_list = sm.n_list;
-	for (int li = warp; li < n_list; li += kLpWarps) {
-		const int sg = sm.seg_list[li];
-		for (int u0 = sg * seg_len; u0 < min((sg + 1) * seg_len, U); u0 += kStep) {
-			float x[kVec];
-			const int u = u0 + lane * kVec;
-			load_vec<BF16>(row, mis, V, u, x);
-#pragma unroll
-			for (int q = 0; q < kVec; ++q)
-				if (x[q] >= tau && x[q] > -CUDART_INF_F) {
-					const int at = atomicAdd(&lead->n_cand, 1);
-					if (at < kCandCap) {
-						lead->cand_v[at] = x[q];
-						lead->cand_i[at] = u - mis + q;
-					}
-				}
-		}
-	}
-	cl.sync();
-	if (rank != 0)
-		return;
-	if (sm.n_cand > kCandCap)
-		radix_candidates<BF16>(row, V, k, sm);
+	// ---- the k largest of the candidates -------------------------------------------------
+	if (sm.n_cand > kCandCap)                           // the same for every thread
+		recollect<BF16, TH>(row, V, mis, k, sm);
 	int n = sm.n_cand;
-	__syncthreads();
 	if (n < k) {
 		// fewer than k elements above -inf: the rest are -inf (or NaN), lowest
 		// index first; the first k elements hold enough of them
-		if (warp == 0) {
+		__syncthreads();
+		if (warp == 1) {
 			const bool low = lane < k && order_val(Elem<BF16>::get(row + min(lane, V - 1))) ==
 							 -CUDART_INF_F;
 			const unsigned b = __ballot_sync(0xffffffffu, low);
@@ -456,30 +606,47 @@ logprobs_kernel(const kllm_logprobs_args a, int seg_len)
 				sm.cand_i[at] = lane;
 			}
 		}
-		__syncthreads();
 		n = k;
 	}
-	for (int i = tid; i < n; i += kLpThreads) {
-		const float v = sm.cand_v[i];
-		const int id = sm.cand_i[i];
+	__syncthreads();                                    // and sm.sub is set
+	if (warp == 0) {
+		float top = -CUDART_INF_F;
+		for (int i = lane; i < n; i += 32)
+			top = fmaxf(top, sm.cand_v[i]);
+		top = warp_sort_desc(top, lane);
+		if (lane == k - 1)
+			sm.tau = top;
+	}
+	__syncthreads();
+	const float last = sm.tau;
+	for (int i = tid; i < n; i += TH)
+		if (sm.cand_v[i] >= last)
+			sm.short_list[atomicAdd(&sm.n_short, 1)] = i;
+	__syncthreads();
+	const int ns = sm.n_short;
+	for (int i = tid; i < ns; i += TH) {
+		const int me = sm.short_list[i], id = sm.cand_i[me];
+		const float v = sm.cand_v[me];
 		int at = 0;
-		for (int j = 0; j < n; ++j) {
-			const float o = sm.cand_v[j];
-			at += (o > v || (o == v && sm.cand_i[j] < id)) ? 1 : 0;
+#pragma unroll 4
+		for (int j = 0; j < ns; ++j) {
+			const int other = sm.short_list[j];
+			const float o = sm.cand_v[other];
+			at += (int)(o > v) | ((int)(o == v) & (int)(sm.cand_i[other] < id));
 		}
 		if (at < k) {
 			a.top_ids[(size_t)r * k + at] = id;
-			a.top_lp[(size_t)r * k + at] = v * inv_t - sm.fin[1];
+			a.top_lp[(size_t)r * k + at] = v * inv_t - sm.sub;
 		}
 	}
 }
 
-template <int BF16, int NT>
-cudaError_t launch_lp(const kllm_logprobs_args &a, int cluster, int seg_len, cudaStream_t st)
+template <int BF16, int NT, int TH>
+cudaError_t launch_lp(const kllm_logprobs_args &a, int cluster, cudaStream_t st)
 {
 	cudaLaunchConfig_t cfg = {};
 	cfg.gridDim = dim3((unsigned)a.num_rows * (unsigned)cluster);
-	cfg.blockDim = dim3(kLpThreads);
+	cfg.blockDim = dim3(TH);
 	cfg.stream = st;
 	cudaLaunchAttribute at[1];
 	at[0].id = cudaLaunchAttributeClusterDimension;
@@ -488,7 +655,23 @@ cudaError_t launch_lp(const kllm_logprobs_args &a, int cluster, int seg_len, cud
 	at[0].val.clusterDim.z = 1;
 	cfg.attrs = at;
 	cfg.numAttrs = 1;
-	return cudaLaunchKernelEx(&cfg, logprobs_kernel<BF16, NT>, a, seg_len);
+	return cudaLaunchKernelEx(&cfg, logprobs_kernel<BF16, NT, TH>, a);
+}
+
+template <int BF16, int NT>
+cudaError_t launch_nt(const kllm_logprobs_args &a, int num_sms, cudaStream_t st)
+{
+	// A row ends in a chain of a microsecond or two that loads nothing. Long rows
+	// take 512 threads; short ones 128, so that eight share an SM and one row's
+	// end runs under the others' loads.
+	const bool wide = a.vocab >= 65536;
+	const int th = wide ? 512 : 128, batch = 32 * Elem<BF16>::kVec * Elem<BF16>::kFly;
+	// CTAs per row: enough to half fill the SMs, none without half a batch a warp
+	int cluster = 1;
+	while (cluster < kMaxCluster && (long long)a.num_rows * cluster * th < 512ll * num_sms &&
+	       a.vocab / (cluster * 2) >= th / 32 * batch / 2)
+		cluster *= 2;
+	return wide ? launch_lp<BF16, NT, 512>(a, cluster, st) : launch_lp<BF16, NT, 128>(a, cluster, st);
 }
 
 }  // namespace
@@ -499,24 +682,14 @@ using namespace kllm;
 extern "C" int kllm_logprobs_launch(const struct kllm_logprobs_args *a, int num_sms, void *stream)
 {
 	cudaStream_t st = static_cast<cudaStream_t>(stream);
-	// segments of 256 elements, longer ones when the vocabulary has more than 1,024
-	int seg_len = 256;
-	while ((a->vocab + 7 + seg_len - 1) / seg_len > kMaxSeg)
-		seg_len *= 2;
-	// CTAs per row: enough for two CTAs on every SM, none with under 4,096 elements
-	int cluster = 1;
-	while (cluster < kMaxCluster && (long long)a->num_rows * cluster < 2ll * num_sms &&
-	       a->vocab / (cluster * 2) >= 4096)
-		cluster *= 2;
 	const int nt = a->num_targets;
-	cudaError_t e;
 	if (a->bf16)
-		e = nt == 0 ? launch_lp<1, 0>(*a, cluster, seg_len, st)
-			    : nt == 1 ? launch_lp<1, 1>(*a, cluster, seg_len, st)
-				      : launch_lp<1, kTgtMax>(*a, cluster, seg_len, st);
-	else
-		e = nt == 0 ? launch_lp<0, 0>(*a, cluster, seg_len, st)
-			    : nt == 1 ? launch_lp<0, 1>(*a, cluster, seg_len, st)
-				      : launch_lp<0, kTgtMax>(*a, cluster, seg_len, st);
-	return (int)e;
+		return (int)(nt == 0 ? launch_nt<1, 0>(*a, num_sms, st)
+			     : nt == 1 ? launch_nt<1, 1>(*a, num_sms, st)
+			     : nt <= 4 ? launch_nt<1, 4>(*a, num_sms, st)
+				       : launch_nt<1, kTgtMax>(*a, num_sms, st));
+	return (int)(nt == 0 ? launch_nt<0, 0>(*a, num_sms, st)
+		     : nt == 1 ? launch_nt<0, 1>(*a, num_sms, st)
+		     : nt <= 4 ? launch_nt<0, 4>(*a, num_sms, st)
+			       : launch_nt<0, kTgtMax>(*a, num_sms, st));
 }
