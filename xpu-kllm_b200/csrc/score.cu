@@ -91,14 +91,21 @@ __device__ __forceinline__ int unit_at(int s, int q, int units)
 // kSlack of them, or exactly k when equal keys leave no such cut (the lowest
 // indices of the equals stay). tau becomes a value that k kept entries reach,
 // so a later logit has to be larger to matter. Called by whole warps; a lane
-// with n < k keeps its list.
-__device__ __forceinline__ void cut_list(uint32_t (*lk)[kSR], int (*li)[kSR], int t, int k, int &n,
-					 float &tau)
+// with n < k keeps its list. The list is held in registers: counting in shared
+// memory, an entry at a time, took 15k cycles a cut.
+__device__ __noinline__ void cut_list(uint32_t (*lk)[kSR], int (*li)[kSR], int t, int k, int &n,
+				      float &tau)
 {
+	uint32_t key[kListCap];
 	uint32_t lo = 0xffffffffu, hi = 0u;
-	for (int e = 0; e < n; ++e) {
-		lo = min(lo, lk[e][t]);
-		hi = max(hi, lk[e][t]);
+#pragma unroll
+	for (int e = 0; e < kListCap; ++e) {
+		key[e] = lk[e][t];
+		if (e >= n)
+			key[e] = 0u;                       // below every number's key
+		else
+			lo = min(lo, key[e]);
+		hi = max(hi, key[e]);
 	}
 	// count(>= lo) >= k and count(>= hi) < k throughout: ends early on a count
 	// of at most k + kSlack, else with hi = lo + 1, lo the k-th largest key
@@ -108,19 +115,19 @@ __device__ __forceinline__ void cut_list(uint32_t (*lk)[kSR], int (*li)[kSR], in
 	int budget = kListCap;                     // of entries equal to lo
 	while (!__all_sync(0xffffffffu, done)) {
 		const uint32_t mid = lo + ((hi - lo) >> 1);
-		int c = 0;
-		for (int e = 0; e < n; ++e)
-			c += lk[e][t] >= mid ? 1 : 0;
+		int c[2] = {0, 0}, above[2] = {0, 0};
+#pragma unroll
+		for (int e = 0; e < kListCap; ++e) {
+			c[e & 1] += key[e] >= mid ? 1 : 0;
+			above[e & 1] += key[e] > lo ? 1 : 0;
+		}
 		if (!done) {
 			if (mid == lo) {
-				int above = 0;
-				for (int e = 0; e < n; ++e)
-					above += lk[e][t] > lo ? 1 : 0;
-				budget = k - above;
+				budget = k - (above[0] + above[1]);
 				done = true;
-			} else if (c >= k) {
+			} else if (c[0] + c[1] >= k) {
 				lo = mid;
-				done = c <= k + kSlack;
+				done = c[0] + c[1] <= k + kSlack;
 			} else {
 				hi = mid;
 			}
@@ -128,15 +135,18 @@ __device__ __forceinline__ void cut_list(uint32_t (*lk)[kSR], int (*li)[kSR], in
 	}
 	if (!work)
 		return;
+	int id[kListCap];
+#pragma unroll
+	for (int e = 0; e < kListCap; ++e)
+		id[e] = li[e][t];
 	int w = 0;
-	for (int e = 0; e < n; ++e) {
-		const uint32_t key = lk[e][t];
-		const int id = li[e][t];
-		const bool eq = key == lo;
-		if (key > lo || (eq && budget > 0)) {
+#pragma unroll
+	for (int e = 0; e < kListCap; ++e) {
+		const bool eq = key[e] == lo;
+		if (key[e] > lo || (eq && budget > 0)) {
 			budget -= eq ? 1 : 0;
-			lk[w][t] = key;
-			li[w][t] = id;
+			lk[w][t] = key[e];
+			li[w][t] = id[e];
 			++w;
 		}
 	}
@@ -313,19 +323,48 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 					break;
 				}
 				tc_fence_after();
-#pragma unroll 1
-				for (int ch = 0; ch < nc; ++ch) {
-					float v[32];
-					tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kSN + ch * 32), v);
+				const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * kSN);
+				// 32 columns of the row; those past the vocabulary read as -inf
+				auto columns = [&](int ch, float (&v)[32]) {
+					tmem_ld32(acc + (uint32_t)(ch * 32), v);
 					const int nb = u * kSU + ch * 32;
-					if (nb >= V)
-						break;                 // zero columns past the vocabulary
 					if (nb + 32 > V) {
 #pragma unroll
 						for (int i = 0; i < 32; ++i)
 							if (nb + i >= V)
 								v[i] = -CUDART_INF_F;
 					}
+				};
+				if (u == u0 && k > 0 && 4 * nc >= k) {
+					// A range's first threshold: the k-th largest of its first tile's
+					// maxima over 8 columns (the list holds them meanwhile). From -inf
+					// the first tile alone would need several cuts.
+#pragma unroll 1
+					for (int ch = 0; ch < nc; ++ch) {
+						float v[32];
+						columns(ch, v);
+#pragma unroll
+						for (int g = 0; g < 4; ++g) {
+							float gm = v[8 * g];
+#pragma unroll
+							for (int i = 1; i < 8; ++i)
+								gm = fmaxf(gm, v[8 * g + i]);
+							sm.list_k[4 * ch + g][t] = key_of(gm == gm ? gm : -CUDART_INF_F);
+						}
+					}
+					n = 4 * nc;
+					cut_list(sm.list_k, sm.list_i, t, k, n, tau);
+					n = 0;
+					if (tau > -CUDART_INF_F)                 // its equals are wanted
+						tau = value_of(key_of(tau) - 1u);
+				}
+#pragma unroll 1
+				for (int ch = 0; ch < nc; ++ch) {
+					float v[32];
+					const int nb = u * kSU + ch * 32;
+					if (nb >= V)
+						break;                 // nothing but padding
+					columns(ch, v);
 					float cm = v[0];
 #pragma unroll
 					for (int i = 1; i < 32; ++i)
@@ -418,17 +457,21 @@ __global__ void __launch_bounds__(kJoinThreads)
 score_join_kernel(const kllm_score_args a)
 {
 	extern __shared__ __align__(8) uint8_t join_raw[];
-	float *cv = reinterpret_cast<float *>(join_raw);               // [splits * (top_n + kSlack)]
-	int *ci = reinterpret_cast<int *>(cv + (size_t)a.splits * (a.top_n + kSlack));
+	const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+	const int k = a.top_n, nt = a.num_targets, K8 = a.hidden_dim / 8, per = k + kSlack;
+	float *cv = reinterpret_cast<float *>(join_raw);               // [splits * per]
+	int *ci = reinterpret_cast<int *>(cv + (size_t)a.splits * per);
+	int *ranges = ci + (size_t)a.splits * per;                     // [splits]
 	__shared__ float red[4][4];
 	__shared__ float dots[KLLM_MAX_TARGETS_I][4];
-	__shared__ int n_cand;
+	__shared__ int n_cand, n_ranges;
 	__shared__ float max_tau;
-	const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-	const int k = a.top_n, nt = a.num_targets, K8 = a.hidden_dim / 8;
 	const size_t rows = (size_t)a.row_blocks * kSR, stride = (size_t)a.splits * rows;
+	const float4 *part = static_cast<const float4 *>(a.part) + r;
 	const float T = a.temperature ? a.temperature[r] : 1.f;
 	const float inv_t = T > 0.f ? 1.f / T : 1.f;
+	if (tid == 0)
+		n_cand = n_ranges = 0;
 
 	// the targets' logits
 	const uint4 *h = reinterpret_cast<const uint4 *>(a.hidden) + (size_t)r * K8;
@@ -437,8 +480,9 @@ score_join_kernel(const kllm_score_args a)
 		float acc = 0.f;
 		if (t >= 0 && t < a.vocab) {
 			const uint4 *w = reinterpret_cast<const uint4 *>(a.weight) + (size_t)t * K8;
+#pragma unroll 4
 			for (int i = tid; i < K8; i += kJoinThreads)
-				acc = dot8(h[i], w[i], acc);
+				acc = dot8(__ldg(h + i), __ldg(w + i), acc);
 		}
 #pragma unroll
 		for (int o = 16; o; o >>= 1)
@@ -448,22 +492,20 @@ score_join_kernel(const kllm_score_args a)
 	}
 	// With at least top_n ranges, the top_n-th largest of the ranges' maxima is
 	// a threshold that top_n logits reach; warp 0 finds it, as y = l c like m
-	if (warp == 0) {
+	if (warp == 0 && k > 0) {
 		float top = -CUDART_INF_F;
 		for (int s = lane; s - lane < a.splits; s += 32) {
-			const float x = s < a.splits ? static_cast<const float4 *>(a.part)[(size_t)s * rows + r].x
-						     : -CUDART_INF_F;
-			const float d = warp_sort_desc(x, lane);
+			const float d = warp_sort_desc(s < a.splits ? part[(size_t)s * rows].x : -CUDART_INF_F, lane);
 			top = s == lane ? d : warp_merge_desc(top, d, lane);
 		}
-		const float y = __shfl_sync(0xffffffffu, top, k > 0 ? k - 1 : 0);
+		const float y = __shfl_sync(0xffffffffu, top, k - 1);
 		if (lane == 0)
 			max_tau = a.splits >= k ? y : -CUDART_INF_F;
 	}
 	// the ranges' triples and the largest threshold any of them reports
 	float m = -CUDART_INF_F, S = 0.f, W = 0.f, tau = -CUDART_INF_F;
 	for (int s = tid; s < a.splits; s += kJoinThreads) {
-		const float4 p = static_cast<const float4 *>(a.part)[(size_t)s * rows + r];
+		const float4 p = part[(size_t)s * rows];
 		join(m, S, W, p.x, p.y, p.z);
 		tau = fmaxf(tau, p.w);
 	}
@@ -481,8 +523,6 @@ score_join_kernel(const kllm_score_args a)
 		red[warp][2] = W;
 		red[warp][3] = tau;
 	}
-	if (tid == 0)
-		n_cand = 0;
 	__syncthreads();
 	m = red[0][0];
 	S = red[0][1];
@@ -510,15 +550,23 @@ score_join_kernel(const kllm_score_args a)
 	}
 	if (k == 0)
 		return;
+	// the ranges whose maximum reaches the threshold, and their entries that do
 	const float c = kLog2e * inv_t, y_min = max_tau;
-	for (int s = tid; s < a.splits; s += kJoinThreads) {
-		const size_t at = (size_t)s * rows + r;
-		const int n = min(a.part_n[at], k + kSlack);
-		for (int e = 0; e < n; ++e) {
+	for (int s = tid; s < a.splits; s += kJoinThreads)
+		if (part[(size_t)s * rows].x >= y_min)
+			ranges[atomicAdd(&n_ranges, 1)] = s;
+	__syncthreads();
+	const int total = n_ranges * per;
+#pragma unroll 4
+	for (int i = tid; i < total; i += kJoinThreads) {
+		const int g = i / per, e = i - g * per;
+		const size_t at = (size_t)ranges[g] * rows + r;
+		if (e < a.part_n[at]) {
 			const uint2 x = static_cast<const uint2 *>(a.part_list)[(size_t)e * stride + at];
-			if (__uint_as_float(x.x) >= tau && __uint_as_float(x.x) * c >= y_min) {
+			const float v = __uint_as_float(x.x);
+			if (v >= tau && v * c >= y_min) {
 				const int p = atomicAdd(&n_cand, 1);
-				cv[p] = __uint_as_float(x.x);
+				cv[p] = v;
 				ci[p] = (int)x.y;
 			}
 		}
@@ -529,8 +577,9 @@ score_join_kernel(const kllm_score_args a)
 		const float v = cv[i];
 		const int id = ci[i];
 		int at = 0;
+#pragma unroll 4
 		for (int j = 0; j < n; ++j)
-			at += (cv[j] > v || (cv[j] == v && ci[j] < id)) ? 1 : 0;
+			at += (int)(cv[j] > v) | ((int)(cv[j] == v) & (int)(ci[j] < id));
 		if (at < k) {
 			a.top_ids[(size_t)r * k + at] = id;
 			a.top_lp[(size_t)r * k + at] = v * inv_t - floor_;
@@ -605,7 +654,7 @@ extern "C" int kllm_score_launch(struct kllm_score_args *a, void *workspace, voi
 	e = cudaGetLastError();
 	if (e != cudaSuccess)
 		return (int)e;
-	const size_t js = (size_t)a->splits * (a->top_n + kSlack) * 8;
+	const size_t js = (size_t)a->splits * ((size_t)(a->top_n + kSlack) * 8 + 4);
 	e = cudaFuncSetAttribute(score_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)js);
 	if (e != cudaSuccess)
 		return (int)e;
