@@ -54,8 +54,7 @@ constexpr uint64_t kScWaitNs = 200000000ull;
 struct ScoreSmem {
 	uint8_t a[kSStages][kSR * kSK * 2];
 	uint8_t b[kSStages][kSN * kSK * 2];
-	uint32_t list_k[kListCap][kSR];
-	int list_i[kListCap][kSR];
+	uint2 list[kListCap][kSR];           // (value, index) of a row's largest logits so far
 	uint64_t full[kSStages], empty[kSStages];
 	uint64_t acc_full[2], acc_empty[2], drain;
 	uint32_t tmem_base;
@@ -93,14 +92,46 @@ __device__ __forceinline__ int unit_at(int s, int q, int units)
 // so a later logit has to be larger to matter. Called by whole warps; a lane
 // with n < k keeps its list. The list is held in registers: counting in shared
 // memory, an entry at a time, took 15k cycles a cut.
-__device__ __noinline__ void cut_list(uint32_t (*lk)[kSR], int (*li)[kSR], int t, int k, int &n,
-				      float &tau)
+struct Cut {
+	int n;                // entries kept
+	float tau;
+};
+
+constexpr uint32_t kListStep = kSR * sizeof(uint2);    // from one entry of a row to its next
+
+// Entries by their address in shared memory: the compiler takes the list for
+// generic memory, and an append for a branch, which made the
+// append most of the epilogue (333 rows of 32,003: 70 us, 53 so).
+__device__ __forceinline__ uint2 list_get(uint32_t at)
+{
+	uint2 x;
+	asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(at) : "memory");
+	return x;
+}
+__device__ __forceinline__ void list_put(uint32_t at, float v, uint32_t id)
+{
+	asm volatile("st.shared.v2.u32 [%0], {%1, %2};" :: "r"(at), "r"(__float_as_uint(v)), "r"(id) : "memory");
+}
+// Appends (v, base + i) at `at` and advances it when v > tau.
+__device__ __forceinline__ void list_offer(uint32_t &at, float v, float tau, int base, int i)
+{
+	asm volatile("{\n\t.reg .pred p;\n\t.reg .u32 id;\n\t"
+		     "setp.gt.f32 p, %1, %2;\n\t"
+		     "@p add.u32 id, %3, %4;\n\t"
+		     "@p st.shared.v2.u32 [%0], {%5, id};\n\t"
+		     "@p add.u32 %0, %0, %6;\n\t}"
+		     : "+r"(at)
+		     : "f"(v), "f"(tau), "r"(base), "r"(i), "r"(__float_as_uint(v)), "n"(kListStep)
+		     : "memory");
+}
+
+__device__ __noinline__ Cut cut_list(uint32_t list, int k, int n, float tau)
 {
 	uint32_t key[kListCap];
 	uint32_t lo = 0xffffffffu, hi = 0u;
 #pragma unroll
 	for (int e = 0; e < kListCap; ++e) {
-		key[e] = lk[e][t];
+		key[e] = key_of(__uint_as_float(list_get(list + e * kListStep).x));
 		if (e >= n)
 			key[e] = 0u;                       // below every number's key
 		else
@@ -134,24 +165,22 @@ __device__ __noinline__ void cut_list(uint32_t (*lk)[kSR], int (*li)[kSR], int t
 		}
 	}
 	if (!work)
-		return;
-	int id[kListCap];
+		return {n, tau};
+	uint32_t id[kListCap];
 #pragma unroll
 	for (int e = 0; e < kListCap; ++e)
-		id[e] = li[e][t];
+		id[e] = list_get(list + e * kListStep).y;
 	int w = 0;
 #pragma unroll
 	for (int e = 0; e < kListCap; ++e) {
 		const bool eq = key[e] == lo;
 		if (key[e] > lo || (eq && budget > 0)) {
 			budget -= eq ? 1 : 0;
-			lk[w][t] = key[e];
-			li[w][t] = id[e];
+			list_put(list + w * kListStep, value_of(key[e]), id[e]);
 			++w;
 		}
 	}
-	n = w;
-	tau = value_of(lo);
+	return {w, value_of(lo)};
 }
 
 __global__ void __launch_bounds__(kScThreads, 1)
@@ -310,11 +339,12 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 			if (!item_range(item, rb, split, u0, u1))
 				continue;
 			const int row = rb * kSR + t;
-			const bool live = row < a.num_rows;
+			const bool live = row < a.num_rows;      // the rest are rows of zeros
 			const float T = (live && a.temperature) ? a.temperature[row] : 1.f;
 			const float c = kLog2e * (T > 0.f ? 1.f / T : 1.f);
 			float m = -CUDART_INF_F, S = 0.f, W = 0.f, tau = -CUDART_INF_F;
-			int n = 0;
+			const uint32_t list = smem_u32(&sm.list[0][t]);
+			uint32_t at = list;                // where the next entry goes
 			for (int u = u0; u < u1; u += 4, ++it) {
 				const int buf = it & 1, nc = min(4, u1 - u) * (kSU / 32);
 				if (!__all_sync(0xffffffffu, sc_wait(sm, &sm.acc_full[buf],
@@ -349,12 +379,11 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 #pragma unroll
 							for (int i = 1; i < 8; ++i)
 								gm = fmaxf(gm, v[8 * g + i]);
-							sm.list_k[4 * ch + g][t] = key_of(gm == gm ? gm : -CUDART_INF_F);
+							list_put(list + (4 * ch + g) * kListStep,
+								 gm == gm ? gm : -CUDART_INF_F, 0u);
 						}
 					}
-					n = 4 * nc;
-					cut_list(sm.list_k, sm.list_i, t, k, n, tau);
-					n = 0;
+					tau = cut_list(list, k, 4 * nc, tau).tau;
 					if (tau > -CUDART_INF_F)                 // its equals are wanted
 						tau = value_of(key_of(tau) - 1u);
 				}
@@ -365,11 +394,11 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 					if (nb >= V)
 						break;                 // nothing but padding
 					columns(ch, v);
-					float cm = v[0];
+					float c4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-					for (int i = 1; i < 32; ++i)
-						cm = fmaxf(cm, v[i]);
-					const float ym = cm * c;
+					for (int i = 4; i < 32; ++i)
+						c4[i & 3] = fmaxf(c4[i & 3], v[i]);
+					const float ym = fmaxf(fmaxf(c4[0], c4[1]), fmaxf(c4[2], c4[3])) * c;
 					if (ym > m) {
 						if (m > -CUDART_INF_F) {
 							const float d = ym - m, f = ex2_approx(-d);
@@ -381,30 +410,28 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 					// sums of 32, then of the chunks: a range has thousands of
 					// terms, and one running fp32 sum over them lost 2e-6
 					const float ref = m == -CUDART_INF_F ? 0.f : m;
-					float s2[2] = {0.f, 0.f}, w2[2] = {0.f, 0.f};
+					float s4[4] = {0.f, 0.f, 0.f, 0.f}, w4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
 					for (int i = 0; i < 32; ++i) {
 						const float d = fmaf(v[i], c, -ref);
 						const float e = ex2_approx(d);
-						s2[i & 1] += e;
-						w2[i & 1] = fmaf(e, fmaxf(d, -1000.f), w2[i & 1]);
+						s4[i & 3] += e;
+						w4[i & 3] = fmaf(e, fmaxf(d, -1000.f), w4[i & 3]);
 					}
-					S += s2[0] + s2[1];
-					W += w2[0] + w2[1];
+					S += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+					W += (w4[0] + w4[1]) + (w4[2] + w4[3]);
 					if (k > 0) {
 #pragma unroll
 						for (int half = 0; half < 2; ++half) {
-							if (live) {
 #pragma unroll
-								for (int i = 16 * half; i < 16 * half + 16; ++i)
-									if (v[i] > tau) {
-										sm.list_k[n][t] = key_of(v[i]);
-										sm.list_i[n][t] = nb + i;
-										++n;
-									}
+							for (int i = 16 * half; i < 16 * half + 16; ++i)
+								list_offer(at, v[i], tau, nb, i);
+							const int n = (int)((at - list) / kListStep);
+							if (__any_sync(0xffffffffu, n > kListTrig)) {
+								const Cut cut = cut_list(list, k, n, tau);
+								at = list + cut.n * kListStep;
+								tau = cut.tau;
 							}
-							if (__any_sync(0xffffffffu, n > kListTrig))
-								cut_list(sm.list_k, sm.list_i, t, k, n, tau);
 						}
 					}
 				}
@@ -413,17 +440,20 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 			}
 			if (!ok)
 				break;
-			if (k > 0)
-				cut_list(sm.list_k, sm.list_i, t, k, n, tau);
-			const size_t at = (size_t)split * a.row_blocks * kSR + (size_t)rb * kSR + t;
-			static_cast<float4 *>(a.part)[at] = make_float4(m, S, W, tau);
+			int n = (int)((at - list) / kListStep);
+			if (k > 0) {
+				const Cut cut = cut_list(list, k, n, tau);
+				n = cut.n;
+				tau = cut.tau;
+			}
+			const size_t to = (size_t)split * a.row_blocks * kSR + (size_t)rb * kSR + t;
+			static_cast<float4 *>(a.part)[to] = make_float4(m, S, W, tau);
 			if (k > 0) {
 				const size_t stride = (size_t)a.splits * a.row_blocks * kSR;
-				a.part_n[at] = n;
+				a.part_n[to] = n;
 				for (int e = 0; e < n; ++e)
-					static_cast<uint2 *>(a.part_list)[(size_t)e * stride + at] =
-					    make_uint2(__float_as_uint(value_of(sm.list_k[e][t])),
-						       (uint32_t)sm.list_i[e][t]);
+					static_cast<uint2 *>(a.part_list)[(size_t)e * stride + to] =
+					    list_get(list + e * kListStep);
 			}
 		}
 	}
