@@ -99,9 +99,9 @@ struct Cut {
 
 constexpr uint32_t kListStep = kSR * sizeof(uint2);    // from one entry of a row to its next
 
-// Entries by their address in shared memory: the compiler takes the list for
-// generic memory, and an append for a branch, which made the
-// append most of the epilogue (333 rows of 32,003: 70 us, 53 so).
+// Entries by their address in shared memory, appended under a predicate: the
+// compiler takes the list for generic memory and an append for a branch, which
+// was most of the epilogue (333 rows of 32,003: 70 us, 53 so).
 __device__ __forceinline__ uint2 list_get(uint32_t at)
 {
 	uint2 x;
@@ -143,19 +143,16 @@ __device__ __noinline__ Cut cut_list(uint32_t list, int k, int n, float tau)
 	const bool work = n >= k;
 	hi = hi + 1u;                              // keys of numbers stay below 2^32 - 1
 	bool done = !work || n <= k + kSlack;
-	int budget = kListCap;                     // of entries equal to lo
+	bool equals = false;
 	while (!__all_sync(0xffffffffu, done)) {
 		const uint32_t mid = lo + ((hi - lo) >> 1);
-		int c[2] = {0, 0}, above[2] = {0, 0};
+		int c[2] = {0, 0};
 #pragma unroll
-		for (int e = 0; e < kListCap; ++e) {
+		for (int e = 0; e < kListCap; ++e)
 			c[e & 1] += key[e] >= mid ? 1 : 0;
-			above[e & 1] += key[e] > lo ? 1 : 0;
-		}
 		if (!done) {
 			if (mid == lo) {
-				budget = k - (above[0] + above[1]);
-				done = true;
+				equals = done = true;
 			} else if (c[0] + c[1] >= k) {
 				lo = mid;
 				done = c[0] + c[1] <= k + kSlack;
@@ -166,6 +163,13 @@ __device__ __noinline__ Cut cut_list(uint32_t list, int k, int n, float tau)
 	}
 	if (!work)
 		return {n, tau};
+	int budget = kListCap;                     // of entries equal to lo
+	if (equals) {
+		budget = k;
+#pragma unroll
+		for (int e = 0; e < kListCap; ++e)
+			budget -= key[e] > lo ? 1 : 0;
+	}
 	uint32_t id[kListCap];
 #pragma unroll
 	for (int e = 0; e < kListCap; ++e)
@@ -195,6 +199,7 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 	const int per_group = a.group_rb * a.splits;
 	const int n_items = (a.row_blocks + a.group_rb - 1) / a.group_rb * per_group;
 
+	grid_launch_dependents();
 	if (tid == 0) {
 		for (int s = 0; s < kSStages; ++s) {
 			mbar_init(&sm.full[s], 1);
@@ -520,6 +525,7 @@ score_join_kernel(const kllm_score_args a)
 		if (lane == 0)
 			dots[j][warp] = acc;
 	}
+	grid_dependency_wait();                // the ranges' results
 	// With at least top_n ranges, the top_n-th largest of the ranges' maxima is
 	// a threshold that top_n logits reach; warp 0 finds it, as y = l c like m
 	if (warp == 0 && k > 0) {
@@ -688,6 +694,16 @@ extern "C" int kllm_score_launch(struct kllm_score_args *a, void *workspace, voi
 	e = cudaFuncSetAttribute(score_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)js);
 	if (e != cudaSuccess)
 		return (int)e;
-	score_join_kernel<<<a->num_rows, kJoinThreads, js, st>>>(*a);
-	return (int)cudaGetLastError();
+	// starts as the ranges' CTAs leave, with the targets' logits, which need none of them
+	cudaLaunchConfig_t cfg = {};
+	cfg.gridDim = dim3((unsigned)a->num_rows);
+	cfg.blockDim = dim3(kJoinThreads);
+	cfg.dynamicSmemBytes = js;
+	cfg.stream = st;
+	cudaLaunchAttribute at[1];
+	at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	at[0].val.programmaticStreamSerializationAllowed = 1;
+	cfg.attrs = at;
+	cfg.numAttrs = 1;
+	return (int)cudaLaunchKernelEx(&cfg, score_join_kernel, (const struct kllm_score_args)*a);
 }
