@@ -59,14 +59,14 @@ namespace {
 
 constexpr int kPRows = 128, kPKeys = 128;
 constexpr int kUnitRows = 256;
-constexpr int kPThreads = 20 * 32;
-constexpr int kWarpProd = 8, kWarpMma = 16, kWarpLoad = 17;
-constexpr int kProd = 256;                    // producer threads
-// Registers: 640 threads launch with 96 each, and the CTA hands them to the
-// warps that need them: a softmax thread holds 64 scores (256 x 112 + 384 x 80
-// of 640 x 96), a suffix warp its tile's fragments (MX: 384 x 144 + 256 x 24;
-// BF16: 256 x 184 + 384 x 32).
+constexpr int kPThreads = 16 * 32;
+constexpr int kWarpProd = 8, kWarpMma = 14, kWarpLoad = 15;
+constexpr int kProd = 192;                    // producer threads
+// Registers: 512 threads launch with 128 each, all of an SM's. A softmax thread
+// holds 128 scores (256 x 160 + 256 x 96); a suffix warp's MX tile takes the 128,
+// its BF16 tile 184 (256 x 184 + 256 x 72).
 constexpr int kRaw = 3;                       // raw stages (MX) / page-address stages (BF16)
+constexpr int kRawKeys = 64;                  // keys of a raw stage
 constexpr float kRaise = 8.f;                 // slack of the lazy reference maximum, log2
 constexpr float kPShift = 7.f;                // f16 P is built 2^7 larger
 constexpr uint64_t kPWaitNs = 200000000ull;
@@ -97,7 +97,7 @@ static_assert(sizeof(PHeader) == 64 && sizeof(PGroup) == 48, "workspace layout")
 constexpr int kPlanThreads = 1024;
 // A CTA's time for n steps or for n tiles a warp, in ns, as measured on the
 // whole chip: set-up, then the rate. They only balance the two parts.
-constexpr float kStepSetNs = 7000.f, kStepNs = 1400.f, kTileSetNs = 4500.f, kTileNs = 1200.f;
+constexpr float kStepSetNs = 10500.f, kStepNsMx = 1500.f, kStepNsBf16 = 2700.f, kTileSetNs = 5000.f, kTileNs = 2500.f;
 
 struct PlanSmem {
 	long long w0[32], w1[32];
@@ -250,7 +250,7 @@ plan_kernel(const kllm_prefix_args a)
 		if (possible) {
 			float t = 0.f;
 			if (n > 0)
-				t = kStepSetNs + kStepNs * ceilf((float)T / (float)n);
+				t = kStepSetNs + (a.kv_dtype ? kStepNsMx : kStepNsBf16) * ceilf((float)T / (float)n);
 			if (N > 0)
 				t = fmaxf(t, kTileSetNs + kTileNs * ceilf((float)N / (float)((a.ctas - n) * a.suf_warps)));
 			atomicMin(&sm.best, ((unsigned long long)__float_as_uint(t) << 32) | (unsigned)n);
@@ -282,9 +282,8 @@ struct PG {
 	static constexpr int NH = D / 64;                     // 64-column halves
 	static constexpr int HALF = kPRows * 128;             // bytes of one half tile
 	static constexpr int TILE = NH * HALF;
-	static constexpr int KB = MX ? 1 : 2;                 // K operand buffers
-	static constexpr int RAW = MX ? kPKeys * D : 16;      // payload of a block
-	static constexpr int RAWS = MX ? kPKeys * D / 8 : 16; // its scales
+	static constexpr int RAW = MX ? kRawKeys * D : 16;    // payload of half a block
+	static constexpr int RAWS = MX ? kRawKeys * D / 8 : 16;  // its scales
 	static constexpr int LPR = D / 8;                     // 16-byte chunks of a bf16 row
 };
 
@@ -292,10 +291,10 @@ template <int D, int KVT>
 struct PrefixSmem {
 	using G = PG<D, KVT>;
 	uint8_t q[2][G::TILE];
-	uint8_t k[G::KB][G::TILE];
+	uint8_t k[2][G::TILE];
 	uint8_t v[2][G::TILE];
-	uint8_t raw[kRaw][G::RAW];            // [128 keys][D] payload
-	uint8_t raws[kRaw][G::RAWS];          // [128 keys][D / 8] scales
+	uint8_t raw[kRaw][G::RAW];            // [64 keys][D] payload
+	uint8_t raws[kRaw][G::RAWS];          // [64 keys][D / 8] scales
 	float qf[2][kPRows];                  // 2^-e of a solo piece's query rows, by piece parity
 	unsigned long long pg[kRaw][2][8];    // page addresses of a block (BF16)
 	uint32_t slot_ok[kRaw];               // pages present, one bit each
@@ -430,50 +429,52 @@ __device__ __forceinline__ void mx16_to_f16(uint2 wl, uint2 wh, uint32_t scl, ui
 	hi.w = f16x2_mul(place_pair(__byte_perm(wh.y, 0u, 0x4342u)), s1);
 }
 
-// One raw block -> the operand tile [128 keys][D] f16, 128-byte swizzle, by the
-// producers; rows of absent pages are zeros. A lane takes 16 codes as two
-// 8-byte chunks; lanes of the upper 64 columns take them in the other order, so
-// that the eight lanes of a row never store to one bank. Loads of kFly rows
-// come before their stores: the compiler cannot tell that the tiles do not
-// overlap.
+// Half a raw block -> rows key0 .. key0 + 63 of the operand tile [128 keys][D]
+// f16, 128-byte swizzle, by the producers; rows of absent pages are zeros. A
+// lane takes 16 codes as two 8-byte chunks; lanes of the upper 64 columns take
+// them in the other order, so that the eight lanes of a row never store to one
+// bank. All loads come before the stores: the compiler cannot tell that the
+// tiles do not overlap.
 template <int D>
-__device__ __forceinline__ void dequant_block(uint8_t *dst, const uint8_t *raw, const uint8_t *rs,
-					      const uint32_t *mask, bool full, int pt)
+__device__ __forceinline__ void dequant_half(uint8_t *dst, int key0, const uint8_t *raw, const uint8_t *rs,
+					     const uint32_t *mask, bool full, int pt)
 {
-	constexpr int LPR = D / 16, RPP = kProd / LPR, kFly = kPKeys / RPP;
+	constexpr int LPR = D / 16, RPP = kProd / LPR, kPass = (kRawKeys + RPP - 1) / RPP;
 	const int l = pt % LPR, row0 = pt / LPR;
+	const bool part = row0 + (kPass - 1) * RPP < kRawKeys;   // the last pass; warp-uniform
 	const int first = l >= 4 ? 1 : 0;
 	const int c0 = (2 * l) & 7;
-	// RPP is a multiple of 8, so the swizzle of a lane's rows is the same
-	uint8_t *o0 = dst + (l >> 2) * (kPRows * 128) + swz(row0, c0 + first);
-	uint8_t *o1 = dst + (l >> 2) * (kPRows * 128) + swz(row0, c0 + 1 - first);
+	// RPP and key0 are multiples of 8, so the swizzle of a lane's rows is the same
+	uint8_t *o0 = dst + (l >> 2) * (kPRows * 128) + swz(key0 + row0, c0 + first);
+	uint8_t *o1 = dst + (l >> 2) * (kPRows * 128) + swz(key0 + row0, c0 + 1 - first);
 	const uint8_t *pl = raw + row0 * D + l * 16 + 8 * first, *ph = raw + row0 * D + l * 16 + 8 * (1 - first);
 	const uint8_t *sl = rs + row0 * (D / 8) + l * 2 + first, *sh = rs + row0 * (D / 8) + l * 2 + 1 - first;
+	uint2 wl[kPass], wh[kPass];
+	uint32_t a[kPass], b[kPass];
 #pragma unroll
-	for (int i0 = 0; i0 < kPKeys / RPP; i0 += kFly) {
-		uint2 wl[kFly], wh[kFly];
-		uint32_t a[kFly], b[kFly];
+	for (int u = 0; u < kPass; ++u) {
+		if (u == kPass - 1 && !part)
+			continue;
+		wl[u] = *reinterpret_cast<const uint2 *>(pl + u * RPP * D);
+		wh[u] = *reinterpret_cast<const uint2 *>(ph + u * RPP * D);
+		a[u] = sl[u * RPP * (D / 8)];
+		b[u] = sh[u * RPP * (D / 8)];
+	}
+	if (!full)
 #pragma unroll
-		for (int u = 0; u < kFly; ++u) {
-			wl[u] = *reinterpret_cast<const uint2 *>(pl + (i0 + u) * RPP * D);
-			wh[u] = *reinterpret_cast<const uint2 *>(ph + (i0 + u) * RPP * D);
-			a[u] = sl[(i0 + u) * RPP * (D / 8)];
-			b[u] = sh[(i0 + u) * RPP * (D / 8)];
+		for (int u = 0; u < kPass; ++u) {
+			const int row = key0 + row0 + u * RPP;
+			if (row < kPKeys && !((mask[row >> 5] >> (row & 31)) & 1u))
+				wl[u] = wh[u] = make_uint2(0u, 0u);
 		}
-		if (!full)
 #pragma unroll
-			for (int u = 0; u < kFly; ++u) {
-				const int row = row0 + (i0 + u) * RPP;
-				if (!((mask[row >> 5] >> (row & 31)) & 1u))
-					wl[u] = wh[u] = make_uint2(0u, 0u);
-			}
-#pragma unroll
-		for (int u = 0; u < kFly; ++u) {
-			uint4 lo, hi;
-			mx16_to_f16(wl[u], wh[u], a[u], b[u], lo, hi);
-			*reinterpret_cast<uint4 *>(o0 + (i0 + u) * RPP * 128) = lo;
-			*reinterpret_cast<uint4 *>(o1 + (i0 + u) * RPP * 128) = hi;
-		}
+	for (int u = 0; u < kPass; ++u) {
+		if (u == kPass - 1 && !part)
+			continue;
+		uint4 lo, hi;
+		mx16_to_f16(wl[u], wh[u], a[u], b[u], lo, hi);
+		*reinterpret_cast<uint4 *>(o0 + u * RPP * 128) = lo;
+		*reinterpret_cast<uint4 *>(o1 + u * RPP * 128) = hi;
 	}
 }
 
@@ -481,6 +482,10 @@ __device__ __forceinline__ void cp_async16(void *dst, const void *src)
 {
 	asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
 		     :: "r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void bulk_prefetch_l2(const void *src, uint32_t bytes)
+{
+	asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit()
 {
@@ -492,16 +497,16 @@ __device__ __forceinline__ void cp_async_wait()
 	asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory");
 }
 
-// 64 scores of this thread's TMEM lane, all loads in flight; keys whose bit in
-// (m0, m1) is clear read as -inf.
-__device__ __forceinline__ void load_scores(uint32_t taddr, bool full, uint32_t m0, uint32_t m1,
-					    uint32_t (&r)[4][16])
+// The 128 scores of this thread's TMEM lane, all loads in flight; keys whose bit
+// in mask is clear read as -inf.
+__device__ __forceinline__ void load_scores(uint32_t taddr, bool full, const uint32_t *mask,
+					    uint32_t (&r)[8][16])
 {
 #pragma unroll
-	for (int q = 0; q < 4; ++q)
+	for (int q = 0; q < 8; ++q)
 		tmem_ld16_nowait(taddr + 16 * q, r[q]);
 #pragma unroll
-	for (int q = 0; q < 4; ++q)
+	for (int q = 0; q < 8; ++q)
 		asm volatile("tcgen05.wait::ld.sync.aligned;"
 			     : "+r"(r[q][0]), "+r"(r[q][1]), "+r"(r[q][2]), "+r"(r[q][3]),
 			       "+r"(r[q][4]), "+r"(r[q][5]), "+r"(r[q][6]), "+r"(r[q][7]),
@@ -510,9 +515,13 @@ __device__ __forceinline__ void load_scores(uint32_t taddr, bool full, uint32_t 
 			     :: "memory");
 	if (!full)
 #pragma unroll
-		for (int i = 0; i < 64; ++i)
-			if (!(((i < 32 ? m0 : m1) >> (i & 31)) & 1u))
-				r[i >> 4][i & 15] = 0xFF800000u;
+		for (int w = 0; w < 4; ++w) {
+			const uint32_t m = mask[w];
+#pragma unroll
+			for (int i = 0; i < 32; ++i)
+				if (!((m >> i) & 1u))
+					r[2 * w + (i >> 4)][i & 15] = 0xFF800000u;
+		}
 }
 
 // One 128-key block of one row: S in the TMEM columns of tS -> P over them
@@ -520,9 +529,9 @@ __device__ __forceinline__ void load_scores(uint32_t taddr, bool full, uint32_t 
 // maximum is known before any P is written, so raising the reference rescales
 // only O and l. Warp-collective; branches around TMEM accesses are
 // warp-uniform. Returns through m_ref and l_sum. Keys 0-63 are announced on
-// p_half as soon as they are written, so their products can start. Two passes
-// over the scores, 64 at a time and rolled: holding all 128 took registers that
-// the other roles then spilled for, and its code thrashed the instruction cache.
+// p_half as soon as they are written, so their products can start. The scores
+// stay in registers between the maximum and the exponentials: read a second
+// time they cost 0.9k of 3.3k cycles a block in TMEM round trips.
 template <int D, int KVT>
 __device__ __forceinline__ void softmax_rows(uint32_t tS, uint32_t tO, const uint32_t *mask,
 					     float sl2, bool o_live, float &m_ref, float &l_sum,
@@ -531,21 +540,16 @@ __device__ __forceinline__ void softmax_rows(uint32_t tS, uint32_t tO, const uin
 	constexpr bool MX = KVT == 1;
 	constexpr float shift = MX ? kPShift : 0.f;
 	const bool full = (mask[0] & mask[1] & mask[2] & mask[3]) == 0xFFFFFFFFu;  // same in all lanes
-	float mx = -CUDART_INF_F;
-#pragma unroll 1
-	for (int half = 0; half < 2; ++half) {
-		uint32_t r[4][16];
-		load_scores(tS + 64 * half, full, mask[2 * half], mask[2 * half + 1], r);
-		float m4[4];
+	uint32_t r[8][16];
+	load_scores(tS, full, mask, r);
+	float m4[4];
 #pragma unroll
-		for (int i = 0; i < 4; ++i)
-			m4[i] = __uint_as_float(r[0][i]);
+	for (int i = 0; i < 4; ++i)
+		m4[i] = __uint_as_float(r[0][i]);
 #pragma unroll
-		for (int k = 4; k < 64; ++k)
-			m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(r[k >> 4][k & 15]));
-		mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-	}
-	const float gl = mx * sl2;
+	for (int k = 4; k < 128; ++k)
+		m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(r[k >> 4][k & 15]));
+	const float gl = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl2;
 	const bool raise = gl > m_ref + kRaise;
 	if (__any_sync(0xffffffffu, raise)) {
 		const float f = raise ? exp2f(m_ref - gl) : 1.f;
@@ -567,46 +571,32 @@ __device__ __forceinline__ void softmax_rows(uint32_t tS, uint32_t tO, const uin
 	// no key present yet (m_ref = -inf): every p is 0, not exp2(-inf + inf)
 	const float moff = m_ref == -CUDART_INF_F ? -CUDART_INF_F : shift - m_ref;
 	float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-	for (int half = 0; half < 2; ++half) {
-		uint32_t r[4][16];
-		load_scores(tS + 64 * half, full, mask[2 * half], mask[2 * half + 1], r);
 #pragma unroll
-		for (int c = 0; c < 64; c += MX ? 32 : 16) {
-			float w[16];
+	for (int c = 0; c < 128; c += MX ? 32 : 16) {
+		float w[16];
+#pragma unroll
+		for (int i = 0; i < (MX ? 16 : 8); ++i) {
+			const int k = c + 2 * i;
+			const float p0 = ex2_approx(fmaf(__uint_as_float(r[k >> 4][k & 15]), sl2, moff));
+			const float p1 = ex2_approx(fmaf(__uint_as_float(r[k >> 4][(k & 15) + 1]), sl2, moff));
+			sum[i & 3] += p0 + p1;
 			if constexpr (MX) {
-#pragma unroll
-				for (int i = 0; i < 16; ++i) {
-					const int k = c + 2 * i;
-					const float p0 = ex2_approx(fmaf(__uint_as_float(r[k >> 4][k & 15]), sl2, moff));
-					const float p1 =
-					    ex2_approx(fmaf(__uint_as_float(r[k >> 4][(k & 15) + 1]), sl2, moff));
-					sum[i & 3] += p0 + p1;
-					w[i] = __uint_as_float(pack_f16x2(p0, p1));
-				}
-				tmem_st16_nowait(tS + 32 * half + c / 2, w);
+				w[i] = __uint_as_float(pack_f16x2(p0, p1));
 			} else {
-#pragma unroll
-				for (int i = 0; i < 8; ++i) {
-					const int k = c + 2 * i;
-					const float p0 = ex2_approx(fmaf(__uint_as_float(r[k >> 4][k & 15]), sl2, moff));
-					const float p1 =
-					    ex2_approx(fmaf(__uint_as_float(r[k >> 4][(k & 15) + 1]), sl2, moff));
-					sum[i & 3] += p0 + p1;
-					const uint32_t hi = pack_bf16x2(p0, p1);
-					w[i] = __uint_as_float(hi);
-					w[8 + i] = __uint_as_float(pack_bf16x2(p0 - __uint_as_float(hi << 16),
-									       p1 - __uint_as_float(hi & 0xFFFF0000u)));
-				}
-				tmem_st16_nowait(tS + 64 * half + c, w);
+				const uint32_t hi = pack_bf16x2(p0, p1);
+				w[i] = __uint_as_float(hi);
+				w[8 + i] = __uint_as_float(pack_bf16x2(p0 - __uint_as_float(hi << 16),
+								       p1 - __uint_as_float(hi & 0xFFFF0000u)));
 			}
 		}
-		tmem_wait_st();
-		if (half == 0) {
+		tmem_st16_nowait(tS + (MX ? c / 2 : c), w);
+		if (c + (MX ? 32 : 16) == 64) {
+			tmem_wait_st();
 			tc_fence_before();
 			mbar_arrive(p_half);
 		}
 	}
+	tmem_wait_st();
 	l_sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
@@ -715,7 +705,7 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 
 	if (warp < kWarpProd) {
 		// ================= softmax of stream t ========================================
-		asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
 		const int t = warp >> 2, rr = (warp & 3) * 32 + lane;
 		const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
 		const uint32_t tS = lane_base + col_s(t), tO = lane_base + col_o(t);
@@ -837,39 +827,38 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 			};
 			if constexpr (G::MX) {
 				for (int j = 0; j < p.nb && ok; ++j)
-					for (int which = 0; which < 2; ++which, ++rf) {
-						const int st = rf % kRaw;
-						ok = wait_warp(&sm.raw_full[st], (uint32_t)((rf / kRaw) & 1));
-						if (which == 0)
-							ok = ok && (kf == 0 || wait_warp(&sm.k_empty[0], (uint32_t)((kf - 1) & 1)));
-						else
-							ok = ok && (vf < 2 || wait_warp(&sm.v_empty[vf & 1],
-										   (uint32_t)(((vf >> 1) - 1) & 1)));
+					for (int which = 0; which < 2 && ok; ++which) {
+						int &cnt = which ? vf : kf;
+						uint64_t *empty = which ? &sm.v_empty[cnt & 1] : &sm.k_empty[cnt & 1];
+						ok = cnt < 2 || wait_warp(empty, (uint32_t)(((cnt >> 1) - 1) & 1));
+						uint8_t *dst = which ? sm.v[cnt & 1] : sm.k[cnt & 1];
+#pragma unroll 1
+						for (int half = 0; half < 2 && ok; ++half, ++rf) {
+							const int st = rf % kRaw;
+							ok = wait_warp(&sm.raw_full[st], (uint32_t)((rf / kRaw) & 1));
+							if (!ok)
+								break;
+							const uint32_t okm = sm.slot_ok[st];
+							// all pages present and no key past the last one
+							const bool full = okm == all_pages && ppb * bs == kPKeys;
+							uint32_t mk[4] = {~0u, ~0u, ~0u, ~0u};
+							if (!full)
+#pragma unroll
+								for (int w = 0; w < 4; ++w)
+									mk[w] = key_mask(okm, w);
+							dequant_half<D>(dst, half * kRawKeys, sm.raw[st], sm.raws[st], mk, full,
+									pt);
+							if (which == 0 && half == 0 && pt == 0)
+#pragma unroll
+								for (int w = 0; w < 4; ++w)
+									sm.key_ok[kf & 3][w] = mk[w];
+							mbar_arrive(&sm.raw_empty[st]);
+						}
 						if (!ok)
 							break;
-						const uint32_t okm = sm.slot_ok[st];
-						// all pages present and no key past the last one
-						const bool full = okm == all_pages && ppb * bs == kPKeys;
-						uint32_t mk[4] = {~0u, ~0u, ~0u, ~0u};
-						if (!full)
-#pragma unroll
-							for (int w = 0; w < 4; ++w)
-								mk[w] = key_mask(okm, w);
-						dequant_block<D>(which ? sm.v[vf & 1] : sm.k[0], sm.raw[st], sm.raws[st], mk,
-								 full, pt);
-						if (which == 0 && pt == 0)
-#pragma unroll
-							for (int w = 0; w < 4; ++w)
-								sm.key_ok[kf & 3][w] = mk[w];
 						fence_async_smem();
-						mbar_arrive(&sm.raw_empty[st]);
-						if (which == 0) {
-							mbar_arrive(&sm.k_full[0]);
-							++kf;
-						} else {
-							mbar_arrive(&sm.v_full[vf & 1]);
-							++vf;
-						}
+						mbar_arrive(which ? &sm.v_full[cnt & 1] : &sm.k_full[cnt & 1]);
+						++cnt;
 					}
 			} else {
 				// fills run two ahead of their arrival: K0 V0 K1 V1 ...
@@ -893,12 +882,10 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 						break;
 					const uint32_t okm = sm.slot_ok[st];
 					uint8_t *dst = (which ? sm.v[cnt & 1] : sm.k[cnt & 1]) + (l >> 3) * G::HALF;
-					// a lane's rows are multiples of 8 apart, so their swizzle is the same
 					constexpr int RPP = kProd / G::LPR;
-					const int row0 = pt / G::LPR;
-					uint8_t *o = dst + swz(row0, l & 7);
 #pragma unroll 4
-					for (int row = row0; row < kPKeys; row += RPP, o += RPP * 128) {
+					for (int row = pt / G::LPR; row < kPKeys; row += RPP) {
+						uint8_t *o = dst + swz(row, l & 7);
 						const int page = ((row >> 4) * inv16) >> 8;        // row / bs
 						if ((okm >> page) & 1u)                            // never past the last page
 							cp_async16(o, reinterpret_cast<const uint8_t *>(sm.pg[st][which][page]) +
@@ -942,7 +929,7 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 		const uint64_t dq0 = umma_desc(smem_u32(sm.q[0]), 16u, 1024u);
 		const uint64_t dq1 = umma_desc(smem_u32(sm.q[1]), 16u, 1024u);
 		const uint64_t dk0 = umma_desc(smem_u32(sm.k[0]), 16u, 1024u);
-		const uint64_t dk1 = umma_desc(smem_u32(sm.k[G::KB - 1]), 16u, 1024u);
+		const uint64_t dk1 = umma_desc(smem_u32(sm.k[1]), 16u, 1024u);
 		const uint64_t dv0 = umma_desc(smem_u32(sm.v[0]), (uint32_t)G::HALF, 1024u);
 		const uint64_t dv1 = umma_desc(smem_u32(sm.v[1]), (uint32_t)G::HALF, 1024u);
 		int kf = 0, vf = 0, np = 0, n_p[2] = {0, 0};
@@ -955,15 +942,15 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 			__syncwarp();
 		};
 		auto wait_k = [&]() {
-			const int b = G::KB == 1 ? 0 : kf & 1, round = G::KB == 1 ? kf : kf >> 1;
+			const int b = kf & 1, round = kf >> 1;
 			return wait_all(&sm.k_full[b], (uint32_t)(round & 1));
 		};
 		auto free_k = [&]() {
-			commit(&sm.k_empty[G::KB == 1 ? 0 : kf & 1]);
+			commit(&sm.k_empty[kf & 1]);
 			++kf;
 		};
 		auto issue_s = [&](int t, int qt) {
-			const uint64_t dq = qt ? dq1 : dq0, dk = (G::KB == 2 && (kf & 1)) ? dk1 : dk0;
+			const uint64_t dq = qt ? dq1 : dq0, dk = (kf & 1) ? dk1 : dk0;
 #pragma unroll
 			for (int kk = 0; kk < D / 16; ++kk) {
 				const uint64_t off = ((uint64_t)(kk >> 2) * G::HALF + (uint64_t)(kk & 3) * 32u) >> 4;
@@ -1092,36 +1079,49 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 				continue;
 			const DevEntry *tb = static_cast<const DevEntry *>(a.table) +
 					     (size_t)p.leader * a.max_blocks;
-			auto load = [&](int b, DevEntry &e) {
+			const unsigned long long off = a.layer_off + (unsigned long long)p.h * sec;
+			auto load = [&](int b) {
+				DevEntry e;
 				const int page = b * ppb + lane;
 				e.k = e.v = 0ull;
 				e.valid = 0;
-				if (lane < ppb && page < p.npages) {
+				if (b < p.b0 + p.nb && lane < ppb && page < p.npages) {
 					e.k = __ldg(&tb[page].k);
 					e.v = __ldg(&tb[page].v);
 					e.valid = __ldg(&tb[page].valid);
 				}
+				return e;
 			};
-			DevEntry nxt;
-			load(p.b0, nxt);
-			for (int j = 0; j < p.nb && ok; ++j) {
-				const DevEntry e = nxt;
-				if (j + 1 < p.nb)
-					load(p.b0 + j + 1, nxt);
+			// this lane's page of a block as section addresses (0: absent), which
+			// start on their way to L2
+			auto check = [&](DevEntry &e) {
 				const bool present = e.valid && e.k != 0ull;
 				const bool aligned = ((e.k | e.v) & 15ull) == 0ull;
 				if (present && !aligned && a.err)
 					atomicOr(a.err, 0x2u);
-				const unsigned long long off = a.layer_off + (unsigned long long)p.h * sec;
 				bool here = present && aligned;
-				if (here && !(in_arenas(a.arenas, e.k + off, sec) &&
-					      in_arenas(a.arenas, e.v + off, sec))) {
+				e.k += off;
+				e.v += off;
+				if (here && !(in_arenas(a.arenas, e.k, sec) && in_arenas(a.arenas, e.v, sec))) {
 					here = false;
 					if (a.err)
 						atomicOr(a.err, KLLM_ERR_PAGE_RANGE_BIT);
 				}
-				const uint32_t mask = __ballot_sync(0xffffffffu, here);
-				for (int which = 0; which < (G::MX ? 2 : 1); ++which, ++rf) {
+				e.valid = here ? 1 : 0;
+				if (here) {
+					bulk_prefetch_l2(reinterpret_cast<const void *>(e.k), (uint32_t)sec);
+					bulk_prefetch_l2(reinterpret_cast<const void *>(e.v), (uint32_t)sec);
+				}
+			};
+			DevEntry cur = load(p.b0), nxt = load(p.b0 + 1);
+			check(cur);
+			for (int j = 0; j < p.nb && ok; ++j) {
+				const DevEntry e = cur;
+				cur = nxt;
+				check(cur);
+				nxt = load(p.b0 + j + 2);
+				const uint32_t mask = __ballot_sync(0xffffffffu, e.valid);
+				for (int part = 0; part < (G::MX ? 4 : 1); ++part, ++rf) {
 					const int st = rf % kRaw;
 					if (rf >= kRaw)
 						ok = __all_sync(0xffffffffu, wait(&sm.raw_empty[st],
@@ -1129,26 +1129,31 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 					if (!ok)
 						break;
 					if constexpr (G::MX) {
+						// rows r0 .. r1 - 1 of the block: this lane's page in this half
+						const int key0 = (part & 1) * kRawKeys;
+						const int r0 = max(lane * bs, key0), r1 = min(lane * bs + bs, key0 + kRawKeys);
+						const int n = e.valid ? max(r1 - r0, 0) : 0;
+						const uint32_t rows = __reduce_add_sync(0xffffffffu, (uint32_t)n);
 						if (lane == 0) {
 							sm.slot_ok[st] = mask;
-							mbar_arrive_expect_tx(&sm.raw_full[st], (uint32_t)(__popc(mask) * sec));
+							mbar_arrive_expect_tx(&sm.raw_full[st], rows * (uint32_t)(D * 9 / 8));
 						}
 #pragma unroll
 						for (int i = 0; i < kRaw; ++i)
 							armed[i] += i == st ? 1u : 0u;
 						__syncwarp();
-						// payload and scales of a page to the rows of its keys
-						if (here) {
-							const uint8_t *src = reinterpret_cast<const uint8_t *>((which ? e.v : e.k) + off);
-							bulk_g2s(sm.raw[st] + lane * bs * D, src, (uint32_t)(bs * D),
+						if (n > 0) {
+							const uint8_t *src = reinterpret_cast<const uint8_t *>(part >> 1 ? e.v : e.k);
+							const int pr = r0 - lane * bs;         // row of the page
+							bulk_g2s(sm.raw[st] + (r0 - key0) * D, src + pr * D, (uint32_t)(n * D),
 								 &sm.raw_full[st]);
-							bulk_g2s(sm.raws[st] + lane * bs * (D / 8), src + bs * D,
-								 (uint32_t)(bs * (D / 8)), &sm.raw_full[st]);
+							bulk_g2s(sm.raws[st] + (r0 - key0) * (D / 8), src + bs * D + pr * (D / 8),
+								 (uint32_t)(n * (D / 8)), &sm.raw_full[st]);
 						}
 					} else {
 						if (lane < 8) {
-							sm.pg[st][0][lane] = e.k + off;
-							sm.pg[st][1][lane] = e.v + off;
+							sm.pg[st][0][lane] = e.k;
+							sm.pg[st][1][lane] = e.v;
 						}
 						if (lane == 0)
 							sm.slot_ok[st] = mask;
@@ -1183,7 +1188,7 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 // Warps of a suffix CTA that work (the BF16 tile needs more registers).
 template <int KVT>
 struct SW {
-	static constexpr int N = KVT == 1 ? 12 : 8;
+	static constexpr int N = KVT == 1 ? 16 : 8;
 };
 
 struct SufSeg {
@@ -1269,13 +1274,16 @@ __device__ __noinline__ void suffix_exact(const kllm_prefix_args &a, int s, int 
 	}
 }
 
+// rows whose tile sums a suffix CTA keeps in shared memory; more are read from L2
+constexpr int kSufSeqs = 2040;
+
 template <int D, int KVT>
 struct SufLayout {
 	using Gm = Geom<D, KVT>;
 	static constexpr int NW = SW<KVT>::N, NST = 3;
 	static constexpr size_t ring = 0, bar = (size_t)NW * NST * Gm::STAGE, meta = bar + 8 * NW * NST;
 	static constexpr size_t lut = meta + 4 * NW * NST, pre = lut + 4 * 256;
-	static constexpr size_t total = pre + 4 * (KLLM_MAX_SEQS_LAUNCH + 1);
+	static constexpr size_t total = pre + 4 * (kSufSeqs + 1);
 };
 
 // CTA `cta` of those that share the N tiles of the suffixes among WS warps.
@@ -1295,7 +1303,7 @@ __device__ __forceinline__ void suffix_role(const kllm_prefix_args &a, uint8_t *
 	int *spre = reinterpret_cast<int *>(smem + Lay::pre);
 	if (cta * NW >= WS)
 		return;                                    // uniform over the CTA
-	const bool local = S <= KLLM_MAX_SEQS_LAUNCH;
+	const bool local = S <= kSufSeqs;
 	if (local)
 		for (int i = tid; i <= S; i += kPThreads)
 			spre[i] = a.tile_pre[i];
@@ -1308,27 +1316,22 @@ __device__ __forceinline__ void suffix_role(const kllm_prefix_args &a, uint8_t *
 		fence_mbar_init();
 	}
 	__syncthreads();
-	if (warp >= NW) {
-		if constexpr (Gm::MX)
-			asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
-		else
-			asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
-		return;
-	}
-	if constexpr (Gm::MX)
-		asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
-	else
+	if constexpr (!Gm::MX) {
+		if (warp >= NW) {
+			asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+			return;
+		}
 		asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+	}
 	const int *pre = local ? spre : a.tile_pre;
 	const int w = cta * NW + warp;
 	if (w >= WS)
 		return;
-	const long long xa = div_steps(w * N, WS), xb = div_steps((w + 1) * N, WS);
-	const int n = (int)(xb - xa);
+	const long long xa = div_steps(w * N, WS);
+	const int n = (int)(div_steps((w + 1) * N, WS) - xa);
 	uint8_t *ring = smem + Lay::ring + (size_t)warp * NST * Gm::STAGE;
 	uint64_t *bar = bars + warp * NST;
 	int *ntoks = meta + warp * NST;
-	const uint64_t policy = l2_evict_first_policy();
 	const size_t sec = Gm::MX ? (size_t)a.block_size * D * 9 / 8 : (size_t)a.block_size * D * 2;
 
 	// block-table entries of 32 consecutive tiles, one a lane: loaded a batch
@@ -1390,6 +1393,7 @@ __device__ __forceinline__ void suffix_role(const kllm_prefix_args &a, uint8_t *
 			const int st = pos % NST, ntok = pack & 0xFF, sub = pack >> 8;
 			ntoks[st] = ntok;
 			if (ntok) {
+				const uint64_t policy = l2_evict_first_policy();
 				mbar_arrive_expect_tx(&bar[st], Gm::STAGE);
 				uint8_t *dK = ring + (size_t)st * Gm::STAGE, *dV = dK + Gm::KV;
 				const uint8_t *sK = reinterpret_cast<const uint8_t *>(ek);
@@ -1523,6 +1527,8 @@ __device__ __forceinline__ void suffix_role(const kllm_prefix_args &a, uint8_t *
 	if constexpr (Gm::MX) {
 		if (redo) {                    // rare: the marked pieces of this warp, exactly
 			__syncwarp();
+			const PHeader *hd = static_cast<const PHeader *>(a.header);
+			const long long xb = div_steps((w + 1) * hd->N, hd->WS);
 			for (long long x = xa; x < xb;) {
 				const SufSeg e = locate_suffix(pre, S, H, x);
 				const int nt = (int)min((long long)(e.ts - e.j), xb - x);
@@ -1541,8 +1547,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
 attend_kernel(const kllm_prefix_args a)
 {
 	extern __shared__ __align__(1024) uint8_t smem_raw[];
-	uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-						   ~(uintptr_t)1023);
+	// an offset, not a rounded pointer: the compiler keeps to shared-memory loads
+	uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
 	// the plan this launch reads is written by the kernel before it
 	grid_dependency_wait();
 	grid_launch_dependents();
@@ -1580,15 +1586,22 @@ join_kernel(const kllm_prefix_args a, float unbias)
 	__shared__ float m_s[kJRows], l_s[kJRows];
 	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 	const int h = blockIdx.y, H = a.num_kv_heads, rows = a.num_seqs * a.group;
-	grid_dependency_wait();
+	// The plan is complete here: the attention's CTAs let this kernel start only
+	// after they have waited for it. Its partials need the wait below.
 	const PHeader *hd = static_cast<const PHeader *>(a.header);
 	const int i = blockIdx.x * kJRows + lane;
+	const int r = tid / (D / 8), part = tid % (D / 8), ii = blockIdx.x * kJRows + r;
+	const int seq2 = min(ii, rows - 1) / a.group;
+	const int t0 = a.tile_pre[seq2], ts = a.tile_pre[seq2 + 1] - t0;
+	const long long N = hd->N, WS = hd->WS;
 	{
 		const int seq = i / a.group;
 		const int g = i < rows ? a.row_group[seq] : -1;
 		float M = -CUDART_INF_F, L = 0.f;
 		float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-		if (g >= 0) {
+		if (g < 0)
+			grid_dependency_wait();
+		else {
 			const long long T = hd->T, W = hd->W;
 			const PGroup G = static_cast<const PGroup *>(a.groups)[g];
 			const int lr = (seq - G.row0) * a.group + i % a.group;
@@ -1601,6 +1614,7 @@ join_kernel(const kllm_prefix_args a, float unbias)
 			const long long c0 = div_steps((ux + 1) * W - 1, T), c1 = div_steps((ux + cost) * W - 1, T);
 			const long long base = G.r0 + (long long)h * G.alloc + tile * kUnitRows + kUnitRows * c0;
 			const int sh = solo ? 1 : 0, np = (int)(c1 - c0 + 1) << sh;
+			grid_dependency_wait();
 			for (int p0 = 0; p0 < np; p0 += kFly) {
 				float l[kFly], m[kFly];
 				float4 o[kFly][2];
@@ -1657,17 +1671,15 @@ join_kernel(const kllm_prefix_args a, float unbias)
 		}
 	}
 	__syncthreads();
-	const int r = tid / (D / 8), part = tid % (D / 8), ii = blockIdx.x * kJRows + r;
 	if (ii >= rows)
 		return;
-	const int seq = ii / a.group, hh = ii - seq * a.group;
+	const int seq = seq2, hh = ii - seq * a.group;
 	float M = m_s[r], L = l_s[r], acc[8];
 #pragma unroll
 	for (int q = 0; q < 8; ++q)
 		acc[q] = acc_s[r][part * 8 + q];
-	const int t0 = a.tile_pre[seq], ts = a.tile_pre[seq + 1] - t0;
 	if (ts > 0) {
-		const long long N = hd->N, WS = hd->WS, x0 = (long long)t0 * H + (long long)h * ts;
+		const long long x0 = (long long)t0 * H + (long long)h * ts;
 		const long long w0 = div_steps((x0 + 1) * WS - 1, N), w1 = div_steps((x0 + ts) * WS - 1, N);
 		const size_t slot = (size_t)seq * H + h + w0;
 		const int np = (int)(w1 - w0 + 1);
