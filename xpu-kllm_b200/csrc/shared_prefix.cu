@@ -30,11 +30,14 @@
 // one stream's products run under the other's softmax. Warps:
 //   0-3 / 4-7  one row a thread: queries into the operand tile, softmax of
 //              stream 0 / 1, the piece's partial
-//   8-15       producers: K and V blocks into the swizzled operand layout (MX:
-//              dequantised to f16 from staged raw pages; BF16: copied by
-//              cp.async)
-//   16         TMEM allocation and MMA issue
-//   17         page lookup and bulk copies of raw pages (three stages)
+//   8-13       producers, each on its own items of 16 keys: K and V into the
+//              swizzled operand layout. MX codes come from L2 into registers an
+//              item ahead and are placed as f16; BF16 rows are copied by cp.async,
+//              whose completion arrives on the tile's barrier by itself. With all
+//              producers on one staged tile at a time a pair of blocks took 6k
+//              cycles, 5k so (softmax 2.5-3.7k, products 1.3k).
+//   14         TMEM allocation and MMA issue
+//   15         page lookup, and the pages on their way to L2
 // MX computes in f16 like the decode: K and V are payload x scale / 4, the
 // query row times a power of two; P is one f16 (11 bits; its 2^-12 stays under
 // the output's 2^-9) built 2^7 larger, so that what underflows is below 2^-32
@@ -44,7 +47,8 @@
 // suffix_role. The decode's tiles (16 tokens of one sequence and kv head, all G
 // query heads, m16n8k16) laid end to end; each warp takes an equal contiguous
 // range, as the split-KV decode does, but leaves every piece as a partial for
-// the join, which reads them anyway: no counters, no last-arriver merge.
+// the join, which reads them anyway: no counters, no last-arriver merge. 16
+// warps a CTA (MX) read 1.26 GB at 5.2 TB/s, 12 read it at 4.8 TB/s.
 // Every wait is bounded in wall time; a timeout sets KLLM_ERR_TIMEOUT.
 
 #include "kllm_decode_tile.cuh"
@@ -61,12 +65,11 @@ constexpr int kPRows = 128, kPKeys = 128;
 constexpr int kUnitRows = 256;
 constexpr int kPThreads = 16 * 32;
 constexpr int kWarpProd = 8, kWarpMma = 14, kWarpLoad = 15;
-constexpr int kProd = 192;                    // producer threads
+constexpr int kPW = 6;                        // producer warps
 // Registers: 512 threads launch with 128 each, all of an SM's. A softmax thread
 // holds 128 scores (256 x 160 + 256 x 96); a suffix warp's MX tile takes the 128,
 // its BF16 tile 184 (256 x 184 + 256 x 72).
-constexpr int kRaw = 3;                       // raw stages (MX) / page-address stages (BF16)
-constexpr int kRawKeys = 64;                  // keys of a raw stage
+constexpr int kPg = 4;                        // blocks whose page addresses are known
 constexpr float kRaise = 8.f;                 // slack of the lazy reference maximum, log2
 constexpr float kPShift = 7.f;                // f16 P is built 2^7 larger
 constexpr uint64_t kPWaitNs = 200000000ull;
@@ -96,8 +99,10 @@ static_assert(sizeof(PHeader) == 64 && sizeof(PGroup) == 48, "workspace layout")
 
 constexpr int kPlanThreads = 1024;
 // A CTA's time for n steps or for n tiles a warp, in ns, as measured on the
-// whole chip: set-up, then the rate. They only balance the two parts.
-constexpr float kStepSetNs = 10500.f, kStepNsMx = 1500.f, kStepNsBf16 = 2700.f, kTileSetNs = 5000.f, kTileNs = 2500.f;
+// whole chip: set-up, then the rate. They only balance the two parts; for 256
+// rows of 8,192 shared tokens any split from 96 to 108 CTAs of 148 is within 4%.
+constexpr float kStepSetNs = 10500.f, kStepNsMx = 1500.f, kStepNsBf16 = 2700.f;
+constexpr float kTileSetNs = 5000.f, kTileNs = 2500.f;
 
 struct PlanSmem {
 	long long w0[32], w1[32];
@@ -282,9 +287,8 @@ struct PG {
 	static constexpr int NH = D / 64;                     // 64-column halves
 	static constexpr int HALF = kPRows * 128;             // bytes of one half tile
 	static constexpr int TILE = NH * HALF;
-	static constexpr int RAW = MX ? kRawKeys * D : 16;    // payload of half a block
-	static constexpr int RAWS = MX ? kRawKeys * D / 8 : 16;  // its scales
-	static constexpr int LPR = D / 8;                     // 16-byte chunks of a bf16 row
+	static constexpr int FILL = kPKeys / 16 * (MX ? 1 : 32);  // arrivals that fill a tile
+	static constexpr int LPR = MX ? D / 16 : D / 8;       // 16-byte pieces of a row
 };
 
 template <int D, int KVT>
@@ -293,15 +297,12 @@ struct PrefixSmem {
 	uint8_t q[2][G::TILE];
 	uint8_t k[2][G::TILE];
 	uint8_t v[2][G::TILE];
-	uint8_t raw[kRaw][G::RAW];            // [64 keys][D] payload
-	uint8_t raws[kRaw][G::RAWS];          // [64 keys][D / 8] scales
 	float qf[2][kPRows];                  // 2^-e of a solo piece's query rows, by piece parity
-	unsigned long long pg[kRaw][2][8];    // page addresses of a block (BF16)
-	uint32_t slot_ok[kRaw];               // pages present, one bit each
-	uint32_t key_ok[4][4];                // key masks of the last four blocks
+	unsigned long long pg[kPg][2][8];     // section addresses of a block's pages, 0: absent
+	alignas(16) uint32_t key_ok[8][4];    // key masks of the last eight blocks
 	uint64_t q_full, q_empty;
 	uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-	uint64_t raw_full[kRaw], raw_empty[kRaw];
+	uint64_t pg_full[kPg], pg_empty[kPg];
 	uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
 	uint64_t drain;
 	uint32_t tmem_base;
@@ -411,13 +412,13 @@ __device__ __forceinline__ uint32_t place_pair(uint32_t x)
 	return h + (h & 0x40004000u);
 }
 
-// Sixteen codes (two scale blocks) of a row -> 16 f16 values payload x scale /
-// 4, the second block's eight in `hi`: the scale is placed and multiplied by
-// 2^14, which makes it x 64, and x 64 x 2^-8 is / 4.
-__device__ __forceinline__ void mx16_to_f16(uint2 wl, uint2 wh, uint32_t scl, uint32_t sch, uint4 &lo,
-					    uint4 &hi)
+// Sixteen codes (two scale blocks, their codes in bytes 0 and 2 of sc) of a row
+// -> 16 f16 values payload x scale / 4, the second block's eight in `hi`: the
+// scale is placed and multiplied by 2^14, which makes it x 64, and x 64 x 2^-8
+// is / 4.
+__device__ __forceinline__ void mx16_to_f16(uint2 wl, uint2 wh, uint32_t sc, uint4 &lo, uint4 &hi)
 {
-	const uint32_t s = f16x2_mul(place_pair(scl | (sch << 16)), 0x74007400u);
+	const uint32_t s = f16x2_mul(place_pair(sc), 0x74007400u);
 	const uint32_t s0 = __byte_perm(s, 0u, 0x1010u), s1 = __byte_perm(s, 0u, 0x3232u);
 	lo.x = f16x2_mul(place_pair(__byte_perm(wl.x, 0u, 0x4140u)), s0);
 	lo.y = f16x2_mul(place_pair(__byte_perm(wl.x, 0u, 0x4342u)), s0);
@@ -427,55 +428,6 @@ __device__ __forceinline__ void mx16_to_f16(uint2 wl, uint2 wh, uint32_t scl, ui
 	hi.y = f16x2_mul(place_pair(__byte_perm(wh.x, 0u, 0x4342u)), s1);
 	hi.z = f16x2_mul(place_pair(__byte_perm(wh.y, 0u, 0x4140u)), s1);
 	hi.w = f16x2_mul(place_pair(__byte_perm(wh.y, 0u, 0x4342u)), s1);
-}
-
-// Half a raw block -> rows key0 .. key0 + 63 of the operand tile [128 keys][D]
-// f16, 128-byte swizzle, by the producers; rows of absent pages are zeros. A
-// lane takes 16 codes as two 8-byte chunks; lanes of the upper 64 columns take
-// them in the other order, so that the eight lanes of a row never store to one
-// bank. All loads come before the stores: the compiler cannot tell that the
-// tiles do not overlap.
-template <int D>
-__device__ __forceinline__ void dequant_half(uint8_t *dst, int key0, const uint8_t *raw, const uint8_t *rs,
-					     const uint32_t *mask, bool full, int pt)
-{
-	constexpr int LPR = D / 16, RPP = kProd / LPR, kPass = (kRawKeys + RPP - 1) / RPP;
-	const int l = pt % LPR, row0 = pt / LPR;
-	const bool part = row0 + (kPass - 1) * RPP < kRawKeys;   // the last pass; warp-uniform
-	const int first = l >= 4 ? 1 : 0;
-	const int c0 = (2 * l) & 7;
-	// RPP and key0 are multiples of 8, so the swizzle of a lane's rows is the same
-	uint8_t *o0 = dst + (l >> 2) * (kPRows * 128) + swz(key0 + row0, c0 + first);
-	uint8_t *o1 = dst + (l >> 2) * (kPRows * 128) + swz(key0 + row0, c0 + 1 - first);
-	const uint8_t *pl = raw + row0 * D + l * 16 + 8 * first, *ph = raw + row0 * D + l * 16 + 8 * (1 - first);
-	const uint8_t *sl = rs + row0 * (D / 8) + l * 2 + first, *sh = rs + row0 * (D / 8) + l * 2 + 1 - first;
-	uint2 wl[kPass], wh[kPass];
-	uint32_t a[kPass], b[kPass];
-#pragma unroll
-	for (int u = 0; u < kPass; ++u) {
-		if (u == kPass - 1 && !part)
-			continue;
-		wl[u] = *reinterpret_cast<const uint2 *>(pl + u * RPP * D);
-		wh[u] = *reinterpret_cast<const uint2 *>(ph + u * RPP * D);
-		a[u] = sl[u * RPP * (D / 8)];
-		b[u] = sh[u * RPP * (D / 8)];
-	}
-	if (!full)
-#pragma unroll
-		for (int u = 0; u < kPass; ++u) {
-			const int row = key0 + row0 + u * RPP;
-			if (row < kPKeys && !((mask[row >> 5] >> (row & 31)) & 1u))
-				wl[u] = wh[u] = make_uint2(0u, 0u);
-		}
-#pragma unroll
-	for (int u = 0; u < kPass; ++u) {
-		if (u == kPass - 1 && !part)
-			continue;
-		uint4 lo, hi;
-		mx16_to_f16(wl[u], wh[u], a[u], b[u], lo, hi);
-		*reinterpret_cast<uint4 *>(o0 + u * RPP * 128) = lo;
-		*reinterpret_cast<uint4 *>(o1 + u * RPP * 128) = hi;
-	}
 }
 
 __device__ __forceinline__ void cp_async16(void *dst, const void *src)
@@ -490,6 +442,12 @@ __device__ __forceinline__ void bulk_prefetch_l2(const void *src, uint32_t bytes
 __device__ __forceinline__ void cp_async_commit()
 {
 	asm volatile("cp.async.commit_group;" ::: "memory");
+}
+// One arrival on `bar` (counted at its initialisation) once this thread's copies
+// so far are done.
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar)
+{
+	asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void cp_async_wait()
@@ -660,18 +618,18 @@ __device__ __forceinline__ void init_prefix(PrefixSmem<D, KVT> &sm)
 	mbar_init(&sm.q_full, 256);
 	mbar_init(&sm.q_empty, 1);
 	for (int i = 0; i < 2; ++i) {
-		mbar_init(&sm.k_full[i], kProd);
+		mbar_init(&sm.k_full[i], PG<D, KVT>::FILL);
 		mbar_init(&sm.k_empty[i], 1);
-		mbar_init(&sm.v_full[i], kProd);
+		mbar_init(&sm.v_full[i], PG<D, KVT>::FILL);
 		mbar_init(&sm.v_empty[i], 1);
 		mbar_init(&sm.s_full[i], 1);
 		mbar_init(&sm.p_half[i], 128);
 		mbar_init(&sm.p_full[i], 128);
 		mbar_init(&sm.o_full[i], 1);
 	}
-	for (int i = 0; i < kRaw; ++i) {
-		mbar_init(&sm.raw_full[i], 1);
-		mbar_init(&sm.raw_empty[i], kProd);
+	for (int i = 0; i < kPg; ++i) {
+		mbar_init(&sm.pg_full[i], 1);
+		mbar_init(&sm.pg_empty[i], kPW);
 	}
 	mbar_init(&sm.drain, 1);
 	sm.abort = 0;
@@ -705,7 +663,7 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 
 	if (warp < kWarpProd) {
 		// ================= softmax of stream t ========================================
-		asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
 		const int t = warp >> 2, rr = (warp & 3) * 32 + lane;
 		const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
 		const uint32_t tS = lane_base + col_s(t), tO = lane_base + col_o(t);
@@ -756,7 +714,7 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 					      (G::MX ? (p.solo && t ? sm.qf[np & 1][rr] : qf) * KLLM_MX_DEC_UNBIAS
 						     : 1.f);
 				if (warp_live)
-					softmax_rows<D, KVT>(tS, tO, sm.key_ok[(kf + j) & 3], sl2, !first, m_ref,
+					softmax_rows<D, KVT>(tS, tO, sm.key_ok[(kf + j) & 7], sl2, !first, m_ref,
 							     l_sum, &sm.p_half[t]);
 				else
 					mbar_arrive(&sm.p_half[t]);
@@ -801,9 +759,16 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 		}
 	} else if (warp < kWarpMma) {
 		// ================= producers ====================================================
-		asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-		const int pt = tid - kWarpProd * 32;
-		int kf = 0, vf = 0, rf = 0;                  // K fills, V fills, raw stages
+		asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+		// An item is 16 keys of K or V of one block (never more than one page), 16
+		// items a block, and each warp takes every kPW-th on its own: with all
+		// warps on one tile at a time, half of the time went into its barriers.
+		constexpr int RP = 32 / G::LPR, NP = 16 / RP;      // rows a pass, passes of an item
+		const int pw = warp - kWarpProd, l = lane % G::LPR, sub = lane / G::LPR;
+		// (key / 16) x inv16 / 256 = key / bs for keys below 128 and the block sizes
+		// 16, 32 .. 128
+		const int inv16 = 256 / (bs >> 4) + 1;
+		int gb0 = 0;                                 // blocks of the pieces before
 		bool ok = true;
 		auto wait_warp = [&](uint64_t *bar, uint32_t parity) {
 			return __all_sync(0xffffffffu, wait(bar, parity));
@@ -812,114 +777,124 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 			const Piece p = next_piece(a, x, xe, cta);
 			if (p.nb <= 0)
 				continue;
-			// ---- K and V blocks ---------------------------------------------------------
-			const uint32_t all_pages = (1u << ppb) - 1u;
-			// key bits of word w of a block whose pages present are okm
-			auto key_mask = [&](uint32_t okm, int w) {
-				uint32_t m = 0;
-#pragma unroll
-				for (int i = 0; i < 2; ++i) {
-					const int page = (32 * w + 16 * i) / bs;
-					if (page < ppb && ((okm >> page) & 1u))
-						m |= 0xFFFFu << (16 * i);
+			const int n_it = p.nb * 16;
+			int cur = -1;                            // block whose addresses are here
+			// this lane's first byte of item i; 0 when its page is absent. The first
+			// item of a block waits for its addresses, the last one frees them.
+			auto locate = [&](int i, int &row) {
+				const int j = i >> 4, slot = (gb0 + j) % kPg, key = (i & 7) * 16;
+				if (j != cur) {
+					ok = ok && wait_warp(&sm.pg_full[slot], (uint32_t)(((gb0 + j) / kPg) & 1));
+					cur = j;
 				}
-				return m;
+				const int page = ((key >> 4) * inv16) >> 8;
+				row = key - page * bs + sub;
+				const unsigned long long at = ok ? sm.pg[slot][(i >> 3) & 1][page] : 0ull;
+				__syncwarp();
+				if (((i + kPW) >> 4) != j && lane == 0)
+					mbar_arrive(&sm.pg_empty[slot]);
+				return at;
+			};
+			auto full_bar = [&](int i) {
+				const int b = (gb0 + (i >> 4)) & 1;
+				return (i & 8) ? &sm.v_full[b] : &sm.k_full[b];
+			};
+			auto tile_of = [&](int i) {
+				const int b = (gb0 + (i >> 4)) & 1;
+				return (i & 8) ? sm.v[b] : sm.k[b];
+			};
+			auto empty_bar = [&](int i) {
+				const int b = (gb0 + (i >> 4)) & 1;
+				return (i & 8) ? &sm.v_empty[b] : &sm.k_empty[b];
 			};
 			if constexpr (G::MX) {
-				for (int j = 0; j < p.nb && ok; ++j)
-					for (int which = 0; which < 2 && ok; ++which) {
-						int &cnt = which ? vf : kf;
-						uint64_t *empty = which ? &sm.v_empty[cnt & 1] : &sm.k_empty[cnt & 1];
-						ok = cnt < 2 || wait_warp(empty, (uint32_t)(((cnt >> 1) - 1) & 1));
-						uint8_t *dst = which ? sm.v[cnt & 1] : sm.k[cnt & 1];
-#pragma unroll 1
-						for (int half = 0; half < 2 && ok; ++half, ++rf) {
-							const int st = rf % kRaw;
-							ok = wait_warp(&sm.raw_full[st], (uint32_t)((rf / kRaw) & 1));
-							if (!ok)
-								break;
-							const uint32_t okm = sm.slot_ok[st];
-							// all pages present and no key past the last one
-							const bool full = okm == all_pages && ppb * bs == kPKeys;
-							uint32_t mk[4] = {~0u, ~0u, ~0u, ~0u};
-							if (!full)
+				// an item's codes and scales go to registers while the item before is
+				// placed
+				uint4 cw[NP], nw[NP];
+				uint32_t cs[NP], ns[NP];
+				auto fetch = [&](int i, uint4 (&w)[NP], uint32_t (&sc)[NP]) {
+					int row;
+					const unsigned long long at = locate(i, row);
+					const uint8_t *pay = reinterpret_cast<const uint8_t *>(at) + row * D + l * 16;
+					const uint8_t *scl = reinterpret_cast<const uint8_t *>(at) + bs * D + row * (D / 8) + 2 * l;
 #pragma unroll
-								for (int w = 0; w < 4; ++w)
-									mk[w] = key_mask(okm, w);
-							dequant_half<D>(dst, half * kRawKeys, sm.raw[st], sm.raws[st], mk, full,
-									pt);
-							if (which == 0 && half == 0 && pt == 0)
-#pragma unroll
-								for (int w = 0; w < 4; ++w)
-									sm.key_ok[kf & 3][w] = mk[w];
-							mbar_arrive(&sm.raw_empty[st]);
+					for (int u = 0; u < NP; ++u) {
+						w[u] = make_uint4(0u, 0u, 0u, 0u);
+						sc[u] = 0u;
+						if (at) {
+							w[u] = __ldcg(reinterpret_cast<const uint4 *>(pay + u * RP * D));
+							sc[u] = __ldcg(reinterpret_cast<const unsigned short *>(scl + u * RP * (D / 8)));
 						}
-						if (!ok)
-							break;
-						fence_async_smem();
-						mbar_arrive(which ? &sm.v_full[cnt & 1] : &sm.k_full[cnt & 1]);
-						++cnt;
 					}
-			} else {
-				// fills run two ahead of their arrival: K0 V0 K1 V1 ...
-				const int l = pt % G::LPR;
-				const int kf0 = kf, n_fill = 2 * p.nb;
-				// (row / 16) x inv16 / 256 = row / bs for rows below 128 and the block
-				// sizes 16, 32 .. 128
-				const int inv16 = 256 / (bs >> 4) + 1;
-				auto arrive_fill = [&](int f) {
-					const int b = (kf0 + (f >> 1)) & 1;
-					mbar_arrive((f & 1) ? &sm.v_full[b] : &sm.k_full[b]);
 				};
-				for (int f = 0; f < n_fill; ++f) {
-					const int which = f & 1, st = rf % kRaw;
-					int &cnt = which ? vf : kf;
-					uint64_t *empty = which ? &sm.v_empty[cnt & 1] : &sm.k_empty[cnt & 1];
-					if (which == 0)
-						ok = wait_warp(&sm.raw_full[st], (uint32_t)((rf / kRaw) & 1));
-					ok = ok && (cnt < 2 || wait_warp(empty, (uint32_t)(((cnt >> 1) - 1) & 1)));
+				// Lanes of the upper 64 columns store their second chunk first, so that
+				// the eight lanes of a row never store to one bank.
+				const bool swap = l >= 4;
+				const uint32_t pick = swap ? 0x4041u : 0x4140u;
+				const int c0 = (2 * l) & 7, half = (l >> 2) * G::HALF;
+				auto place = [&](int i, const uint4 (&w)[NP], const uint32_t (&sc)[NP]) {
+					const int cnt = gb0 + (i >> 4);
+					ok = ok && (cnt < 2 || wait_warp(empty_bar(i), (uint32_t)(((cnt >> 1) - 1) & 1)));
+					if (!ok)
+						return;
+					uint8_t *dst = tile_of(i) + half;
+#pragma unroll
+					for (int u = 0; u < NP; ++u) {
+						const uint2 wa = make_uint2(w[u].x, w[u].y), wb = make_uint2(w[u].z, w[u].w);
+						uint4 lo, hi;
+						mx16_to_f16(swap ? wb : wa, swap ? wa : wb, __byte_perm(sc[u], 0u, pick), lo, hi);
+						const int row = (i & 7) * 16 + u * RP + sub;
+						*reinterpret_cast<uint4 *>(dst + swz(row, c0 + (swap ? 1 : 0))) = lo;
+						*reinterpret_cast<uint4 *>(dst + swz(row, c0 + (swap ? 0 : 1))) = hi;
+					}
+					fence_async_smem();
+					__syncwarp();
+					if (lane == 0)
+						mbar_arrive(full_bar(i));
+				};
+				fetch(pw, cw, cs);
+#pragma unroll 1
+				for (int i = pw; i < n_it && ok; i += 2 * kPW) {
+					if (i + kPW < n_it)
+						fetch(i + kPW, nw, ns);
+					place(i, cw, cs);
+					if (i + 2 * kPW < n_it)
+						fetch(i + 2 * kPW, cw, cs);
+					if (i + kPW < n_it && ok)
+						place(i + kPW, nw, ns);
+				}
+			} else {
+				// copies run as far ahead as buffers are free; their completion arrives
+				// on the barrier by itself, and the MMA warp has the proxy fence
+				for (int i = pw; i < n_it; i += kPW) {
+					int row;
+					const unsigned long long at = locate(i, row);
+					const int cnt = gb0 + (i >> 4);
+					ok = ok && (cnt < 2 || wait_warp(empty_bar(i), (uint32_t)(((cnt >> 1) - 1) & 1)));
 					if (!ok)
 						break;
-					const uint32_t okm = sm.slot_ok[st];
-					uint8_t *dst = (which ? sm.v[cnt & 1] : sm.k[cnt & 1]) + (l >> 3) * G::HALF;
-					constexpr int RPP = kProd / G::LPR;
-#pragma unroll 4
-					for (int row = pt / G::LPR; row < kPKeys; row += RPP) {
-						uint8_t *o = dst + swz(row, l & 7);
-						const int page = ((row >> 4) * inv16) >> 8;        // row / bs
-						if ((okm >> page) & 1u)                            // never past the last page
-							cp_async16(o, reinterpret_cast<const uint8_t *>(sm.pg[st][which][page]) +
-									  (row - page * bs) * (D * 2) + l * 16);
+					uint8_t *dst = tile_of(i) + (l >> 3) * G::HALF;
+					const uint8_t *src = reinterpret_cast<const uint8_t *>(at) + row * (D * 2) + l * 16;
+#pragma unroll
+					for (int u = 0; u < NP; ++u) {
+						uint8_t *o = dst + swz((i & 7) * 16 + u * RP + sub, l & 7);
+						if (at)
+							cp_async16(o, src + u * RP * (D * 2));
 						else
 							*reinterpret_cast<uint4 *>(o) = make_uint4(0u, 0u, 0u, 0u);
 					}
-					cp_async_commit();
-					if (which == 0) {
-						if (pt < 4)
-							sm.key_ok[kf & 3][pt] = key_mask(okm, pt);
-					} else {
-						mbar_arrive(&sm.raw_empty[st]);
-						++rf;
-					}
-					++cnt;
-					if (f >= 2) {
-						cp_async_wait<2>();
-						fence_async_smem();
-						arrive_fill(f - 2);
-					}
+					if (at)
+						cp_async_arrive(full_bar(i));
+					else
+						mbar_arrive(full_bar(i));
 				}
-				// the piece's last two fills
+				cp_async_commit();
 				cp_async_wait<0>();
-				fence_async_smem();
-				if (ok) {
-					if (n_fill >= 2)
-						arrive_fill(n_fill - 2);
-					arrive_fill(n_fill - 1);
-				}
 			}
+			gb0 += p.nb;
 		}
 	} else {
-	asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+	asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
 	if (warp == kWarpMma) {
 		// ================= MMA issue =======================================================
 		// The whole warp runs this role (descriptors stay warp-uniform); one
@@ -943,7 +918,11 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 		};
 		auto wait_k = [&]() {
 			const int b = kf & 1, round = kf >> 1;
-			return wait_all(&sm.k_full[b], (uint32_t)(round & 1));
+			if (!wait_all(&sm.k_full[b], (uint32_t)(round & 1)))
+				return false;
+			if constexpr (!G::MX)
+				fence_async_smem();
+			return true;
 		};
 		auto free_k = [&]() {
 			commit(&sm.k_empty[kf & 1]);
@@ -1020,6 +999,8 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 				ok = wait_all(&sm.v_full[vf & 1], (uint32_t)((vf >> 1) & 1));
 				if (!ok)
 					break;
+				if constexpr (!G::MX)
+					fence_async_smem();
 				if (p.solo) {
 					const int t = j & 1;
 					ok = take_p(t, j < 2);
@@ -1070,8 +1051,7 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 		mbar_wait_ns(&sm.drain, 0u, kPWaitNs);
 	} else if (warp == kWarpLoad) {
 		// ================= page lookup and raw copies ========================================
-		int rf = 0;
-		uint32_t armed[kRaw] = {0, 0, 0};
+		int gb = 0;                                  // blocks posted
 		bool ok = true;
 		while (x < xe && ok) {
 			const Piece p = next_piece(a, x, xe, cta);
@@ -1121,55 +1101,31 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 				check(cur);
 				nxt = load(p.b0 + j + 2);
 				const uint32_t mask = __ballot_sync(0xffffffffu, e.valid);
-				for (int part = 0; part < (G::MX ? 4 : 1); ++part, ++rf) {
-					const int st = rf % kRaw;
-					if (rf >= kRaw)
-						ok = __all_sync(0xffffffffu, wait(&sm.raw_empty[st],
-										  (uint32_t)((rf / kRaw - 1) & 1)));
-					if (!ok)
-						break;
-					if constexpr (G::MX) {
-						// rows r0 .. r1 - 1 of the block: this lane's page in this half
-						const int key0 = (part & 1) * kRawKeys;
-						const int r0 = max(lane * bs, key0), r1 = min(lane * bs + bs, key0 + kRawKeys);
-						const int n = e.valid ? max(r1 - r0, 0) : 0;
-						const uint32_t rows = __reduce_add_sync(0xffffffffu, (uint32_t)n);
-						if (lane == 0) {
-							sm.slot_ok[st] = mask;
-							mbar_arrive_expect_tx(&sm.raw_full[st], rows * (uint32_t)(D * 9 / 8));
-						}
-#pragma unroll
-						for (int i = 0; i < kRaw; ++i)
-							armed[i] += i == st ? 1u : 0u;
-						__syncwarp();
-						if (n > 0) {
-							const uint8_t *src = reinterpret_cast<const uint8_t *>(part >> 1 ? e.v : e.k);
-							const int pr = r0 - lane * bs;         // row of the page
-							bulk_g2s(sm.raw[st] + (r0 - key0) * D, src + pr * D, (uint32_t)(n * D),
-								 &sm.raw_full[st]);
-							bulk_g2s(sm.raws[st] + (r0 - key0) * (D / 8), src + bs * D + pr * (D / 8),
-								 (uint32_t)(n * (D / 8)), &sm.raw_full[st]);
-						}
-					} else {
-						if (lane < 8) {
-							sm.pg[st][0][lane] = e.k;
-							sm.pg[st][1][lane] = e.v;
-						}
-						if (lane == 0)
-							sm.slot_ok[st] = mask;
-						__syncwarp();
-						if (lane == 0)
-							mbar_arrive(&sm.raw_full[st]);
-					}
+				const int slot = gb % kPg;
+				if (gb >= kPg)
+					ok = __all_sync(0xffffffffu, wait(&sm.pg_empty[slot], (uint32_t)((gb / kPg - 1) & 1)));
+				if (!ok)
+					break;
+				if (lane < 8) {
+					sm.pg[slot][0][lane] = e.valid ? e.k : 0ull;
+					sm.pg[slot][1][lane] = e.valid ? e.v : 0ull;
 				}
+				if (lane < 4) {                        // keys 32 lane .. 32 lane + 31
+					uint32_t m = 0;
+#pragma unroll
+					for (int i = 0; i < 2; ++i) {
+						const int page = (32 * lane + 16 * i) / bs;
+						if (page < ppb && ((mask >> page) & 1u))
+							m |= 0xFFFFu << (16 * i);
+					}
+					sm.key_ok[gb & 7][lane] = m;
+				}
+				__syncwarp();
+				if (lane == 0)
+					mbar_arrive(&sm.pg_full[slot]);
+				++gb;
 			}
 		}
-		// after an abort, wait (bounded) for this CTA's own bulk copies
-		if (G::MX && *reinterpret_cast<volatile int *>(&sm.abort))
-#pragma unroll
-			for (int i = 0; i < kRaw; ++i)
-				if (armed[i] > 0)
-					mbar_wait_ns(&sm.raw_full[i], (armed[i] - 1) & 1u, kPWaitNs);
 	}
 	}
 
