@@ -33,6 +33,7 @@
 #include "kllm_internal.h"
 #include "kllm_topk.cuh"
 
+#include <cfloat>
 #include <cooperative_groups.h>
 
 namespace cg = cooperative_groups;
@@ -57,7 +58,9 @@ struct LpSmem {
 	int n_cand;                           // rank 0's
 	int short_list[kCandCap];             // candidates that reach the last threshold
 	int n_short;
-	float tl[kTgtMax];                    // the targets' logits
+	float tl[kTgtMax];                    // the targets' logits (+inf: no such target)
+	int ti[kTgtMax];                      // their indices
+	float tau_run;                        // the last threshold a warp found, only ever raised
 	float tau;
 	float sub;                            // what logprobs subtract: lse, 0 in an empty row
 	uint32_t hist[256];
@@ -324,8 +327,8 @@ __device__ __noinline__ void recollect(const typename Elem<BF16>::T *row, int V,
 		radix_candidates<BF16, TH>(row, V, k, sm);
 }
 
-// NT: targets counted in the pass (0, 1, up to 4, up to kTgtMax). TH threads.
-template <int BF16, int NT, int TH>
+// TH threads.
+template <int BF16, int TH>
 __global__ void __launch_bounds__(TH, 1024 / TH)
 logprobs_kernel(const kllm_logprobs_args a)
 {
@@ -345,8 +348,10 @@ logprobs_kernel(const kllm_logprobs_args a)
 	LpSmem *lead = cl.map_shared_rank(&sm, 0);
 	if (tid < 32)
 		sm.gkey[tid] = sm.all_key[tid] = 0u;  // below every number's key
-	if (tid == 0)
+	if (tid == 0) {
 		sm.n_cand = sm.n_short = 0;
+		sm.tau_run = -CUDART_INF_F;
+	}
 	// every CTA of the cluster runs, its memory set, before another writes to it
 	if (CL > 1)
 		cl.sync();
@@ -358,30 +363,16 @@ logprobs_kernel(const kllm_logprobs_args a)
 	const float inv_t = temp > 0.f ? 1.f / temp : 1.f;
 	const float c = kLog2e * inv_t;
 
-	// A target counts the elements above it, and its equals at lower indices: >=
-	// in the batches before the one it lies in, > in those after it, and one by
-	// one in that one.
-	constexpr int NTA = NT > 0 ? NT : 1;
-	float tl[NTA];
-	int ti[NTA], cnt[NTA];
-	if constexpr (NT > 0) {
-#pragma unroll
-		for (int j = 0; j < NT; ++j) {
-			const int t = j < nt ? a.targets[(size_t)r * nt + j] : -1;
-			ti[j] = (t >= 0 && t < V) ? t : -1;
-			tl[j] = ti[j] >= 0 ? Elem<BF16>::get(row + ti[j]) : CUDART_INF_F;
-			cnt[j] = 0;
-			if (tid == 0)
-				sm.tl[j] = tl[j];
-		}
-	}
-
 	// ---- one pass: this thread's (m, S, W), ranks, segment maxima --------------
 	// A batch at a time: one maximum, one look at the reference and one at each
 	// target's place for its 32 elements (a vector at a time these took 35
 	// instructions an element, and the pass was bound by them). Its loads are in
 	// flight together; the 32 warps of an SM hide each other's.
+	// What rarely happens is a rolled loop that reads its vector again: unrolled
+	// over the batch and the targets it was half of the instructions, and the
+	// fetches of its code stalled the rest (999 rows of 32,003 bf16: 41 us).
 	float m = -CUDART_INF_F, S = 0.f, W = 0.f, tau = -CUDART_INF_F;
+	int rank_n = 0;                               // lane j: target j's rank so far
 #pragma unroll 1
 	for (int it = 0, here = b0; it == 0 || here < U; ++it, here += stride) {
 		float x[kFly][kVec];
@@ -396,6 +387,12 @@ logprobs_kernel(const kllm_logprobs_args a)
 			for (int q = 0; q < kFly; ++q)
 				raw[q] = load_raw<BF16>(row, mis, V, here + q * kStep + lane * kVec);
 		}                                                      // past the end: all -inf
+		if (it == 0 && tid < nt) {
+			const int t = a.targets[(size_t)r * nt + tid];
+			const bool in = t >= 0 && t < V;
+			sm.ti[tid] = in ? t : -1;
+			sm.tl[tid] = in ? Elem<BF16>::get(row + t) : CUDART_INF_F;
+		}
 #pragma unroll
 		for (int q = 0; q < kFly; ++q)
 			Elem<BF16>::unpack(raw[q], x[q]);
@@ -436,46 +433,78 @@ logprobs_kernel(const kllm_logprobs_args a)
 		unpack2(w2, wa, wb);
 		S += sa + sb;
 		W += wa + wb;
-		if constexpr (NT > 0) {
+		if (k > 0)
+			atomicMax(&sm.gkey[lane], key_of(bm));
+		if (it == 0)
+			__syncthreads();  // the targets are here, all warps' first batches in the groups
+		// A target counts the elements above it, and its equals at lower indices:
+		// >= in the batches before the one it lies in, > in those after it, and one
+		// by one in that one. A batch below the target counts nothing.
+#pragma unroll 1
+		for (int j = 0; j < nt; ++j) {
+			const float t = sm.tl[j];
+			if (!__any_sync(0xffffffffu, bm >= t))
+				continue;
+			const int rel = sm.ti[j] + mis - here;             // place in the batch
+			int n;
+			if (rel >= kBatch) {                               // the same for the whole warp
+				n = Elem<BF16>::count(raw, t, true);
+			} else if (rel < 0) {
+				n = Elem<BF16>::count(raw, t, false);
+			} else {
+				n = 0;
 #pragma unroll
-			for (int j = 0; j < NT; ++j)
-				if (j < nt) {
-					const int rel = ti[j] + mis - here;        // place in the batch
-					const float t = tl[j];
-					if (rel >= kBatch)                         // the same for the whole warp
-						cnt[j] += Elem<BF16>::count(raw, t, true);
-					else if (rel < 0)
-						cnt[j] += Elem<BF16>::count(raw, t, false);
-					else {
+				for (int q = 0; q < kFly; ++q) {
+					float y[kVec];
+					Elem<BF16>::unpack(raw[q], y);
 #pragma unroll
-						for (int q = 0; q < kFly; ++q)
-#pragma unroll
-							for (int z = 0; z < kVec; ++z)
-								cnt[j] += (int)(x[q][z] > t) |
-									  ((int)(x[q][z] == t) &
-									   (int)(q * kStep + lane * kVec + z < rel));
-					}
+					for (int z = 0; z < kVec; ++z)
+						n += (int)(y[z] > t) |
+						     ((int)(y[z] == t) & (int)(q * kStep + lane * kVec + z < rel));
 				}
+			}
+			n = __reduce_add_sync(0xffffffffu, n);
+			if (lane == j)
+				rank_n += n;
 		}
 		if (k > 0) {
-			atomicMax(&sm.gkey[lane], key_of(bm));
-			if (it == 0)
-				__syncthreads();          // all warps' first batches are in the groups
-			if ((it & (it + 1)) == 0)         // after 1, 2, 4, 8 .. batches
+			if (it == 0) {
 				tau = group_tau(sm.gkey, k, lane);
-			if (__any_sync(0xffffffffu, bm >= tau && bm > -CUDART_INF_F)) {
+			} else if ((it & (it + 1)) == 0 && __popc(it) % kWarps == warp) {
+				// after 2, 4, 8 .. batches, by one warp for all: an old threshold
+				// only collects more
+				tau = group_tau(sm.gkey, k, lane);
+				if (lane == 0)
+					*reinterpret_cast<volatile float *>(&sm.tau_run) = tau;
+			} else {
+				tau = fmaxf(tau, *reinterpret_cast<volatile float *>(&sm.tau_run));
+			}
+			const float reach = fmaxf(tau, -FLT_MAX);          // and not -inf
+			if (__any_sync(0xffffffffu, bm >= reach)) {
+				uint32_t todo = 0;                             // vectors with a candidate
 #pragma unroll
-				for (int q = 0; q < kFly; ++q)
-					if (vm[q] >= tau && vm[q] > -CUDART_INF_F)
+				for (int q = 0; q < kFly; ++q) {
+					// fp32's eight are found again: kept, they take registers the pass needs
+					float y = vm[q];
+					if constexpr (!BF16)
+						y = fmaxf(fmaxf(x[q][0], x[q][1]), fmaxf(x[q][2], x[q][3]));
+					todo |= y >= reach ? 1u << q : 0u;
+				}
+				while (todo) {
+					const int u = here + (__ffs(todo) - 1) * kStep + lane * kVec;
+					todo &= todo - 1u;
+					float y[kVec];
+					Elem<BF16>::unpack(load_raw<BF16>(row, mis, V, u), y);
 #pragma unroll
-						for (int z = 0; z < kVec; ++z)
-							if (x[q][z] >= tau && x[q][z] > -CUDART_INF_F) {
-								const int at = atomicAdd(&lead->n_cand, 1);
-								if (at < kCandCap) {
-									lead->cand_v[at] = x[q][z];
-									lead->cand_i[at] = here + q * kStep + lane * kVec + z - mis;
-								}
+					for (int z = 0; z < kVec; ++z)
+						if (y[z] >= reach) {
+							const int at = atomicAdd(&lead->n_cand, 1);
+							if (at < kCandCap) {
+								lead->cand_v[at] = y[z];
+								lead->cand_i[at] = u + z - mis;
 							}
+						}
+				}
 			}
 		}
 	}
@@ -488,21 +517,13 @@ logprobs_kernel(const kllm_logprobs_args a)
 		const float w2 = __shfl_xor_sync(0xffffffffu, W, o);
 		join(m, S, W, m2, s2, w2);
 	}
-	if constexpr (NT > 0) {
-#pragma unroll
-		for (int j = 0; j < NT; ++j)
-			cnt[j] = __reduce_add_sync(0xffffffffu, cnt[j]);
-	}
 	if (lane == 0) {
 		sm.wm[warp] = m;
 		sm.ws[warp] = S;
 		sm.ww[warp] = W;
-		if constexpr (NT > 0) {
-#pragma unroll
-			for (int j = 0; j < NT; ++j)
-				sm.wr[warp][j] = cnt[j];
-		}
 	}
+	if (lane < nt)
+		sm.wr[warp][lane] = rank_n;
 	__syncthreads();
 	if (warp == 0) {
 		float M = -CUDART_INF_F, s = 0.f, w = 0.f;
@@ -525,14 +546,12 @@ logprobs_kernel(const kllm_logprobs_args a)
 			lead->cs[rank] = s;
 			lead->cw[rank] = w;
 		}
-		if constexpr (NT > 0) {
-			if (lane < NT) {
-				int n = 0;
+		if (lane < nt) {
+			int n = 0;
 #pragma unroll
-				for (int i = 0; i < kWarps; ++i)
-					n += sm.wr[i][lane];
-				lead->cr[rank][lane] = n;
-			}
+			for (int i = 0; i < kWarps; ++i)
+				n += sm.wr[i][lane];
+			lead->cr[rank][lane] = n;
 		}
 	}
 	if (CL > 1)
@@ -568,20 +587,17 @@ logprobs_kernel(const kllm_logprobs_args a)
 			if (a.entropy)
 				a.entropy[r] = dead ? 0.f : (l2 - w / s) * kLn2;
 		}
-		if constexpr (NT > 0) {
-			if (lane < nt) {
-				const int t = a.targets[(size_t)r * nt + lane];
-				const bool in = t >= 0 && t < V;
-				const float l = in ? sm.tl[lane] : -CUDART_INF_F;
-				a.target_lp[(size_t)r * nt + lane] = in ? l * inv_t - sub : -CUDART_INF_F;
-				if (a.target_rank) {
-					int n = 0;
-					for (int i = 0; i < CL; ++i)
-						n += sm.cr[i][lane];
-					if (l == -CUDART_INF_F)
-						n -= mis;               // the padding before the row read as -inf
-					a.target_rank[(size_t)r * nt + lane] = in && l == l ? n : -1;
-				}
+		if (lane < nt) {
+			const bool in = sm.ti[lane] >= 0;
+			const float l = in ? sm.tl[lane] : -CUDART_INF_F;
+			a.target_lp[(size_t)r * nt + lane] = in ? l * inv_t - sub : -CUDART_INF_F;
+			if (a.target_rank) {
+				int n = 0;
+				for (int i = 0; i < CL; ++i)
+					n += sm.cr[i][lane];
+				if (l == -CUDART_INF_F)
+					n -= mis;                   // the padding before the row read as -inf
+				a.target_rank[(size_t)r * nt + lane] = in && l == l ? n : -1;
 			}
 		}
 	}
@@ -641,7 +657,7 @@ logprobs_kernel(const kllm_logprobs_args a)
 	}
 }
 
-template <int BF16, int NT, int TH>
+template <int BF16, int TH>
 cudaError_t launch_lp(const kllm_logprobs_args &a, int cluster, cudaStream_t st)
 {
 	cudaLaunchConfig_t cfg = {};
@@ -655,11 +671,11 @@ cudaError_t launch_lp(const kllm_logprobs_args &a, int cluster, cudaStream_t st)
 	at[0].val.clusterDim.z = 1;
 	cfg.attrs = at;
 	cfg.numAttrs = 1;
-	return cudaLaunchKernelEx(&cfg, logprobs_kernel<BF16, NT, TH>, a);
+	return cudaLaunchKernelEx(&cfg, logprobs_kernel<BF16, TH>, a);
 }
 
-template <int BF16, int NT>
-cudaError_t launch_nt(const kllm_logprobs_args &a, int num_sms, cudaStream_t st)
+template <int BF16>
+cudaError_t launch_rows(const kllm_logprobs_args &a, int num_sms, cudaStream_t st)
 {
 	// A row ends in a chain of a microsecond or two that loads nothing. Long rows
 	// take 512 threads; short ones 128, so that eight share an SM and one row's
@@ -671,7 +687,7 @@ cudaError_t launch_nt(const kllm_logprobs_args &a, int num_sms, cudaStream_t st)
 	while (cluster < kMaxCluster && (long long)a.num_rows * cluster * th < 512ll * num_sms &&
 	       a.vocab / (cluster * 2) >= th / 32 * batch / 2)
 		cluster *= 2;
-	return wide ? launch_lp<BF16, NT, 512>(a, cluster, st) : launch_lp<BF16, NT, 128>(a, cluster, st);
+	return wide ? launch_lp<BF16, 512>(a, cluster, st) : launch_lp<BF16, 128>(a, cluster, st);
 }
 
 }  // namespace
@@ -682,14 +698,5 @@ using namespace kllm;
 extern "C" int kllm_logprobs_launch(const struct kllm_logprobs_args *a, int num_sms, void *stream)
 {
 	cudaStream_t st = static_cast<cudaStream_t>(stream);
-	const int nt = a->num_targets;
-	if (a->bf16)
-		return (int)(nt == 0 ? launch_nt<1, 0>(*a, num_sms, st)
-			     : nt == 1 ? launch_nt<1, 1>(*a, num_sms, st)
-			     : nt <= 4 ? launch_nt<1, 4>(*a, num_sms, st)
-				       : launch_nt<1, kTgtMax>(*a, num_sms, st));
-	return (int)(nt == 0 ? launch_nt<0, 0>(*a, num_sms, st)
-		     : nt == 1 ? launch_nt<0, 1>(*a, num_sms, st)
-		     : nt <= 4 ? launch_nt<0, 4>(*a, num_sms, st)
-			       : launch_nt<0, kTgtMax>(*a, num_sms, st));
+	return (int)(a->bf16 ? launch_rows<1>(*a, num_sms, st) : launch_rows<0>(*a, num_sms, st));
 }
