@@ -38,7 +38,7 @@ struct LaySmem {
 	int ctx[kLayRows];        // effective lengths
 	int cu[kLayRows + 1];     // exclusive sums of new tokens (cut at INT32_MAX)
 	int first[kLayRows];      // exclusive sums of wanted blocks
-	unsigned long long warp_sum[32];
+	unsigned long long warp_tok[32], warp_blk[32];
 };
 
 // ctx and new of row s after clamping and the fork rules. Two rows' lengths
@@ -85,6 +85,24 @@ __device__ __forceinline__ bool free_entry(const kllm_layout_args &a, long long 
 	return true;
 }
 
+// Blocks of n tokens; n is at most 2^31 - 1 and the sum stays in 32 bits unsigned.
+__device__ __forceinline__ int blocks_of(int n, int bs)
+{
+	return (int)(((unsigned)n + (unsigned)bs - 1u) / (unsigned)bs);
+}
+
+// x / d for quotients below 2^52, inv = 1 / d: a 64-bit division is some 100
+// instructions, and a decode step's tokens all need one.
+__device__ __forceinline__ unsigned long long div_small(unsigned long long x, unsigned long long d, double inv)
+{
+	unsigned long long q = (unsigned long long)((double)x * inv);    // off by one at most
+	if (q * d > x)
+		--q;
+	else if (x - q * d >= d)
+		++q;
+	return q;
+}
+
 __device__ __forceinline__ unsigned long long warp_incl(unsigned long long x, int lane)
 {
 #pragma unroll
@@ -118,40 +136,35 @@ layout_kernel(const kllm_layout_args a)
 		if (s < S) {
 			int parent;
 			row_lengths(a, s, ctx[i], nw[i], parent, flags);
-			need[i] = (int)(((long long)ctx[i] + nw[i] + bs - 1) / bs -
-					((long long)ctx[i] + bs - 1) / bs);
+			need[i] = blocks_of(ctx[i] + nw[i], bs) - blocks_of(ctx[i], bs);
 			sm.ctx[s] = ctx[i];
 		}
 		tok += (unsigned long long)nw[i];
 		blk += (unsigned long long)need[i];
 	}
-	unsigned long long total[2];
-	unsigned long long mine[2] = {tok, blk};
+	const unsigned long long it = warp_incl(tok, lane), ib = warp_incl(blk, lane);
+	if (lane == 31) {
+		sm.warp_tok[warp] = it;
+		sm.warp_blk[warp] = ib;
+	}
+	__syncthreads();
+	if (warp < 2) {
+		unsigned long long *w = warp ? sm.warp_blk : sm.warp_tok;
+		w[lane] = warp_incl(w[lane], lane);
+	}
+	__syncthreads();
+	const unsigned long long total[2] = {sm.warp_tok[31], sm.warp_blk[31]};
+	unsigned long long run_t = (warp ? sm.warp_tok[warp - 1] : 0ull) + it - tok;
+	unsigned long long run_b = (warp ? sm.warp_blk[warp - 1] : 0ull) + ib - blk;
 #pragma unroll
-	for (int q = 0; q < 2; ++q) {
-		const unsigned long long incl = warp_incl(mine[q], lane);
-		if (lane == 31)
-			sm.warp_sum[warp] = incl;
-		__syncthreads();
-		if (warp == 0)
-			sm.warp_sum[lane] = warp_incl(sm.warp_sum[lane], lane);
-		__syncthreads();
-		const unsigned long long before = (warp ? sm.warp_sum[warp - 1] : 0ull) + incl - mine[q];
-		total[q] = sm.warp_sum[31];
-		unsigned long long run = before;
-#pragma unroll
-		for (int i = 0; i < kPerThread; ++i) {
-			const int s = tid * kPerThread + i;
-			if (s < S) {
-				const int v = (int)min(run, 0x7fffffffull);
-				if (q == 0)
-					sm.cu[s] = v;
-				else
-					sm.first[s] = v;
-			}
-			run += (unsigned long long)(q == 0 ? nw[i] : need[i]);
+	for (int i = 0; i < kPerThread; ++i) {
+		const int s = tid * kPerThread + i;
+		if (s < S) {
+			sm.cu[s] = (int)min(run_t, 0x7fffffffull);
+			sm.first[s] = (int)min(run_b, 0x7fffffffull);
 		}
-		__syncthreads();
+		run_t += (unsigned long long)nw[i];
+		run_b += (unsigned long long)need[i];
 	}
 	if (tid == 0)
 		sm.cu[S] = (int)min(total[0], 0x7fffffffull);
@@ -192,15 +205,53 @@ layout_kernel(const kllm_layout_args a)
 			    table + (size_t)parent * a.max_blocks);
 			unsigned long long *dst = reinterpret_cast<unsigned long long *>(
 			    table + (size_t)s * a.max_blocks);
-			for (int w = lane; w < 3 * n; w += 32)
-				dst[w] = src[w];
+			// a batch of loads before its stores: one at a time, a row of 1,000
+			// blocks was 96 round trips and most of the launch
+			constexpr int kFly = 12;
+			for (int w0 = lane; w0 < 3 * n; w0 += 32 * kFly) {
+				unsigned long long v[kFly];
+#pragma unroll
+				for (int q = 0; q < kFly; ++q)
+					if (w0 + 32 * q < 3 * n)
+						v[q] = src[w0 + 32 * q];
+#pragma unroll
+				for (int q = 0; q < kFly; ++q)
+					if (w0 + 32 * q < 3 * n)
+						dst[w0 + 32 * q] = v[q];
+			}
 		}
 	}
 
 	// ---- tokens ------------------------------------------------------------------
+	// Each warp takes a contiguous run of them. It finds the row of its first
+	// token by 32 probes a round, and from there on a lane looks only between the
+	// rows of the warp's first and last token.
 	const long long span = max((long long)n_tok, (long long)a.token_capacity);
-	for (long long t0 = (long long)gw * 32; t0 < span; t0 += (long long)n_warps * 32) {
+	const long long per = ((span + n_warps - 1) / n_warps + 31) / 32 * 32;
+	const long long end = min(span, (gw + 1) * per);
+	const double inv_slot = 1.0 / (double)a.slot_bytes;
+	// the last row whose tokens start at or before t < n_tok
+	auto row_of = [&](int t) {
+		int lo = 0, hi = S - 1;
+		while (lo < hi) {
+			const int step = (hi - lo + 31) / 32;              // rows lo + 1 .. hi
+			const int at = lo + 1 + lane * step;
+			const unsigned b = __ballot_sync(0xffffffffu, at <= hi && sm.cu[min(at, hi)] <= t);
+			const int n = __popc(b);                           // the first n probes hold
+			hi = n ? min(hi, lo + n * step) : lo;
+			lo = n ? lo + 1 + (n - 1) * step : lo;
+		}
+		return lo;
+	};
+	int s0 = -1;
+	for (long long t0 = (long long)gw * per; t0 < end; t0 += 32) {
 		const long long t = t0 + lane;
+		int s1 = s0;
+		if (t0 < n_tok) {
+			if (s0 < 0)
+				s0 = row_of((int)t0);
+			s1 = row_of((int)min(t0 + 31, (long long)n_tok - 1));
+		}
 		if (t >= n_tok) {
 			if (t < a.token_capacity) {
 				a.token_seq[t] = -1;
@@ -210,17 +261,17 @@ layout_kernel(const kllm_layout_args a)
 			}
 			continue;
 		}
-		// the last row whose tokens start at or before t
-		int lo = 0, hi = S - 1;
+		int lo = s0, hi = s1;
 		while (lo < hi) {
 			const int mid = (lo + hi + 1) >> 1;
-			if ((long long)sm.cu[mid] <= t)
+			if (sm.cu[mid] <= (int)t)
 				lo = mid;
 			else
 				hi = mid - 1;
 		}
+		s0 = s1;
 		const int s = lo, c = sm.ctx[s], pos = c + (int)(t - sm.cu[s]);
-		const int j = pos / bs, off = pos - j * bs, old = (int)(((long long)c + bs - 1) / bs);
+		const int j = pos / bs, off = pos - j * bs, old = blocks_of(c, bs);
 		long long slot;
 		if (j >= old) {
 			LayEntry e;
@@ -231,7 +282,7 @@ layout_kernel(const kllm_layout_args a)
 		} else {
 			const LayEntry *e = table + (size_t)s * a.max_blocks + j;
 			const bool ok = (int)(e->valid & 0xffffffffll) != 0;
-			const unsigned long long at = (e->k - a.arena_base - a.k_offset) / a.slot_bytes;
+			const unsigned long long at = div_small(e->k - a.arena_base - a.k_offset, a.slot_bytes, inv_slot);
 			slot = ok && at < a.total_slots ? (long long)at : -1;
 		}
 		if (t < a.token_capacity) {
