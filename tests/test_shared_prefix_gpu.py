@@ -207,6 +207,15 @@ def test_error_bits(be):
     assert int(dev.err.item()) == kb.ERR_PAGE_RANGE and (got == 0).all()
 
 
+@pytest.mark.parametrize("kv", [MX, BF16])
+def test_more_rows_than_a_plan_keeps_at_hand(be, kv):
+    """5,200 rows in 1,500 groups: the plan takes several rounds, and the tile
+    sums do not fit the suffix CTAs' shared memory."""
+    rng = np.random.default_rng(8)
+    groups = [(16 * int(rng.integers(0, 3)) + 3, rng.integers(0, 70, 3).tolist()) for _ in range(1500)]
+    check(be, cfg(kv, 2, 1, d=64), groups, loose=rng.integers(0, 40, 700).tolist())
+
+
 def test_same_bits_every_time_and_on_another_stream(be):
     import torch
     case = pc.PrefixCase(cfg(MX, 32, 8), [(1111, suffixes(30, 1111, 60, 3))])
