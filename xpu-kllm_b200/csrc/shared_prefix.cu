@@ -1072,8 +1072,7 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 				}
 				return e;
 			};
-			// this lane's page of a block as section addresses (0: absent), which
-			// start on their way to L2
+			// this lane's page of a block as section addresses (valid 0: absent)
 			auto check = [&](DevEntry &e) {
 				const bool present = e.valid && e.k != 0ull;
 				const bool aligned = ((e.k | e.v) & 15ull) == 0ull;
@@ -1088,18 +1087,11 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 						atomicOr(a.err, KLLM_ERR_PAGE_RANGE_BIT);
 				}
 				e.valid = here ? 1 : 0;
-				if (here) {
-					bulk_prefetch_l2(reinterpret_cast<const void *>(e.k), (uint32_t)sec);
-					bulk_prefetch_l2(reinterpret_cast<const void *>(e.v), (uint32_t)sec);
-				}
 			};
 			DevEntry cur = load(p.b0), nxt = load(p.b0 + 1);
 			check(cur);
 			for (int j = 0; j < p.nb && ok; ++j) {
 				const DevEntry e = cur;
-				cur = nxt;
-				check(cur);
-				nxt = load(p.b0 + j + 2);
 				const uint32_t mask = __ballot_sync(0xffffffffu, e.valid);
 				const int slot = gb % kPg;
 				if (gb >= kPg)
@@ -1124,6 +1116,16 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 				if (lane == 0)
 					mbar_arrive(&sm.pg_full[slot]);
 				++gb;
+				cur = nxt;
+				nxt = load(p.b0 + j + 2);
+				check(cur);
+				// On its way to L2 up to five blocks ahead of the producers; not the
+				// second block, whose address they already wait for (the two requests
+				// of 16 pages take the warp 1.2k cycles).
+				if (j > 0 && cur.valid) {
+					bulk_prefetch_l2(reinterpret_cast<const void *>(cur.k), (uint32_t)sec);
+					bulk_prefetch_l2(reinterpret_cast<const void *>(cur.v), (uint32_t)sec);
+				}
 			}
 		}
 	}
