@@ -22,7 +22,8 @@
 // raises the thresholds. A row appends about top_n (1 + ln(columns / top_n))
 // logits in all. Ranges of up to 16 row blocks run side by side, so that a
 // vocabulary tile is read from HBM once and by its other row blocks from L2.
-// Warps: 0 TMA producer, 1 TMEM allocation and MMA issue, 2-5 epilogue. Two
+// Warps: 0 TMA producer, 1 TMEM allocation and MMA issue, 2-5 the rows' sums,
+// 6-9 their lists (in one warp the two took 1.5k cycles for 32 columns). Two
 // accumulators of 256 TMEM columns let the epilogue of a tile run under the
 // next one's products. Waits are bounded in wall time (KLLM_ERR_TIMEOUT).
 //
@@ -45,7 +46,7 @@ constexpr int kSU = 64;                    // vocabulary columns per unit
 constexpr int kSN = 256;                   // columns per tile (MMA N), 4 units
 constexpr int kSK = 64;                    // hidden elements per stage
 constexpr int kSStages = 3;
-constexpr int kScThreads = 192;
+constexpr int kScThreads = 320;
 constexpr int kListCap = 64;
 constexpr int kListTrig = 48;              // a list above this is cut (16 more may come)
 constexpr int kSlack = 4;                  // a cut keeps top_n .. top_n + kSlack entries
@@ -112,6 +113,15 @@ __device__ __forceinline__ void list_put(uint32_t at, float v, uint32_t id)
 {
 	asm volatile("st.shared.v2.u32 [%0], {%1, %2};" :: "r"(at), "r"(__float_as_uint(v)), "r"(id) : "memory");
 }
+// Puts x at `at` and advances it when key >= least.
+__device__ __forceinline__ void list_keep(uint32_t &at, uint2 x, uint32_t key, uint32_t least)
+{
+	asm volatile("{\n\t.reg .pred p;\n\t"
+		     "setp.ge.u32 p, %1, %2;\n\t"
+		     "@p st.shared.v2.u32 [%0], {%3, %4};\n\t"
+		     "@p add.u32 %0, %0, %5;\n\t}"
+		     : "+r"(at) : "r"(key), "r"(least), "r"(x.x), "r"(x.y), "n"(kListStep) : "memory");
+}
 // Appends (v, base + i) at `at` and advances it when v > tau.
 __device__ __forceinline__ void list_offer(uint32_t &at, float v, float tau, int base, int i)
 {
@@ -125,12 +135,14 @@ __device__ __forceinline__ void list_offer(uint32_t &at, float v, float tau, int
 		     : "memory");
 }
 
+// CAP: entries looked at (n <= CAP). KEEP false: only the threshold.
+template <int CAP, bool KEEP>
 __device__ __noinline__ Cut cut_list(uint32_t list, int k, int n, float tau)
 {
-	uint32_t key[kListCap];
+	uint32_t key[CAP];
 	uint32_t lo = 0xffffffffu, hi = 0u;
 #pragma unroll
-	for (int e = 0; e < kListCap; ++e) {
+	for (int e = 0; e < CAP; ++e) {
 		key[e] = key_of(__uint_as_float(list_get(list + e * kListStep).x));
 		if (e >= n)
 			key[e] = 0u;                       // below every number's key
@@ -142,49 +154,58 @@ __device__ __noinline__ Cut cut_list(uint32_t list, int k, int n, float tau)
 	// of at most k + kSlack, else with hi = lo + 1, lo the k-th largest key
 	const bool work = n >= k;
 	hi = hi + 1u;                              // keys of numbers stay below 2^32 - 1
-	bool done = !work || n <= k + kSlack;
+	bool done = !work || (KEEP && n <= k + kSlack);
 	bool equals = false;
 	while (!__all_sync(0xffffffffu, done)) {
 		const uint32_t mid = lo + ((hi - lo) >> 1);
-		int c[2] = {0, 0};
+		int c[4] = {0, 0, 0, 0};
 #pragma unroll
-		for (int e = 0; e < kListCap; ++e)
-			c[e & 1] += key[e] >= mid ? 1 : 0;
+		for (int e = 0; e < CAP; ++e)
+			c[e & 3] += key[e] >= mid ? 1 : 0;
+		const int above = (c[0] + c[1]) + (c[2] + c[3]);
 		if (!done) {
 			if (mid == lo) {
 				equals = done = true;
-			} else if (c[0] + c[1] >= k) {
+			} else if (above >= k) {
 				lo = mid;
-				done = c[0] + c[1] <= k + kSlack;
+				done = above <= k + kSlack;
 			} else {
 				hi = mid;
 			}
 		}
 	}
-	if (!work)
+	if (work)
+		tau = value_of(lo);
+	if constexpr (!KEEP)
 		return {n, tau};
-	int budget = kListCap;                     // of entries equal to lo
-	if (equals) {
-		budget = k;
+	// the entries that stay move down; none does before it has been read
+	const uint32_t least = work ? lo : 1u;     // a list with n < k stays as it is
+	uint32_t at = list;
+	int budget = 0;                            // of entries equal to lo
+	const bool ties = __any_sync(0xffffffffu, equals);
+	if (ties) {
+		budget = equals ? k : CAP;
+		if (equals)
 #pragma unroll
-		for (int e = 0; e < kListCap; ++e)
-			budget -= key[e] > lo ? 1 : 0;
+			for (int e = 0; e < CAP; ++e)
+				budget -= key[e] > lo ? 1 : 0;
 	}
-	uint32_t id[kListCap];
 #pragma unroll
-	for (int e = 0; e < kListCap; ++e)
-		id[e] = list_get(list + e * kListStep).y;
-	int w = 0;
+	for (int e0 = 0; e0 < CAP; e0 += 16) {
+		uint2 x[16];
 #pragma unroll
-	for (int e = 0; e < kListCap; ++e) {
-		const bool eq = key[e] == lo;
-		if (key[e] > lo || (eq && budget > 0)) {
-			budget -= eq ? 1 : 0;
-			list_put(list + w * kListStep, value_of(key[e]), id[e]);
-			++w;
-		}
+		for (int e = 0; e < 16; ++e)
+			x[e] = list_get(list + (e0 + e) * kListStep);
+		if (ties)
+#pragma unroll
+			for (int e = 0; e < 16; ++e)
+				if (key[e0 + e] == least && work && --budget < 0)
+					key[e0 + e] = 0u;
+#pragma unroll
+		for (int e = 0; e < 16; ++e)
+			list_keep(at, x[e], key[e0 + e], least);
 	}
-	return {w, value_of(lo)};
+	return {(int)((at - list) / kListStep), tau};
 }
 
 __global__ void __launch_bounds__(kScThreads, 1)
@@ -207,7 +228,7 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 		}
 		for (int b = 0; b < 2; ++b) {
 			mbar_init(&sm.acc_full[b], 1);
-			mbar_init(&sm.acc_empty[b], 128);
+			mbar_init(&sm.acc_empty[b], a.top_n > 0 ? 256 : 128);
 		}
 		mbar_init(&sm.drain, 1);
 		sm.abort = 0;
@@ -335,20 +356,21 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 		mbar_wait_ns(&sm.drain, 0u, kScWaitNs);
 	} else {
 		// ================= epilogue: one row a thread ==================================
+		// Warps 2-5 keep the row's sums, warps 6-9 its list.
 		const int q = warp & 3, t = q * 32 + lane;
 		const int k = a.top_n, V = a.vocab;
+		const bool lists = warp >= 6;
+		const uint32_t list = smem_u32(&sm.list[0][t]);
 		int it = 0;
-		bool ok = true;
+		bool ok = !lists || k > 0;
 		for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
 			int rb, split, u0, u1;
 			if (!item_range(item, rb, split, u0, u1))
 				continue;
-			const int row = rb * kSR + t;
-			const bool live = row < a.num_rows;      // the rest are rows of zeros
-			const float T = (live && a.temperature) ? a.temperature[row] : 1.f;
+			const int row = rb * kSR + t;            // past the last: a row of zeros
+			const float T = (row < a.num_rows && a.temperature) ? a.temperature[row] : 1.f;
 			const float c = kLog2e * (T > 0.f ? 1.f / T : 1.f);
 			float m = -CUDART_INF_F, S = 0.f, W = 0.f, tau = -CUDART_INF_F;
-			const uint32_t list = smem_u32(&sm.list[0][t]);
 			uint32_t at = list;                // where the next entry goes
 			for (int u = u0; u < u1; u += 4, ++it) {
 				const int buf = it & 1, nc = min(4, u1 - u) * (kSU / 32);
@@ -370,7 +392,7 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 								v[i] = -CUDART_INF_F;
 					}
 				};
-				if (u == u0 && k > 0 && 4 * nc >= k) {
+				if (lists && u == u0 && 4 * nc >= k) {
 					// A range's first threshold: the k-th largest of its first tile's
 					// maxima over 8 columns (the list holds them meanwhile). From -inf
 					// the first tile alone would need several cuts.
@@ -388,7 +410,7 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 								 gm == gm ? gm : -CUDART_INF_F, 0u);
 						}
 					}
-					tau = cut_list(list, k, 4 * nc, tau).tau;
+					tau = cut_list<kSN / 8, false>(list, k, 4 * nc, tau).tau;
 					if (tau > -CUDART_INF_F)                 // its equals are wanted
 						tau = value_of(key_of(tau) - 1u);
 				}
@@ -399,6 +421,21 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 					if (nb >= V)
 						break;                 // nothing but padding
 					columns(ch, v);
+					if (lists) {
+#pragma unroll
+						for (int half = 0; half < 2; ++half) {
+#pragma unroll
+							for (int i = 16 * half; i < 16 * half + 16; ++i)
+								list_offer(at, v[i], tau, nb, i);
+							const int n = (int)((at - list) / kListStep);
+							if (__any_sync(0xffffffffu, n > kListTrig)) {
+								const Cut cut = cut_list<kListCap, true>(list, k, n, tau);
+								at = list + cut.n * kListStep;
+								tau = cut.tau;
+							}
+						}
+						continue;
+					}
 					float c4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
 					for (int i = 4; i < 32; ++i)
@@ -425,40 +462,25 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 					}
 					S += (s4[0] + s4[1]) + (s4[2] + s4[3]);
 					W += (w4[0] + w4[1]) + (w4[2] + w4[3]);
-					if (k > 0) {
-#pragma unroll
-						for (int half = 0; half < 2; ++half) {
-#pragma unroll
-							for (int i = 16 * half; i < 16 * half + 16; ++i)
-								list_offer(at, v[i], tau, nb, i);
-							const int n = (int)((at - list) / kListStep);
-							if (__any_sync(0xffffffffu, n > kListTrig)) {
-								const Cut cut = cut_list(list, k, n, tau);
-								at = list + cut.n * kListStep;
-								tau = cut.tau;
-							}
-						}
-					}
 				}
 				tc_fence_before();
 				mbar_arrive(&sm.acc_empty[buf]);
 			}
 			if (!ok)
 				break;
-			int n = (int)((at - list) / kListStep);
-			if (k > 0) {
-				const Cut cut = cut_list(list, k, n, tau);
-				n = cut.n;
-				tau = cut.tau;
-			}
 			const size_t to = (size_t)split * a.row_blocks * kSR + (size_t)rb * kSR + t;
-			static_cast<float4 *>(a.part)[to] = make_float4(m, S, W, tau);
-			if (k > 0) {
+			float *part = static_cast<float *>(a.part) + 4 * to;
+			if (lists) {
+				const Cut cut = cut_list<kListCap, true>(list, k, (int)((at - list) / kListStep), tau);
 				const size_t stride = (size_t)a.splits * a.row_blocks * kSR;
-				a.part_n[to] = n;
-				for (int e = 0; e < n; ++e)
+				part[3] = cut.tau;
+				a.part_n[to] = cut.n;
+				for (int e = 0; e < cut.n; ++e)
 					static_cast<uint2 *>(a.part_list)[(size_t)e * stride + to] =
 					    list_get(list + e * kListStep);
+			} else {
+				*reinterpret_cast<float2 *>(part) = make_float2(m, S);
+				part[2] = W;
 			}
 		}
 	}
