@@ -55,7 +55,8 @@ constexpr uint64_t kScWaitNs = 200000000ull;
 struct ScoreSmem {
 	uint8_t a[kSStages][kSR * kSK * 2];
 	uint8_t b[kSStages][kSN * kSK * 2];
-	uint2 list[kListCap][kSR];           // (value, index) of a row's largest logits so far
+	// (value, index) of a row's largest logits so far; one more for list_offer
+	uint2 list[kListCap + 1][kSR];
 	uint64_t full[kSStages], empty[kSStages];
 	uint64_t acc_full[2], acc_empty[2], drain;
 	uint32_t tmem_base;
@@ -100,9 +101,9 @@ struct Cut {
 
 constexpr uint32_t kListStep = kSR * sizeof(uint2);    // from one entry of a row to its next
 
-// Entries by their address in shared memory, appended under a predicate: the
-// compiler takes the list for generic memory and an append for a branch, which
-// was most of the epilogue (333 rows of 32,003: 70 us, 53 so).
+// Entries by their address in shared memory: the compiler takes the list for
+// generic memory and an append for a branch, which was most of the epilogue
+// (333 rows of 32,003: 70 us, 53 so).
 __device__ __forceinline__ uint2 list_get(uint32_t at)
 {
 	uint2 x;
@@ -113,26 +114,12 @@ __device__ __forceinline__ void list_put(uint32_t at, float v, uint32_t id)
 {
 	asm volatile("st.shared.v2.u32 [%0], {%1, %2};" :: "r"(at), "r"(__float_as_uint(v)), "r"(id) : "memory");
 }
-// Puts x at `at` and advances it when key >= least.
-__device__ __forceinline__ void list_keep(uint32_t &at, uint2 x, uint32_t key, uint32_t least)
+// Puts (v, id) at `at` and advances it when `stays`. The store is
+// unconditional: under a predicate the 32 of a chunk took 300 cycles more.
+__device__ __forceinline__ void list_offer(uint32_t &at, float v, uint32_t id, bool stays)
 {
-	asm volatile("{\n\t.reg .pred p;\n\t"
-		     "setp.ge.u32 p, %1, %2;\n\t"
-		     "@p st.shared.v2.u32 [%0], {%3, %4};\n\t"
-		     "@p add.u32 %0, %0, %5;\n\t}"
-		     : "+r"(at) : "r"(key), "r"(least), "r"(x.x), "r"(x.y), "n"(kListStep) : "memory");
-}
-// Appends (v, base + i) at `at` and advances it when v > tau.
-__device__ __forceinline__ void list_offer(uint32_t &at, float v, float tau, int base, int i)
-{
-	asm volatile("{\n\t.reg .pred p;\n\t.reg .u32 id;\n\t"
-		     "setp.gt.f32 p, %1, %2;\n\t"
-		     "@p add.u32 id, %3, %4;\n\t"
-		     "@p st.shared.v2.u32 [%0], {%5, id};\n\t"
-		     "@p add.u32 %0, %0, %6;\n\t}"
-		     : "+r"(at)
-		     : "f"(v), "f"(tau), "r"(base), "r"(i), "r"(__float_as_uint(v)), "n"(kListStep)
-		     : "memory");
+	list_put(at, v, id);
+	at += stays ? kListStep : 0u;
 }
 
 // CAP: entries looked at (n <= CAP). KEEP false: only the threshold.
@@ -203,7 +190,7 @@ __device__ __noinline__ Cut cut_list(uint32_t list, int k, int n, float tau)
 					key[e0 + e] = 0u;
 #pragma unroll
 		for (int e = 0; e < 16; ++e)
-			list_keep(at, x[e], key[e0 + e], least);
+			list_offer(at, __uint_as_float(x[e].x), x[e].y, key[e0 + e] >= least);
 	}
 	return {(int)((at - list) / kListStep), tau};
 }
@@ -426,7 +413,7 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 						for (int half = 0; half < 2; ++half) {
 #pragma unroll
 							for (int i = 16 * half; i < 16 * half + 16; ++i)
-								list_offer(at, v[i], tau, nb, i);
+								list_offer(at, v[i], (uint32_t)(nb + i), v[i] > tau);
 							const int n = (int)((at - list) / kListStep);
 							if (__any_sync(0xffffffffu, n > kListTrig)) {
 								const Cut cut = cut_list<kListCap, true>(list, k, n, tau);
