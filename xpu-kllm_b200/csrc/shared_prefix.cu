@@ -1528,38 +1528,72 @@ attend_kernel(const kllm_prefix_args a)
 
 // ---- join -----------------------------------------------------------------------------
 
-constexpr int kJRows = 32;
+constexpr int kJRows = 16;
 
-// One CTA: 32 consecutive rows (sequence-major) of one kv head. Phase 1: a lane
-// per row, a warp per two chunks of 4 dims: the prefix pieces folded into a
-// running (max, sum, o), six pieces' loads in flight (the partials hold [D /
-// 4][rows][4], so a warp reads 512 contiguous bytes). Phase 2: D / 8 threads
-// per row fold the suffix pieces (rows of D) and store.
-template <int D>
-__global__ void __launch_bounds__(4 * D)
+// A running (max, sum, 4 dims of o) and the fold of pieces into it; a piece
+// with l = 0 counts nothing (its o is not written).
+struct JoinAcc {
+	float M, L, o[4];
+};
+template <int N>
+__device__ __forceinline__ void fold(JoinAcc &A, const float (&l)[N], const float (&m)[N], const float4 (&o)[N])
+{
+	float mb = A.M;
+#pragma unroll
+	for (int u = 0; u < N; ++u)
+		if (l[u] != 0.f)
+			mb = fmaxf(mb, m[u]);
+	if (mb > A.M) {
+		const float f = exp2f(A.M - mb);               // 0 while M is -inf
+		A.L *= f;
+#pragma unroll
+		for (int q = 0; q < 4; ++q)
+			A.o[q] *= f;
+		A.M = mb;
+	}
+#pragma unroll
+	for (int u = 0; u < N; ++u)
+		if (l[u] != 0.f) {
+			const float e = exp2f(m[u] - A.M);
+			A.L = fmaf(l[u], e, A.L);
+			A.o[0] = fmaf(o[u].x, e, A.o[0]);
+			A.o[1] = fmaf(o[u].y, e, A.o[1]);
+			A.o[2] = fmaf(o[u].z, e, A.o[2]);
+			A.o[3] = fmaf(o[u].w, e, A.o[3]);
+		}
+}
+
+// One CTA: 16 consecutive rows (sequence-major) of one kv head, a thread 4 dims
+// of a row. Phase 1, rows fastest: the prefix pieces, kFly pieces' loads in
+// flight (the partials hold [D / 4][rows][4], so 16 lanes read 256 contiguous
+// bytes). Phase 2, dims fastest: the suffix pieces (rows of D), and the store.
+// kFly 8 takes 86 registers, one CTA an SM, and is the faster one when no SM
+// gets a second CTA (64 rows of 8,192 shared tokens 47.4 us against 49.3); kFly
+// 6 takes 64, two CTAs (256 rows: 93 us against 99).
+template <int D, int kFly>
+__global__ void __launch_bounds__(kJRows * D / 4, kFly == 8 ? 1 : 256 / D)
 join_kernel(const kllm_prefix_args a, float unbias)
 {
-	constexpr int kFly = 6, kFlyS = 4;
+	constexpr int kFlyS = kFly / 2;
 	__shared__ float acc_s[kJRows][D + 4];
 	__shared__ float m_s[kJRows], l_s[kJRows];
-	const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+	const int tid = threadIdx.x;
 	const int h = blockIdx.y, H = a.num_kv_heads, rows = a.num_seqs * a.group;
 	// The plan is complete here: the attention's CTAs let this kernel start only
 	// after they have waited for it. Its partials need the wait below.
 	const PHeader *hd = static_cast<const PHeader *>(a.header);
-	const int i = blockIdx.x * kJRows + lane;
-	const int r = tid / (D / 8), part = tid % (D / 8), ii = blockIdx.x * kJRows + r;
+	const int lr1 = tid % kJRows, ch1 = tid / kJRows, i = blockIdx.x * kJRows + lr1;
+	const int lr2 = tid / (D / 4), ch2 = tid % (D / 4), ii = blockIdx.x * kJRows + lr2;
 	const int seq2 = min(ii, rows - 1) / a.group;
 	const int t0 = a.tile_pre[seq2], ts = a.tile_pre[seq2 + 1] - t0;
 	const long long N = hd->N, WS = hd->WS;
 	{
 		const int seq = i / a.group;
 		const int g = i < rows ? a.row_group[seq] : -1;
-		float M = -CUDART_INF_F, L = 0.f;
-		float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-		if (g < 0)
+		JoinAcc A = {-CUDART_INF_F, 0.f, {0.f, 0.f, 0.f, 0.f}};
+		if (g < 0) {
 			grid_dependency_wait();
-		else {
+		} else {
 			const long long T = hd->T, W = hd->W;
 			const PGroup G = static_cast<const PGroup *>(a.groups)[g];
 			const int lr = (seq - G.row0) * a.group + i % a.group;
@@ -1575,7 +1609,7 @@ join_kernel(const kllm_prefix_args a, float unbias)
 			grid_dependency_wait();
 			for (int p0 = 0; p0 < np; p0 += kFly) {
 				float l[kFly], m[kFly];
-				float4 o[kFly][2];
+				float4 o[kFly];
 #pragma unroll
 				for (int u = 0; u < kFly; ++u) {
 					const int p = p0 + u;
@@ -1586,56 +1620,27 @@ join_kernel(const kllm_prefix_args a, float unbias)
 								     (solo && (p & 1) ? urows : 0);
 						l[u] = __ldcg(a.pl + at + r);
 						m[u] = __ldcg(a.pm + at + r);
-						const float *po = a.po + at * D + ((size_t)2 * warp * urows + r) * 4;
-						o[u][0] = __ldcg(reinterpret_cast<const float4 *>(po));
-						o[u][1] = __ldcg(reinterpret_cast<const float4 *>(po + 4 * urows));
+						o[u] = __ldcg(reinterpret_cast<const float4 *>(
+						    a.po + at * D + ((size_t)ch1 * urows + r) * 4));
 					}
 				}
-				float mb = M;
-#pragma unroll
-				for (int u = 0; u < kFly; ++u)
-					if (l[u] != 0.f)
-						mb = fmaxf(mb, m[u]);
-				if (mb > M) {
-					const float f = exp2f(M - mb);       // 0 while M is -inf
-					L *= f;
-#pragma unroll
-					for (int q = 0; q < 8; ++q)
-						acc[q] *= f;
-					M = mb;
-				}
-#pragma unroll
-				for (int u = 0; u < kFly; ++u)
-					if (l[u] != 0.f) {                   // o of an empty piece is not written
-						const float e = exp2f(m[u] - M);
-						L = fmaf(l[u], e, L);
-#pragma unroll
-						for (int q = 0; q < 2; ++q) {
-							acc[4 * q] = fmaf(o[u][q].x, e, acc[4 * q]);
-							acc[4 * q + 1] = fmaf(o[u][q].y, e, acc[4 * q + 1]);
-							acc[4 * q + 2] = fmaf(o[u][q].z, e, acc[4 * q + 2]);
-							acc[4 * q + 3] = fmaf(o[u][q].w, e, acc[4 * q + 3]);
-						}
-					}
+				fold(A, l, m, o);
 			}
 		}
-#pragma unroll
-		for (int q = 0; q < 2; ++q)
-			*reinterpret_cast<float4 *>(&acc_s[lane][8 * warp + 4 * q]) =
-			    make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
-		if (warp == 0) {
-			m_s[lane] = M;
-			l_s[lane] = L;
+		*reinterpret_cast<float4 *>(&acc_s[lr1][4 * ch1]) = make_float4(A.o[0], A.o[1], A.o[2], A.o[3]);
+		if (ch1 == 0) {
+			m_s[lr1] = A.M;
+			l_s[lr1] = A.L;
 		}
 	}
 	__syncthreads();
 	if (ii >= rows)
 		return;
 	const int seq = seq2, hh = ii - seq * a.group;
-	float M = m_s[r], L = l_s[r], acc[8];
-#pragma unroll
-	for (int q = 0; q < 8; ++q)
-		acc[q] = acc_s[r][part * 8 + q];
+	JoinAcc A;
+	A.M = m_s[lr2];
+	A.L = l_s[lr2];
+	*reinterpret_cast<float4 *>(A.o) = *reinterpret_cast<const float4 *>(&acc_s[lr2][4 * ch2]);
 	if (ts > 0) {
 		const long long x0 = (long long)t0 * H + (long long)h * ts;
 		const long long w0 = div_steps((x0 + 1) * WS - 1, N), w1 = div_steps((x0 + ts) * WS - 1, N);
@@ -1643,7 +1648,7 @@ join_kernel(const kllm_prefix_args a, float unbias)
 		const int np = (int)(w1 - w0 + 1);
 		for (int p0 = 0; p0 < np; p0 += kFlyS) {
 			float l[kFlyS], m[kFlyS];
-			float4 o[kFlyS][2];
+			float4 o[kFlyS];
 #pragma unroll
 			for (int u = 0; u < kFlyS; ++u) {
 				l[u] = 0.f;
@@ -1652,44 +1657,16 @@ join_kernel(const kllm_prefix_args a, float unbias)
 					const size_t at = (slot + p0 + u) * a.group + hh;
 					l[u] = __ldcg(a.xl + at);
 					m[u] = __ldcg(a.xm + at);
-					const float4 *xo = reinterpret_cast<const float4 *>(a.xo + at * D + part * 8);
-					o[u][0] = __ldcg(xo);
-					o[u][1] = __ldcg(xo + 1);
+					o[u] = __ldcg(reinterpret_cast<const float4 *>(a.xo + at * D + 4 * ch2));
 				}
 			}
-			float mb = M;
-#pragma unroll
-			for (int u = 0; u < kFlyS; ++u)
-				if (l[u] != 0.f)
-					mb = fmaxf(mb, m[u]);
-			if (mb > M) {
-				const float f = exp2f(M - mb);
-				L *= f;
-#pragma unroll
-				for (int q = 0; q < 8; ++q)
-					acc[q] *= f;
-				M = mb;
-			}
-#pragma unroll
-			for (int u = 0; u < kFlyS; ++u)
-				if (l[u] != 0.f) {               // o of a piece without tokens counts nothing
-					const float e = exp2f(m[u] - M);
-					L = fmaf(l[u], e, L);
-#pragma unroll
-					for (int q = 0; q < 2; ++q) {
-						acc[4 * q] = fmaf(o[u][q].x, e, acc[4 * q]);
-						acc[4 * q + 1] = fmaf(o[u][q].y, e, acc[4 * q + 1]);
-						acc[4 * q + 2] = fmaf(o[u][q].z, e, acc[4 * q + 2]);
-						acc[4 * q + 3] = fmaf(o[u][q].w, e, acc[4 * q + 3]);
-					}
-				}
+			fold(A, l, m, o);
 		}
 	}
-	const float inv = L != 0.f ? unbias / L : 0.f;    // an empty row gives zeros
+	const float inv = A.L != 0.f ? unbias / A.L : 0.f;    // an empty row gives zeros
 	const size_t row = (size_t)seq * a.num_heads + (size_t)h * a.group + hh;
-	*reinterpret_cast<uint4 *>(static_cast<uint8_t *>(a.out) + (row * D + part * 8) * 2) =
-	    make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
-		       pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
+	*reinterpret_cast<uint2 *>(static_cast<uint8_t *>(a.out) + (row * D + 4 * ch2) * 2) =
+	    make_uint2(pack_bf16x2(A.o[0] * inv, A.o[1] * inv), pack_bf16x2(A.o[2] * inv, A.o[3] * inv));
 }
 
 template <typename... KArgs, typename... Args>
@@ -1786,7 +1763,10 @@ extern "C" int kllm_prefix_launch(struct kllm_prefix_args *a, void *stream)
 	const dim3 grid((unsigned)(((long long)a->num_seqs * a->group + kJRows - 1) / kJRows),
 			(unsigned)a->num_kv_heads);
 	const float unbias = a->kv_dtype ? KLLM_MX_DEC_UNBIAS : 1.f;
+	const bool one = (long long)grid.x * grid.y <= a->ctas;
 	if (a->head_dim == 128)
-		return (int)launch_dependent(join_kernel<128>, grid, 4 * 128, 0, st, 1, *a, unbias);
-	return (int)launch_dependent(join_kernel<64>, grid, 4 * 64, 0, st, 1, *a, unbias);
+		return (int)launch_dependent(one ? join_kernel<128, 8> : join_kernel<128, 6>, grid, kJRows * 32,
+					     0, st, 1, *a, unbias);
+	return (int)launch_dependent(one ? join_kernel<64, 8> : join_kernel<64, 6>, grid, kJRows * 16, 0, st,
+				     1, *a, unbias);
 }
