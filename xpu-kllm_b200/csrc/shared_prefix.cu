@@ -97,7 +97,7 @@ static_assert(sizeof(PHeader) == 64 && sizeof(PGroup) == 48, "workspace layout")
 
 // ---- plan ------------------------------------------------------------------------
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 256;
 // A CTA's time for n steps or for n tiles a warp, in ns, as measured on the
 // whole chip: set-up, then the rate. They only balance the two parts; for 256
 // rows of 8,192 shared tokens any split from 96 to 108 CTAs of 148 is within 4%.
