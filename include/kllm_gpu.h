@@ -16,7 +16,8 @@
  * Part 2 adds versioned entry points the reference lacks: 16-token pages,
  * the MX-FP8 KV format, split-KV partial outputs, KV append with
  * quantize-on-write, the partial merge, chunked prefill, a bit-exact gather
- * for tests and the NCCL split-KV exchange.
+ * for tests, the NCCL split-KV exchange, and parallel sampling with scored
+ * answers (batch layout, shared-prefix decode, log-probabilities).
  *
  * Conventions (all calls):
  *   - every pointer inside a params struct is a DEVICE pointer unless the
