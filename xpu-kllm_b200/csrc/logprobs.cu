@@ -118,6 +118,11 @@ struct Elem<0> {
 		}
 		return n;
 	}
+	static __device__ __forceinline__ float vmax(uint4 v)
+	{
+		return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+			     fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+	}
 	static __device__ __forceinline__ void unpack(uint4 v, float (&x)[4])
 	{
 		x[0] = __uint_as_float(v.x);
@@ -135,7 +140,7 @@ struct Elem<1> {
 		return __uint_as_float((uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(p)) << 16);
 	}
 	// The comparisons of two elements give two bf16 ones or zeros, whose sums
-	// (at most 16 each) are exact.
+	// (at most 32 each) are exact.
 	static __device__ __forceinline__ int count(const uint4 (&raw)[kFly], float t, bool equal)
 	{
 		const __nv_bfloat162 t2 = __float2bfloat162_rn(t);       // t is a bf16 value
@@ -150,6 +155,12 @@ struct Elem<1> {
 			}
 		}
 		return (int)(__low2float(n) + __high2float(n));
+	}
+	static __device__ __forceinline__ float vmax(uint4 v)
+	{
+		auto h = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162 *>(&w); };
+		const __nv_bfloat162 m = __hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w)));
+		return fmaxf(__low2float(m), __high2float(m));
 	}
 	static __device__ __forceinline__ void unpack(uint4 v, float (&x)[8])
 	{
@@ -375,7 +386,6 @@ logprobs_kernel(const kllm_logprobs_args a)
 	int rank_n = 0;                               // lane j: target j's rank so far
 #pragma unroll 1
 	for (int it = 0, here = b0; it == 0 || here < U; ++it, here += stride) {
-		float x[kFly][kVec];
 		uint4 raw[kFly];
 		if (here >= mis && here + kBatch <= U) {               // the same for the whole warp
 			const uint4 *p = reinterpret_cast<const uint4 *>(row + (here - mis)) + lane;
@@ -393,18 +403,10 @@ logprobs_kernel(const kllm_logprobs_args a)
 			sm.ti[tid] = in ? t : -1;
 			sm.tl[tid] = in ? Elem<BF16>::get(row + t) : CUDART_INF_F;
 		}
+		float bm = -CUDART_INF_F;
 #pragma unroll
 		for (int q = 0; q < kFly; ++q)
-			Elem<BF16>::unpack(raw[q], x[q]);
-		float vm[kFly], bm = -CUDART_INF_F;        // maxima of the vectors, of all
-#pragma unroll
-		for (int q = 0; q < kFly; ++q) {
-			vm[q] = x[q][0];
-#pragma unroll
-			for (int z = 1; z < kVec; ++z)
-				vm[q] = fmaxf(vm[q], x[q][z]);
-			bm = fmaxf(bm, vm[q]);
-		}
+			bm = fmaxf(bm, Elem<BF16>::vmax(raw[q]));
 		const float ym = bm * c;
 		if (ym > m) {
 			if (m > -CUDART_INF_F) {
@@ -419,15 +421,18 @@ logprobs_kernel(const kllm_logprobs_args a)
 		const uint64_t c2 = pack2(c, c), r2 = pack2(-ref, -ref);
 		uint64_t s2 = 0ull, w2 = 0ull;
 #pragma unroll
-		for (int q = 0; q < kFly; ++q)
+		for (int q = 0; q < kFly; ++q) {
+			float x[kVec];
+			Elem<BF16>::unpack(raw[q], x);
 #pragma unroll
 			for (int z = 0; z < kVec; z += 2) {
 				float d0, d1;
-				unpack2(fma2(pack2(x[q][z], x[q][z + 1]), c2, r2), d0, d1);
+				unpack2(fma2(pack2(x[z], x[z + 1]), c2, r2), d0, d1);
 				const uint64_t e2 = pack2(ex2_approx(d0), ex2_approx(d1));
 				s2 = add2(s2, e2);
 				w2 = fma2(e2, pack2(fmaxf(d0, -1000.f), fmaxf(d1, -1000.f)), w2);  // 0 x -inf counts 0
 			}
+		}
 		float sa, sb, wa, wb;
 		unpack2(s2, sa, sb);
 		unpack2(w2, wa, wb);
@@ -483,13 +488,8 @@ logprobs_kernel(const kllm_logprobs_args a)
 			if (__any_sync(0xffffffffu, bm >= reach)) {
 				uint32_t todo = 0;                             // vectors with a candidate
 #pragma unroll
-				for (int q = 0; q < kFly; ++q) {
-					// fp32's eight are found again: kept, they take registers the pass needs
-					float y = vm[q];
-					if constexpr (!BF16)
-						y = fmaxf(fmaxf(x[q][0], x[q][1]), fmaxf(x[q][2], x[q][3]));
-					todo |= y >= reach ? 1u << q : 0u;
-				}
+				for (int q = 0; q < kFly; ++q)
+					todo |= Elem<BF16>::vmax(raw[q]) >= reach ? 1u << q : 0u;
 				while (todo) {
 					const int u = here + (__ffs(todo) - 1) * kStep + lane * kVec;
 					todo &= todo - 1u;
