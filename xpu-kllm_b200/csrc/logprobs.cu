@@ -27,7 +27,10 @@
 // rows still cover the GPU; the CTAs share maxima, sums and candidates through
 // distributed shared memory, so no workspace and no atomic on global memory is
 // needed and the result does not depend on the order in which CTAs finish.
-// Bound: HBM, each logit read once.
+// Floor: HBM, each logit read once; bound: instruction issue (15 to 20 an element
+// with ranks and alternatives; without them the same pass runs at 5.2 TB/s).
+// Measured: 256 fp32 rows of 128,256 with a target and 20 alternatives 34 us,
+// 3.9 TB/s; 999 bf16 rows of 32,003 with three targets 35 us, 1.8 TB/s.
 
 #include "kllm_device.cuh"
 #include "kllm_internal.h"
@@ -381,7 +384,7 @@ logprobs_kernel(const kllm_logprobs_args a)
 	// flight together; the 32 warps of an SM hide each other's.
 	// What rarely happens is a rolled loop that reads its vector again: unrolled
 	// over the batch and the targets it was half of the instructions, and the
-	// fetches of its code stalled the rest (999 rows of 32,003 bf16: 41 us).
+	// fetches of its code stalled the rest (999 rows of 32,003 bf16: 41 us, 35 so).
 	float m = -CUDART_INF_F, S = 0.f, W = 0.f, tau = -CUDART_INF_F;
 	int rank_n = 0;                               // lane j: target j's rank so far
 #pragma unroll 1

@@ -32,6 +32,12 @@
 // alone holds top_n logits that reach it; and with top_n ranges or more the
 // top_n-th largest of their maxima), orders them, and takes each target's
 // logit as a dot product of its own.
+//
+// Bound: HBM for few rows (24 rows of 4,096 against 128,256: 200 us, 5.3 TB/s of
+// the matrix's 1.05 GB, of which 6 us are the last tile's lists and 7 the join),
+// shared-memory bandwidth for many (a stage's 48 KB and its reads; 2,048 rows:
+// 1.75 ms, 1,230 TFLOP/s, at the power cap). 333 rows of 1,024 against 32,003: 41
+// us, 530 TFLOP/s, 2.5 tiles a CTA, so first products and last lists are bare.
 
 #include "kllm_device.cuh"
 #include "kllm_internal.h"
@@ -103,7 +109,7 @@ constexpr uint32_t kListStep = kSR * sizeof(uint2);    // from one entry of a ro
 
 // Entries by their address in shared memory: the compiler takes the list for
 // generic memory and an append for a branch, which was most of the epilogue
-// (333 rows of 32,003: 70 us, 53 so).
+// (333 rows of 32,003 took 70 us with it and 53 without).
 __device__ __forceinline__ uint2 list_get(uint32_t at)
 {
 	uint2 x;
