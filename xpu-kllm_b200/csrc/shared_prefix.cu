@@ -111,11 +111,15 @@ constexpr int kPlanThreads = 256;
 // rows of 8,192 shared tokens any split from 96 to 108 CTAs of 148 is within 4%.
 constexpr float kStepSetNs = 10500.f, kStepNsMx = 1500.f, kStepNsBf16 = 2700.f;
 constexpr float kTileSetNs = 5000.f, kTileNs = 2500.f;
+// Each further unit that a CTA works on (64 rows with 16 or 128 shared tokens:
+// 54 us without this term, 36 with it).
+constexpr float kPieceNs = 4500.f;
 
 struct PlanSmem {
 	long long w0[32], w1[32];
 	int leader[KLLM_MAX_SEQS_LAUNCH];
 	unsigned long long best;
+	int units;
 };
 
 // Tokens of group g's prefix that are whole pages inside the table.
@@ -180,6 +184,8 @@ plan_kernel(const kllm_prefix_args a)
 		bad |= b < 0 || e < b || e > S;
 		sm.leader[g] = 0x7fffffff;
 	}
+	if (tid == 0)
+		sm.units = 0;
 	bad = __syncthreads_or(bad);
 
 	// ---- rows: group, suffix, exclusive sums of the suffixes' tiles --------------
@@ -245,6 +251,7 @@ plan_kernel(const kllm_prefix_args a)
 				p.nblk = (p.npages + ppb - 1) / ppb;
 				x = (long long)a.num_kv_heads * p.tiles * p.nblk * p.wgt;
 				r = (long long)a.num_kv_heads * p.alloc;
+				atomicAdd(&sm.units, a.num_kv_heads * p.tiles);
 			}
 		}
 		block_scan2(sm, x, r, p.x0, p.r0, run_x, run_r);
@@ -263,7 +270,8 @@ plan_kernel(const kllm_prefix_args a)
 		if (possible) {
 			float t = 0.f;
 			if (n > 0)
-				t = kStepSetNs + (a.kv_dtype ? kStepNsMx : kStepNsBf16) * ceilf((float)T / (float)n);
+				t = kStepSetNs + (a.kv_dtype ? kStepNsMx : kStepNsBf16) * ceilf((float)T / (float)n) +
+				    kPieceNs * (ceilf((float)sm.units / (float)n) - 1.f);
 			if (N > 0)
 				t = fmaxf(t, kTileSetNs + kTileNs * ceilf((float)N / (float)((a.ctas - n) * a.suf_warps)));
 			atomicMin(&sm.best, ((unsigned long long)__float_as_uint(t) << 32) | (unsigned)n);
