@@ -77,10 +77,30 @@ constexpr int kPW = 6;                        // producer warps
 // Registers: 512 threads launch with 128 each, all of an SM's. A softmax thread
 // holds 128 scores (256 x 160 + 256 x 96); a suffix warp's MX tile takes the 128,
 // its BF16 tile 184 (256 x 184 + 256 x 72).
+constexpr int kRegsLaunch = 128;
 constexpr int kPg = 4;                        // blocks whose page addresses are known
 constexpr float kRaise = 8.f;                 // slack of the lazy reference maximum, log2
 constexpr float kPShift = 7.f;                // f16 P is built 2^7 larger
 constexpr uint64_t kPWaitNs = 200000000ull;
+
+// Moves registers between warps 0 .. FIRST - 1 (HI a thread from now on) and
+// the others (LO). All warps of a warpgroup have to execute the same setmaxnreg,
+// so this stands before the roles split and FIRST is a multiple of four; what
+// one side takes, the other gives up. True in the warps below FIRST.
+template <int FIRST, int HI, int LO>
+__device__ __forceinline__ bool split_registers(int warp)
+{
+	constexpr int rest = kPThreads / 32 - FIRST;
+	static_assert(FIRST % 4 == 0 && rest % 4 == 0, "a warpgroup takes one setmaxnreg");
+	static_assert(FIRST * HI + rest * LO <= kPThreads / 32 * kRegsLaunch, "more than the launch holds");
+	static_assert(HI % 8 == 0 && LO % 8 == 0 && HI >= kRegsLaunch && LO <= kRegsLaunch, "inc and dec");
+	if (warp < FIRST) {
+		asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(HI));
+		return true;
+	}
+	asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(LO));
+	return false;
+}
 
 struct PGroup {
 	long long x0;         // first work step of the group's units
@@ -677,9 +697,8 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 	const int sec = bs * (G::MX ? D * 9 / 8 : D * 2);
 	auto wait = [&](uint64_t *bar, uint32_t parity) { return p_wait(&sm.abort, bar, parity, a.err); };
 
-	if (warp < kWarpProd) {
+	if (split_registers<kWarpProd, 160, 96>(warp)) {
 		// ================= softmax of stream t ========================================
-		asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
 		const int t = warp >> 2, rr = (warp & 3) * 32 + lane;
 		const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
 		const uint32_t tS = lane_base + col_s(t), tO = lane_base + col_o(t);
@@ -775,7 +794,6 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 		}
 	} else if (warp < kWarpMma) {
 		// ================= producers ====================================================
-		asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
 		// An item is 16 keys of K or V of one block (never more than one page), 16
 		// items a block, and each warp takes every kPW-th on its own: with all
 		// warps on one tile at a time, half of the time went into its barriers.
@@ -909,9 +927,7 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 			}
 			gb0 += p.nb;
 		}
-	} else {
-	asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-	if (warp == kWarpMma) {
+	} else if (warp == kWarpMma) {
 		// ================= MMA issue =======================================================
 		// The whole warp runs this role (descriptors stay warp-uniform); one
 		// elected lane issues.
@@ -1145,7 +1161,6 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 			}
 		}
 	}
-	}
 
 	tc_fence_before();
 	__syncthreads();
@@ -1290,13 +1305,9 @@ __device__ __forceinline__ void suffix_role(const kllm_prefix_args &a, uint8_t *
 		fence_mbar_init();
 	}
 	__syncthreads();
-	if constexpr (!Gm::MX) {
-		if (warp >= NW) {
-			asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+	if constexpr (!Gm::MX)
+		if (!split_registers<NW, 184, 72>(warp))
 			return;
-		}
-		asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-	}
 	const int *pre = local ? spre : a.tile_pre;
 	const int w = cta * NW + warp;
 	if (w >= WS)
