@@ -219,3 +219,21 @@ def test_a_vocabulary_past_the_segment_table(be, bf16):
     """More than 1,024 segments of four vectors: segments grow with the row."""
     V = 1300007
     check(be, normal(2, V, 21), some_targets(2, V, 3, 5), 32, bf16=bf16, shift=1)
+
+
+@pytest.mark.parametrize("R,V", [(2, 128256), (300, 70001), (3, 33000), (400, 5000)])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_finite_masks_with_few_tokens_allowed(be, R, V, bf16):
+    """Thousands of equal logits under a handful of larger ones that lie far
+    apart: the exact selection meets one of those in every part of the row.
+    Fewer and more of them than alternatives; rows of one CTA and of several."""
+    fills = [-1e4, -3.0, -1e4, 0.0]          # bf16 values or nearly so
+    x = np.empty((R, V), np.float32)
+    t = np.zeros((R, 2), int)
+    for r in range(R):
+        n = 2 + 3 * (r % 4)                  # 2 .. 11 allowed tokens
+        at = (np.arange(n) * (V - 2)) // (n - 1) + (r % 2)
+        x[r] = fills[r % 4]
+        x[r, at] = 1.0 + np.arange(n) % 5
+        t[r] = (at[-1], at[0] + 1)
+    check(be, x, t, 7 if R > 100 else 20, bf16=bf16)

@@ -69,6 +69,7 @@ struct LpSmem {
 	uint32_t hist[256];
 	uint32_t prefix;
 	int remain, base_eq;
+	int done;                             // radix_candidates: nothing more to find
 	int wcnt[16];
 };
 
@@ -265,7 +266,7 @@ __device__ __noinline__ void radix_candidates(const typename Elem<BF16>::T *row,
 		sm.base_eq = 0;               // equals taken so far
 	}
 	__syncthreads();
-	// in index order, 512 elements at a time: equals keep their order
+	// in index order, TH elements at a time: equals keep their order
 	for (int base = 0; base < V; base += TH) {
 		const int i = base + tid;
 		const float l = i < V ? Elem<BF16>::get(row + i) : 0.f;
@@ -293,10 +294,14 @@ __device__ __noinline__ void radix_candidates(const typename Elem<BF16>::T *row,
 			sm.cand_i[n_gt + at] = i;
 		}
 		__syncthreads();
-		if (tid == 0)
+		// One thread decides for all, while no warp can be counting: a warp of the
+		// next round would change n_cand under the others' test of it.
+		if (tid == 0) {
 			sm.base_eq += all;
+			sm.done = sm.base_eq >= need_eq && sm.n_cand >= n_gt;
+		}
 		__syncthreads();
-		if (sm.base_eq >= need_eq && sm.n_cand >= n_gt)
+		if (sm.done)
 			break;
 	}
 	if (tid == 0)
