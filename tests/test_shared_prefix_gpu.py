@@ -284,3 +284,59 @@ def test_refusals(be):
     assert be.shared_prefix(**{**ok, "num_seqs": 0, "num_groups": 0}) == 0
     short = kb.SharedPrefixParams(struct_size=8)
     assert be.lib.kllm_gpu_shared_prefix_attention(be.ctx, ctypes.byref(short)) == kb.EINVAL
+
+
+def decode_of(be, case, dev, scale):
+    """kllm_gpu_paged_attention_v2 of the same tables."""
+    import torch
+    c = case.cfg
+    out = torch.zeros_like(dev.out)
+    rc = be.decode_v2(output=out.data_ptr(), query=dev.q.data_ptr(),
+                      block_tables=dev.tab.data_ptr(), seq_lens=dev.lens.data_ptr(),
+                      num_seqs=len(case.lens), num_heads=c.hq, num_kv_heads=c.hkv, head_dim=c.d,
+                      max_blocks_per_seq=case.max_blocks, block_size=c.block, kv_dtype=c.kv_dtype,
+                      layer=0, layer_stride=c.layer_stride(), scale=scale, split=1,
+                      stream=torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    return wl.bf16_to_f32(out.cpu().numpy().view(np.uint16))
+
+
+def assert_contract(got, want, what):
+    """The parity contract of attention outputs."""
+    r = np.abs(got - want) / (1e-3 + 2e-2 * np.abs(want))
+    assert np.isfinite(got).all() and r.max() <= 1.0, (what, float(r.max()))
+
+
+@pytest.mark.parametrize("kv,size,unit", [(MX, 4000.0, 1 / 64), (BF16, 400.0, 1 / 16)])
+@pytest.mark.parametrize("hq,hkv,n", [(8, 2, 6), (8, 1, 33)])
+def test_values_that_cancel(be, kv, size, unit, hq, hkv, n):
+    """Two keys of nearly equal weight hold nearly opposite values: the output
+    is what is left of a few thousand, so P has to keep more bits than the
+    output. The two lie in one block, or in blocks of different streams."""
+    import kvcase
+    import oracle
+    c = cfg(kv, hq, hkv)
+    rng = np.random.default_rng(n)
+    for first, second in ((37, 90), (37, 200), (130, 390)):
+        case = pc.PrefixCase(c, [(400, suffixes(n, 400, 20, 3))])
+        pages, bs = len(case.arena), c.block
+        k = np.zeros((pages * bs, hkv, c.d), np.float32)
+        v = rng.standard_normal(k.shape).astype(np.float32)
+        amp = size * (0.25 + 0.75 * rng.random((hkv, c.d)))
+        for tok, sign in ((first, 1.0), (second, -1.0)):
+            at = case.slots[0, tok // bs] * bs + tok % bs
+            k[at], k[at, :, 0] = 8.0, sign / 16           # 20 nats above the others
+            v[at] = sign * amp
+        for which, x in ((0, k), (1, v)):
+            b = wl.f32_to_bf16(x)
+            pay, sc = oracle.mx_quantize(b) if kv == MX else (b, None)
+            case.arena[:, 0, which] = kvcase._pages_from_rows(c, pay, sc, pages, 0)
+        q = np.full((n, hq, c.d), 0.25, np.float32)
+        q[:, :, 0] = rng.integers(4, 30, (n, hq)) * unit * rng.choice([-1, 1], (n, hq))
+        case.q = wl.f32_to_bf16(q)
+        dev = pc.OnDevice(case)
+        want = case.want()[0]
+        assert np.median(np.abs(want)) > 0.3
+        assert_contract(decode_of(be, case, dev, c.scale), want, "decode")
+        assert_contract(dev.run(be), want, (first, second))

@@ -78,6 +78,30 @@ __device__ __forceinline__ float ex2_approx(float x)
 	return y;
 }
 
+// Two fp32 values as one operand of the packed instructions.
+__device__ __forceinline__ uint64_t pack2(float a, float b)
+{
+	uint64_t r;
+	asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+	return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b)
+{
+	asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+	uint64_t r;
+	asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+	return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+	uint64_t r;
+	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+	return r;
+}
+
 // Bounded wait: each try_wait suspends for a hardware-bounded interval, so
 // kMaxTries bounds the wait to well under a minute. Returns false on expiry.
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity)
@@ -216,6 +240,14 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
 {
 	__half2 v = __floats2half2_rn(lo, hi);
 	return *reinterpret_cast<uint32_t *>(&v);
+}
+
+// Same, cut instead of rounded.
+__device__ __forceinline__ uint32_t pack_f16x2_rz(float lo, float hi)
+{
+	uint32_t d;
+	asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+	return d;
 }
 
 __device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b)

@@ -73,30 +73,6 @@ struct LpSmem {
 	int wcnt[16];
 };
 
-// Two fp32 values as one operand of the packed instructions.
-__device__ __forceinline__ uint64_t pack2(float a, float b)
-{
-	uint64_t r;
-	asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-	return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b)
-{
-	asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
-{
-	uint64_t r;
-	asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-	return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
-{
-	uint64_t r;
-	asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-	return r;
-}
-
 template <int BF16>
 struct Elem;
 template <>

@@ -38,10 +38,10 @@
 //   14         TMEM allocation and MMA issue
 //   15         page lookup, and the pages on their way to L2
 // MX computes in f16 like the decode: K and V are payload x scale / 4, the
-// query row times a power of two; P is one f16 (11 bits; its 2^-12 stays under
-// the output's 2^-9) built 2^7 larger, so that what underflows is below 2^-32
-// of the row's largest. BF16 pages keep P as bf16 hi + lo: one bf16 P would add
-// as much error as the output's own rounding.
+// query row times a power of two, P built 2^7 larger, so that what underflows is
+// below 2^-32 of the row's largest. P is a hi + lo pair of V's type as in the
+// decode (f16: 21 bits, bf16: 16) and takes two products: with one f16 an output
+// left over from values of 4,000 that cancel missed 1e-3 + 2e-2 |out| by 15x.
 //
 // suffix_role. The decode's tiles (16 tokens of one sequence and kv head, all G
 // query heads, m16n8k16) laid end to end; each warp takes an equal contiguous
@@ -52,12 +52,12 @@
 //
 // Bound: the floor is HBM (each shared page once, each own page once) or, for
 // many rows, the tensor core; what holds is each stream's chain softmax -> P V
-// -> S -> softmax, 4-5k cycles for a pair of blocks whose products take 1.5-2k
-// (leaving out the exponentials and the placing of codes altogether saves 7%),
-// and some 30 us of plan, first block, last block and join. Measured, 32 query
-// heads on 8 kv heads, d 128, MX, pages not in L2: 64 rows that share 8,192
-// tokens (93 MB) 58 us, 1.6 TB/s; 256 rows (34.8 GFLOP) 93 us, 374 TFLOP/s; 8
-// rows that share 512 tokens 20.5 us.
+// -> S -> softmax, some 5k cycles for a pair of blocks (with a P of one f16 4-5k,
+// of which the products took 1.5-2k; they take twice that for P V now), and some
+// 30 us of plan, first block, last block and join. Measured, 32 query heads on 8
+// kv heads, d 128, MX, pages not in L2: 64 rows that share 8,192 tokens (93 MB)
+// 60-64 us, 1.5 TB/s; 256 rows (34.8 GFLOP) 114 us, 305 TFLOP/s (with one f16
+// 56 and 100); 8 rows that share 512 tokens 20.5 us.
 
 #include "kllm_decode_tile.cuh"
 #include "kllm_device.cuh"
@@ -127,8 +127,9 @@ static_assert(sizeof(PHeader) == 64 && sizeof(PGroup) == 48, "workspace layout")
 
 constexpr int kPlanThreads = 256;
 // A CTA's time for n steps or for n tiles a warp, in ns, as measured on the
-// whole chip: set-up, then the rate. They only balance the two parts; for 256
-// rows of 8,192 shared tokens any split from 96 to 108 CTAs of 148 is within 4%.
+// whole chip: set-up, then the rate. They only balance the two parts: steps of
+// 1,500 and 1,800 ns give 105 and 102 us for 256 rows of 8,192 shared tokens, 53
+// and 55 us for 64 rows.
 constexpr float kStepSetNs = 10500.f, kStepNsMx = 1500.f, kStepNsBf16 = 2700.f;
 constexpr float kTileSetNs = 5000.f, kTileNs = 2500.f;
 // Each further unit that a CTA works on (64 rows with 16 or 128 shared tokens:
@@ -518,8 +519,8 @@ __device__ __forceinline__ void load_scores(uint32_t taddr, bool full, const uin
 		}
 }
 
-// One 128-key block of one row: S in the TMEM columns of tS -> P over them
-// (f16 pairs in columns 0-63, or bf16 groups of 8 hi + 8 lo). The row's block
+// One 128-key block of one row: S in the TMEM columns of tS -> P over them, 16
+// columns for 16 keys: 8 of hi pairs, 8 of lo pairs. The row's block
 // maximum is known before any P is written, so raising the reference rescales
 // only O and l. Warp-collective; branches around TMEM accesses are
 // warp-uniform. Returns through m_ref and l_sum. Keys 0-63 are announced on
@@ -564,27 +565,39 @@ __device__ __forceinline__ void softmax_rows(uint32_t tS, uint32_t tO, const uin
 	}
 	// no key present yet (m_ref = -inf): every p is 0, not exp2(-inf + inf)
 	const float moff = m_ref == -CUDART_INF_F ? -CUDART_INF_F : shift - m_ref;
+	// two keys an instruction where the hardware has it
+	const uint64_t sl2_2 = pack2(sl2, sl2), moff_2 = pack2(moff, moff);
 	float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-	for (int c = 0; c < 128; c += MX ? 32 : 16) {
+	for (int c = 0; c < 128; c += 16) {
 		float w[16];
 #pragma unroll
-		for (int i = 0; i < (MX ? 16 : 8); ++i) {
+		for (int i = 0; i < 8; ++i) {
 			const int k = c + 2 * i;
-			const float p0 = ex2_approx(fmaf(__uint_as_float(r[k >> 4][k & 15]), sl2, moff));
-			const float p1 = ex2_approx(fmaf(__uint_as_float(r[k >> 4][(k & 15) + 1]), sl2, moff));
-			sum[i & 3] += p0 + p1;
+			float x0, x1;
+			unpack2(fma2(pack2(__uint_as_float(r[k >> 4][k & 15]),
+					   __uint_as_float(r[k >> 4][(k & 15) + 1])), sl2_2, moff_2), x0, x1);
+			const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
 			if constexpr (MX) {
-				w[i] = __uint_as_float(pack_f16x2(p0, p1));
+				float &s0 = sum[2 * (i & 1)], &s1 = sum[2 * (i & 1) + 1];
+				unpack2(add2(pack2(s0, s1), pack2(p0, p1)), s0, s1);
+				// hi: P cut to f16's 11 bits; lo: what that leaves off
+				const float n0 = __uint_as_float((__float_as_uint(p0) & 0xFFFFE000u) | 0x80000000u);
+				const float n1 = __uint_as_float((__float_as_uint(p1) & 0xFFFFE000u) | 0x80000000u);
+				float l0, l1;
+				unpack2(add2(pack2(p0, p1), pack2(n0, n1)), l0, l1);
+				w[i] = __uint_as_float(pack_f16x2_rz(p0, p1));
+				w[8 + i] = __uint_as_float(pack_f16x2(l0, l1));
 			} else {
+				sum[i & 3] += p0 + p1;
 				const uint32_t hi = pack_bf16x2(p0, p1);
 				w[i] = __uint_as_float(hi);
 				w[8 + i] = __uint_as_float(pack_bf16x2(p0 - __uint_as_float(hi << 16),
 								       p1 - __uint_as_float(hi & 0xFFFF0000u)));
 			}
 		}
-		tmem_st16_nowait(tS + (MX ? c / 2 : c), w);
-		if (c + (MX ? 32 : 16) == 64) {
+		tmem_st16_nowait(tS + c, w);
+		if (c + 16 == 64) {
 			tmem_wait_st();
 			tc_fence_before();
 			mbar_arrive(p_half);
@@ -976,17 +989,11 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 			const uint32_t d = tmem + col_o(t), pa = tmem + col_s(t);
 #pragma unroll
 			for (int g = half * 4; g < half * 4 + 4; ++g) {        // 16-key groups
-				if constexpr (G::MX) {
-					if (leader)
-						umma_f16_ts(d, pa + 8u * g, dv + (uint64_t)((g * 2048) >> 4), id_pv,
-							    (first && g == 0) ? 0u : 1u);
-				} else {
 #pragma unroll
-					for (int lo = 0; lo < 2; ++lo)
-						if (leader)
-							umma_f16_ts(d, pa + 16u * g + 8u * lo, dv + (uint64_t)((g * 2048) >> 4),
-								    id_pv, (first && g == 0 && lo == 0) ? 0u : 1u);
-				}
+				for (int lo = 0; lo < 2; ++lo)
+					if (leader)
+						umma_f16_ts(d, pa + 16u * g + 8u * lo, dv + (uint64_t)((g * 2048) >> 4),
+							    id_pv, (first && g == 0 && lo == 0) ? 0u : 1u);
 			}
 			__syncwarp();
 		};
