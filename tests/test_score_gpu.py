@@ -213,3 +213,21 @@ def test_refusals(be):
     assert be.score_tokens(**{**ok, "num_rows": 0}) == 0
     short = kb.ScoreParams(struct_size=8)
     assert be.lib.kllm_gpu_score_tokens(be.ctx, ctypes.byref(short)) == kb.EINVAL
+
+
+@pytest.mark.parametrize("V", [128256, 33000])
+@pytest.mark.parametrize("top", [1, 20, 32])
+def test_logits_of_zero_at_the_threshold(be, V, top):
+    """A padding row of zeros has every logit at 0, and its alternatives are the
+    lowest indices; so do rows with a few positive logits over many zeros."""
+    R, K = 6, 64
+    h, w = grid_case(R, K, V, V + top)
+    h[:4] = 0
+    w[:, :3] = 0
+    h[1, 0] = h[2, 1] = h[3, 2] = 0.25
+    w[::7, 0] = -0.125                       # zeros and below
+    w[np.arange(0, V, V // 5), 1] = 0.125    # five or six above zero
+    w[:, 2] = -0.125                         # nothing but the last few at zero
+    w[V - 40:, 2] = 0
+    got = check(be, h, w, some_targets(R, V, 2, 1), top)
+    assert (got["top_ids"][0] == np.arange(top)).all()

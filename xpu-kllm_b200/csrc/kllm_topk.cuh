@@ -42,6 +42,13 @@ __device__ __forceinline__ float value_of(uint32_t key)
 {
 	return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
+// The largest value below v. The key below +0 stands for -0, which compares
+// equal to it, so zero steps over that one.
+__device__ __forceinline__ float value_below(float v)
+{
+	const uint32_t key = key_of(v) - 1u;
+	return value_of(key == 0x7fffffffu ? key - 1u : key);
+}
 
 // 32 values, one a lane, sorted descending over the warp (bitonic network).
 __device__ __forceinline__ float bitonic_step(float x, int stride, bool keep_max)

@@ -405,7 +405,7 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 					}
 					tau = cut_list<kSN / 8, false>(list, k, 4 * nc, tau).tau;
 					if (tau > -CUDART_INF_F)                 // its equals are wanted
-						tau = value_of(key_of(tau) - 1u);
+						tau = value_below(tau);
 				}
 #pragma unroll 1
 				for (int ch = 0; ch < nc; ++ch) {
