@@ -77,6 +77,35 @@ def assert_near(got, want, tol, what):
         what, float((err / tol[fin]).max()), got[fin][np.argmax(err / tol[fin])])
 
 
+def distance_bound(entropy, distance, V):
+    """Absolute bound of a log-probability that is formed from its distance D to
+    the row's maximum and the logarithm of the sum S relative to it. The distance
+    is one subtraction, one division and one product (3 eps D) and enters one
+    more; ln S takes four roundings of at most ln V. A term of S is 2^d with d off
+    by 5 eps of itself (D times two constants, on average the entropy at most) and
+    the exponential's 2^-22; each raise of a thread's maximum (one a batch of at
+    least 4,096 elements a CTA) and each of up to 16 joins is such a factor too,
+    and a thread adds at most V / 512 + 64 terms, the joins 32 more."""
+    rel = 5 * EPS * entropy + (V / 4096 + 17) * 2.0 ** -22 + (V / 512 + 96) * EPS
+    return rel + 4 * EPS * distance + 5 * EPS * (np.log(V) + 1)
+
+
+def assert_distances(got, want, V):
+    """Log-probabilities within distance_bound, whatever the logits' size, and
+    none above 0; the entropy weighs each term's error by its distance, on average
+    the entropy itself; lse alone keeps the size of the logits."""
+    ent = want["entropy"]
+    for k in ("logprob", "top_logprobs"):
+        dist = np.maximum(0.0, want["top_logprobs"][:, :1] - want[k])
+        assert (got[k] <= 0).all(), k
+        assert_near(got[k], want[k], distance_bound(ent[:, None], dist, V), k)
+    tol = distance_bound(ent, 0.0, V)
+    assert_near(got["entropy"], want["entropy"], 2 * tol * (1 + ent) + tol, "entropy")
+    assert (got["entropy"] >= 0).all()
+    assert_near(got["lse"], want["lse"], tol + 4 * EPS * want["zmax"], "lse")
+    assert (got["top_ids"] == want["top_ids"]).all()
+
+
 def layout(ctx_lens, new_lens, fork_from, free, table, *, block, base, slot_bytes, total, k_off,
            v_off, capacity):
     """Batch layout by its rules, one row and one token at a time. table:

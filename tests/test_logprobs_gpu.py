@@ -237,3 +237,47 @@ def test_finite_masks_with_few_tokens_allowed(be, R, V, bf16):
         x[r, at] = 1.0 + np.arange(n) % 5
         t[r] = (at[-1], at[0] + 1)
     check(be, x, t, 7 if R > 100 else 20, bf16=bf16)
+
+
+@pytest.mark.parametrize("R,V", [(1, 128256), (3, 33000), (5, 700)])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("temperature", [None, 4.0, 0.5])
+def test_rows_of_the_lowest_value(be, R, V, bf16, temperature):
+    """A finite mask that leaves nothing is a row of equal logits: its softmax
+    is uniform. The largest finite logits, and both in one row, hold as well."""
+    import torch
+    low = float(torch.finfo(torch.bfloat16 if bf16 else torch.float32).min)
+    t = np.tile([0, V // 2, V - 1], (R, 1))
+    tmp = None if temperature is None else np.full(R, temperature, np.float32)
+    for fill, other in ((low, low), (-low, -low), (low, -low)):
+        x = np.full((R, V), fill, np.float32)
+        x[:, 1::3] = other
+        got = run(be, x, t, 20, tmp, bf16)
+        n = V if fill == other else len(range(1, V, 3))
+        tol = sc.distance_bound(np.log(n), 0.0, V)
+        sc.assert_near(got["entropy"], np.full(R, np.log(n)), 4 * tol, "entropy")
+        sc.assert_near(got["top_logprobs"], np.full((R, 20), -np.log(n)), tol, "top")
+        want = np.where(x[np.arange(R)[:, None], t] == x.max(1, keepdims=True), -np.log(n), -np.inf)
+        lp = got["logprob"].astype(np.float64)
+        lp = np.where(lp < -1e30, -np.inf, lp)      # a distance of 6.8e38 / T rounds to -inf or not
+        sc.assert_near(lp, want, tol, "logprob")
+        first = np.arange(20) if fill == other else 1 + 3 * np.arange(20)
+        assert (got["top_ids"] == first).all()
+        with np.errstate(over="ignore"):
+            lse = (np.float64(max(fill, other)) / (temperature or 1.0) + np.log(n)).astype(np.float32)
+        fine = np.where(np.isfinite(lse), 2.0 ** -20 * np.abs(lse), 0.0)
+        sc.assert_near(got["lse"], np.full(R, lse, np.float64), fine, "lse")
+
+
+@pytest.mark.parametrize("offset,temperature", [(0, None), (1000, None), (-5e4, None), (0, 0.01),
+                                                (0, 1e-3), (300, 0.02), (-1e6, 0.5)])
+@pytest.mark.parametrize("R,V", [(1, 128256), (40, 20000), (5, 3001)])
+def test_distances_to_the_maximum(be, R, V, offset, temperature):
+    """Log-probabilities depend on the distance to the row's maximum alone: a
+    common offset and a low temperature cost no accuracy, and none is above 0."""
+    x = normal(R, V, V + R) + np.float32(offset)
+    tmp = None if temperature is None else np.full(R, temperature, np.float32)
+    t = some_targets(R, V, 3, 8)
+    t[:, 2] = x.argmax(1)
+    got = run(be, x, t, 20, tmp)
+    sc.assert_distances(got, sc.rows(x, tmp, t, 20), V)

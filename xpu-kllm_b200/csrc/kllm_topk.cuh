@@ -32,6 +32,28 @@ __device__ __forceinline__ void join(float &m, float &s, float &w, float m2, flo
 	m = M;
 }
 
+// The same with m the maximum logit itself and sums of 2^((l - m) c): a raise
+// from m to M is (M - m) c, cut where 2^-d is 0 (M - m may be infinite).
+__device__ __forceinline__ float raise_of(float m, float M, float c)
+{
+	return fminf((M - m) * c, 1000.f);
+}
+__device__ __forceinline__ void join(float &m, float &s, float &w, float m2, float s2, float w2, float c)
+{
+	const float M = fmaxf(m, m2);
+	if (M == -CUDART_INF_F) {     // nothing finite on either side (NaN sums stay NaN)
+		s += s2;
+		w += w2;
+		return;
+	}
+	const float d1 = m == -CUDART_INF_F ? 0.f : raise_of(m, M, c);
+	const float d2 = m2 == -CUDART_INF_F ? 0.f : raise_of(m2, M, c);
+	const float f1 = ex2_approx(-d1), f2 = ex2_approx(-d2);
+	w = f1 * fmaf(-d1, s, w) + f2 * fmaf(-d2, s2, w2);
+	s = f1 * s + f2 * s2;
+	m = M;
+}
+
 // fp32 values as unsigned integers of the same order (-0 as +0), and back.
 __device__ __forceinline__ uint32_t key_of(float v)
 {

@@ -5,11 +5,16 @@
 // The reference has no counterpart: its sampler keeps one token and no
 // probability (userspace/decode/decode_loop.c:58-185).
 //
-// With y = l x log2(e) / T (l: logit) every thread keeps, over its elements,
-//   m = max y,  S = sum 2^(y - m),  W = sum 2^(y - m) (y - m)
-// and raises m a batch at a time: for m' = m + d the sums become S' = 2^-d S,
+// With c = log2(e) / T every thread keeps, over its logits l,
+//   m = max l,  S = sum 2^((l - m) c),  W = sum 2^((l - m) c) (l - m) c
+// and raises m a batch at a time: for d = (m' - m) c the sums become S' = 2^-d S,
 // W' = 2^-d (W - d S). Triples of threads, warps and CTAs join by the same
-// rule; then lse = (m + log2 S) ln 2 and the entropy is (log2 S - W / S) ln 2.
+// rule; then lse = m / T + log2 S ln 2 and the entropy is (log2 S - W / S) ln 2.
+// The maximum is subtracted before the product: the sums do not depend on the
+// logits' size, and m c may pass fp32's range where the logits do not (a row
+// masked with the type's lowest value). A log-probability is the distance to the
+// maximum, (l - m) / T - log2 S ln 2, for the same reason: z - lse would round at
+// the size of z.
 //
 // Top alternatives, in the same pass. The elements fall into 32 groups by lane,
 // and each group's maximum so far is kept; the k-th largest of those, tau, is
@@ -65,7 +70,7 @@ struct LpSmem {
 	int ti[kTgtMax];                      // their indices
 	float tau_run;                        // the last threshold a warp found, only ever raised
 	float tau;
-	float sub;                            // what logprobs subtract: lse, 0 in an empty row
+	float top, ln_s;                      // the row's maximum and ln S, 0 in an empty row
 	uint32_t hist[256];
 	uint32_t prefix;
 	int remain, base_eq;
@@ -355,8 +360,8 @@ logprobs_kernel(const kllm_logprobs_args a)
 
 	const int stride = CL * kWarps * kBatch, b0 = (rank * kWarps + warp) * kBatch;
 	const float temp = a.temperature ? a.temperature[r] : 1.f;
-	const float inv_t = temp > 0.f ? 1.f / temp : 1.f;
-	const float c = kLog2e * inv_t;
+	const float inv_t = temp > 0.f ? fminf(1.f / temp, FLT_MAX) : 1.f;
+	const float c = fminf(kLog2e * inv_t, FLT_MAX);
 
 	// ---- one pass: this thread's (m, S, W), ranks, segment maxima --------------
 	// A batch at a time: one maximum, one look at the reference and one at each
@@ -391,14 +396,13 @@ logprobs_kernel(const kllm_logprobs_args a)
 #pragma unroll
 		for (int q = 0; q < kFly; ++q)
 			bm = fmaxf(bm, Elem<BF16>::vmax(raw[q]));
-		const float ym = bm * c;
-		if (ym > m) {
+		if (bm > m) {
 			if (m > -CUDART_INF_F) {
-				const float d = ym - m, f = ex2_approx(-d);
+				const float d = raise_of(m, bm, c), f = ex2_approx(-d);
 				W = f * fmaf(-d, S, W);
 				S *= f;
 			}
-			m = ym;
+			m = bm;
 		}
 		const float ref = m == -CUDART_INF_F ? 0.f : m;
 		// two elements an instruction where the hardware has it
@@ -411,7 +415,7 @@ logprobs_kernel(const kllm_logprobs_args a)
 #pragma unroll
 			for (int z = 0; z < kVec; z += 2) {
 				float d0, d1;
-				unpack2(fma2(pack2(x[z], x[z + 1]), c2, r2), d0, d1);
+				unpack2(mul2(add2(pack2(x[z], x[z + 1]), r2), c2), d0, d1);
 				const uint64_t e2 = pack2(ex2_approx(d0), ex2_approx(d1));
 				s2 = add2(s2, e2);
 				w2 = fma2(e2, pack2(fmaxf(d0, -1000.f), fmaxf(d1, -1000.f)), w2);  // 0 x -inf counts 0
@@ -499,7 +503,7 @@ logprobs_kernel(const kllm_logprobs_args a)
 		const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
 		const float s2 = __shfl_xor_sync(0xffffffffu, S, o);
 		const float w2 = __shfl_xor_sync(0xffffffffu, W, o);
-		join(m, S, W, m2, s2, w2);
+		join(m, S, W, m2, s2, w2, c);
 	}
 	if (lane == 0) {
 		sm.wm[warp] = m;
@@ -521,7 +525,7 @@ logprobs_kernel(const kllm_logprobs_args a)
 			const float m2 = __shfl_xor_sync(0xffffffffu, M, o);
 			const float s2 = __shfl_xor_sync(0xffffffffu, s, o);
 			const float w2 = __shfl_xor_sync(0xffffffffu, w, o);
-			join(M, s, w, m2, s2, w2);
+			join(M, s, w, m2, s2, w2, c);
 		}
 		if (k > 0)
 			atomicMax(&lead->all_key[lane], sm.gkey[lane]);
@@ -558,23 +562,22 @@ logprobs_kernel(const kllm_logprobs_args a)
 			const float m2 = __shfl_xor_sync(0xffffffffu, M, o);
 			const float s2 = __shfl_xor_sync(0xffffffffu, s, o);
 			const float w2 = __shfl_xor_sync(0xffffffffu, w, o);
-			join(M, s, w, m2, s2, w2);
+			join(M, s, w, m2, s2, w2, c);
 		}
-		const float l2 = log2f(s);
 		const bool dead = M == -CUDART_INF_F && s == 0.f;
-		const float lse = dead ? -CUDART_INF_F : (M + l2) * kLn2;
-		const float sub = dead ? 0.f : lse;
+		const float l2 = log2f(s), top = dead ? 0.f : M, ln_s = dead ? 0.f : l2 * kLn2;
 		if (lane == 0) {
-			sm.sub = sub;
+			sm.top = top;
+			sm.ln_s = ln_s;
 			if (a.lse)
-				a.lse[r] = lse;
+				a.lse[r] = dead ? -CUDART_INF_F : fmaf(M, inv_t, ln_s);
 			if (a.entropy)
 				a.entropy[r] = dead ? 0.f : (l2 - w / s) * kLn2;
 		}
 		if (lane < nt) {
 			const bool in = sm.ti[lane] >= 0;
 			const float l = in ? sm.tl[lane] : -CUDART_INF_F;
-			a.target_lp[(size_t)r * nt + lane] = in ? l * inv_t - sub : -CUDART_INF_F;
+			a.target_lp[(size_t)r * nt + lane] = in ? fmaf(l - top, inv_t, -ln_s) : -CUDART_INF_F;
 			if (a.target_rank) {
 				int n = 0;
 				for (int i = 0; i < CL; ++i)
@@ -608,7 +611,7 @@ logprobs_kernel(const kllm_logprobs_args a)
 		}
 		n = k;
 	}
-	__syncthreads();                                    // and sm.sub is set
+	__syncthreads();                                    // and sm.top is set
 	if (warp == 0) {
 		float top = -CUDART_INF_F;
 		for (int i = lane; i < n; i += 32)
@@ -636,7 +639,7 @@ logprobs_kernel(const kllm_logprobs_args a)
 		}
 		if (at < k) {
 			a.top_ids[(size_t)r * k + at] = id;
-			a.top_lp[(size_t)r * k + at] = v * inv_t - sm.sub;
+			a.top_lp[(size_t)r * k + at] = fmaf(v - sm.top, inv_t, -sm.ln_s);
 		}
 	}
 }
