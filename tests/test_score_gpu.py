@@ -231,3 +231,38 @@ def test_logits_of_zero_at_the_threshold(be, V, top):
     w[V - 40:, 2] = 0
     got = check(be, h, w, some_targets(R, V, 2, 1), top)
     assert (got["top_ids"][0] == np.arange(top)).all()
+
+
+@pytest.mark.parametrize("offset,temperature", [(0, None), (256, None), (0, 0.01), (256, 0.02),
+                                                (-256, 0.02)])
+def test_distances_to_the_maximum(be, offset, temperature):
+    """Log-probabilities depend on the distance to the row's maximum alone: a
+    common offset and a low temperature cost no accuracy, and none is above 0."""
+    R, K, V = 70, 128, 9001
+    h, w = grid_case(R, K, V, 31)
+    h[:, 0], w[:, 0] = 16.0, offset / 16.0
+    T = None if temperature is None else np.full(R, temperature)
+    targets = some_targets(R, V, 3, 6)
+    targets[:, 2] = (h @ w.T).argmax(1)
+    got = run(be, h, w, targets, 20, T)
+    want = sc.rows(h.astype(np.float64) @ w.astype(np.float64).T,
+                   None if T is None else T.astype(np.float32), targets, 20)
+    sc.assert_distances(got, want, V)
+
+
+def test_the_likeliest_token_stays_at_or_below_zero(be):
+    """A target's logit is a sum of its own order: it may round above the maximum
+    of the tensor core's, and at a low temperature that would count."""
+    rng = np.random.default_rng(15)
+    R, K, V = 150, 2048, 3000
+    h = wl.bf16_to_f32(wl.f32_to_bf16(rng.standard_normal((R, K)).astype(np.float32)))
+    w = wl.bf16_to_f32(wl.f32_to_bf16((rng.standard_normal((V, K)) * 0.05).astype(np.float32)))
+    logits = h.astype(np.float64) @ w.astype(np.float64).T
+    best = logits.argmax(1)[:, None]
+    got = run(be, h, w, best, 3, np.full(R, 1e-3))
+    assert (got["logprob"] <= 0).all() and (got["top_logprobs"] <= 0).all()
+    # a logit is off by K eps sum |h w|, each of the two in a distance
+    err = 2 * K * sc.EPS * (np.abs(h).astype(np.float64) @ np.abs(w).T.astype(np.float64)).max(1)
+    want = sc.rows(logits, np.full(R, 1e-3, np.float32), best, 3)
+    sc.assert_near(got["logprob"], want["logprob"],
+                   err[:, None] / 1e-3 + sc.distance_bound(want["entropy"], 0.0, V)[:, None], "best")

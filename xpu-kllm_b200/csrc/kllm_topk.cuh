@@ -13,27 +13,11 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
-// Softmax sums of a set of elements y (log2 domain): m = max y, S = sum 2^(y -
-// m), W = sum 2^(y - m) (y - m). join adds the set (m2, s2, w2) to (m, s, w):
-// for a maximum raised by d the sums become 2^-d S and 2^-d (W - d S). A set
-// without elements has m = -inf, S = 0.
-__device__ __forceinline__ void join(float &m, float &s, float &w, float m2, float s2, float w2)
-{
-	const float M = fmaxf(m, m2);
-	if (M == -CUDART_INF_F) {     // nothing finite on either side (NaN sums stay NaN)
-		s += s2;
-		w += w2;
-		return;
-	}
-	const float d1 = m == -CUDART_INF_F ? 0.f : M - m, d2 = m2 == -CUDART_INF_F ? 0.f : M - m2;
-	const float f1 = ex2_approx(-d1), f2 = ex2_approx(-d2);
-	w = f1 * fmaf(-d1, s, w) + f2 * fmaf(-d2, s2, w2);
-	s = f1 * s + f2 * s2;
-	m = M;
-}
-
-// The same with m the maximum logit itself and sums of 2^((l - m) c): a raise
-// from m to M is (M - m) c, cut where 2^-d is 0 (M - m may be infinite).
+// Softmax sums of a set of logits l, c = log2(e) / T: m = max l, S = sum 2^((l -
+// m) c), W = sum 2^((l - m) c) (l - m) c. join adds the set (m2, s2, w2) to (m, s,
+// w): for a maximum raised by d = (M - m) c the sums become 2^-d S and 2^-d (W - d
+// S). A set without elements has m = -inf, S = 0. A raise is cut where 2^-d is 0
+// (M - m may be infinite).
 __device__ __forceinline__ float raise_of(float m, float M, float c)
 {
 	return fminf((M - m) * c, 1000.f);

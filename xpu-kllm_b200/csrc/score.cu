@@ -7,10 +7,10 @@
 // userspace/compute/infer_gpu.c:212-229).
 //
 //   l[r][v] = sum_k hidden[r][k] weight[v][k]     bf16 in, fp32 sums, tcgen05
-// and per row, over its logits as they leave the tensor core, in the log2
-// domain y = l log2(e) / T: m = max y, S = sum 2^(y - m), W = sum 2^(y - m)
-// (y - m), joined as in logprobs.cu; lse = (m + log2 S) ln 2, entropy =
-// (log2 S - W / S) ln 2.
+// and per row, over its logits as they leave the tensor core, with c = log2(e) /
+// T: m = max l, S = sum 2^((l - m) c), W = sum 2^((l - m) c) (l - m) c, joined as
+// in logprobs.cu; lse = m / T + log2 S ln 2, entropy = (log2 S - W / S) ln 2, and a
+// log-probability is (l - m) / T - log2 S ln 2.
 //
 // score_kernel: a CTA owns 128 rows and a contiguous range of the vocabulary
 // (in units of 64 columns, so ranges differ by one unit at most), taken as
@@ -43,6 +43,8 @@
 #include "kllm_internal.h"
 #include "kllm_topk.cuh"
 #include "kllm_umma.cuh"
+
+#include <cfloat>
 
 namespace kllm {
 namespace {
@@ -362,7 +364,7 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 				continue;
 			const int row = rb * kSR + t;            // past the last: a row of zeros
 			const float T = (row < a.num_rows && a.temperature) ? a.temperature[row] : 1.f;
-			const float c = kLog2e * (T > 0.f ? 1.f / T : 1.f);
+			const float c = fminf(kLog2e * (T > 0.f ? 1.f / T : 1.f), FLT_MAX);
 			float m = -CUDART_INF_F, S = 0.f, W = 0.f, tau = -CUDART_INF_F;
 			uint32_t at = list;                // where the next entry goes
 			for (int u = u0; u < u1; u += 4, ++it) {
@@ -433,28 +435,35 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 #pragma unroll
 					for (int i = 4; i < 32; ++i)
 						c4[i & 3] = fmaxf(c4[i & 3], v[i]);
-					const float ym = fmaxf(fmaxf(c4[0], c4[1]), fmaxf(c4[2], c4[3])) * c;
-					if (ym > m) {
+					const float bm = fmaxf(fmaxf(c4[0], c4[1]), fmaxf(c4[2], c4[3]));
+					if (bm > m) {
 						if (m > -CUDART_INF_F) {
-							const float d = ym - m, f = ex2_approx(-d);
+							const float d = raise_of(m, bm, c), f = ex2_approx(-d);
 							W = f * fmaf(-d, S, W);
 							S *= f;
 						}
-						m = ym;
+						m = bm;
 					}
 					// sums of 32, then of the chunks: a range has thousands of
 					// terms, and one running fp32 sum over them lost 2e-6
 					const float ref = m == -CUDART_INF_F ? 0.f : m;
-					float s4[4] = {0.f, 0.f, 0.f, 0.f}, w4[4] = {0.f, 0.f, 0.f, 0.f};
+					// two columns an instruction where the hardware has it
+					const uint64_t c2 = pack2(c, c), r2 = pack2(-ref, -ref);
+					uint64_t s2[2] = {0ull, 0ull}, w2[2] = {0ull, 0ull};
 #pragma unroll
-					for (int i = 0; i < 32; ++i) {
-						const float d = fmaf(v[i], c, -ref);
-						const float e = ex2_approx(d);
-						s4[i & 3] += e;
-						w4[i & 3] = fmaf(e, fmaxf(d, -1000.f), w4[i & 3]);
+					for (int i = 0; i < 32; i += 2) {
+						float d0, d1;
+						unpack2(mul2(add2(pack2(v[i], v[i + 1]), r2), c2), d0, d1);
+						const uint64_t e2 = pack2(ex2_approx(d0), ex2_approx(d1));
+						const int z = (i >> 1) & 1;
+						s2[z] = add2(s2[z], e2);
+						w2[z] = fma2(e2, pack2(fmaxf(d0, -1000.f), fmaxf(d1, -1000.f)), w2[z]);
 					}
-					S += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-					W += (w4[0] + w4[1]) + (w4[2] + w4[3]);
+					float s0, s1, w0, w1;
+					unpack2(add2(s2[0], s2[1]), s0, s1);
+					unpack2(add2(w2[0], w2[1]), w0, w1);
+					S += s0 + s1;
+					W += w0 + w1;
 				}
 				tc_fence_before();
 				mbar_arrive(&sm.acc_empty[buf]);
@@ -519,7 +528,7 @@ score_join_kernel(const kllm_score_args a)
 	const size_t rows = (size_t)a.row_blocks * kSR, stride = (size_t)a.splits * rows;
 	const float4 *part = static_cast<const float4 *>(a.part) + r;
 	const float T = a.temperature ? a.temperature[r] : 1.f;
-	const float inv_t = T > 0.f ? 1.f / T : 1.f;
+	const float inv_t = T > 0.f ? fminf(1.f / T, FLT_MAX) : 1.f, c = fminf(kLog2e * inv_t, FLT_MAX);
 	if (tid == 0)
 		n_cand = n_ranges = 0;
 
@@ -542,22 +551,22 @@ score_join_kernel(const kllm_score_args a)
 	}
 	grid_dependency_wait();                // the ranges' results
 	// With at least top_n ranges, the top_n-th largest of the ranges' maxima is
-	// a threshold that top_n logits reach; warp 0 finds it, as y = l c like m
+	// a threshold that top_n logits reach; warp 0 finds it
 	if (warp == 0 && k > 0) {
 		float top = -CUDART_INF_F;
 		for (int s = lane; s - lane < a.splits; s += 32) {
 			const float d = warp_sort_desc(s < a.splits ? part[(size_t)s * rows].x : -CUDART_INF_F, lane);
 			top = s == lane ? d : warp_merge_desc(top, d, lane);
 		}
-		const float y = __shfl_sync(0xffffffffu, top, k - 1);
+		const float kth = __shfl_sync(0xffffffffu, top, k - 1);
 		if (lane == 0)
-			max_tau = a.splits >= k ? y : -CUDART_INF_F;
+			max_tau = a.splits >= k ? kth : -CUDART_INF_F;
 	}
 	// the ranges' triples and the largest threshold any of them reports
 	float m = -CUDART_INF_F, S = 0.f, W = 0.f, tau = -CUDART_INF_F;
 	for (int s = tid; s < a.splits; s += kJoinThreads) {
 		const float4 p = part[(size_t)s * rows];
-		join(m, S, W, p.x, p.y, p.z);
+		join(m, S, W, p.x, p.y, p.z, c);
 		tau = fmaxf(tau, p.w);
 	}
 #pragma unroll
@@ -565,7 +574,7 @@ score_join_kernel(const kllm_score_args a)
 		const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
 		const float s2 = __shfl_xor_sync(0xffffffffu, S, o);
 		const float w2 = __shfl_xor_sync(0xffffffffu, W, o);
-		join(m, S, W, m2, s2, w2);
+		join(m, S, W, m2, s2, w2, c);
 		tau = fmaxf(tau, __shfl_xor_sync(0xffffffffu, tau, o));
 	}
 	if (lane == 0) {
@@ -581,30 +590,30 @@ score_join_kernel(const kllm_score_args a)
 	tau = red[0][3];
 #pragma unroll
 	for (int i = 1; i < 4; ++i) {
-		join(m, S, W, red[i][0], red[i][1], red[i][2]);
+		join(m, S, W, red[i][0], red[i][1], red[i][2], c);
 		tau = fmaxf(tau, red[i][3]);
 	}
 	const bool dead = m == -CUDART_INF_F && S == 0.f;
-	const float l2 = log2f(S), lse = dead ? -CUDART_INF_F : (m + l2) * kLn2;
-	const float floor_ = dead ? 0.f : lse;
+	const float l2 = log2f(S), top = dead ? 0.f : m, ln_s = dead ? 0.f : l2 * kLn2;
 	if (tid == 0) {
 		if (a.lse)
-			a.lse[r] = lse;
+			a.lse[r] = dead ? -CUDART_INF_F : fmaf(m, inv_t, ln_s);
 		if (a.entropy)
 			a.entropy[r] = dead ? 0.f : (l2 - W / S) * kLn2;
 	}
 	if (tid < nt) {
 		const int t = a.targets[(size_t)r * nt + tid];
 		const float l = dots[tid][0] + dots[tid][1] + dots[tid][2] + dots[tid][3];
+		// this sum's order is not the tensor core's: l may round above the maximum
 		a.target_lp[(size_t)r * nt + tid] =
-		    (t >= 0 && t < a.vocab) ? l * inv_t - floor_ : -CUDART_INF_F;
+		    (t >= 0 && t < a.vocab) ? fmaf(fminf(l - top, 0.f), inv_t, -ln_s) : -CUDART_INF_F;
 	}
 	if (k == 0)
 		return;
 	// the ranges whose maximum reaches the threshold, and their entries that do
-	const float c = kLog2e * inv_t, y_min = max_tau;
+	const float least = fmaxf(max_tau, tau);
 	for (int s = tid; s < a.splits; s += kJoinThreads)
-		if (part[(size_t)s * rows].x >= y_min)
+		if (part[(size_t)s * rows].x >= least)
 			ranges[atomicAdd(&n_ranges, 1)] = s;
 	__syncthreads();
 	const int total = n_ranges * per;
@@ -615,7 +624,7 @@ score_join_kernel(const kllm_score_args a)
 		if (e < a.part_n[at]) {
 			const uint2 x = static_cast<const uint2 *>(a.part_list)[(size_t)e * stride + at];
 			const float v = __uint_as_float(x.x);
-			if (v >= tau && v * c >= y_min) {
+			if (v >= least) {
 				const int p = atomicAdd(&n_cand, 1);
 				cv[p] = v;
 				ci[p] = (int)x.y;
@@ -633,7 +642,7 @@ score_join_kernel(const kllm_score_args a)
 			at += (int)(cv[j] > v) | ((int)(cv[j] == v) & (int)(ci[j] < id));
 		if (at < k) {
 			a.top_ids[(size_t)r * k + at] = id;
-			a.top_lp[(size_t)r * k + at] = v * inv_t - floor_;
+			a.top_lp[(size_t)r * k + at] = fmaf(v - top, inv_t, -ln_s);
 		}
 	}
 	for (int i = n + tid; i < k; i += kJoinThreads) {   // fewer logits above -inf than top_n
