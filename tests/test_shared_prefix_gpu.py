@@ -340,3 +340,22 @@ def test_values_that_cancel(be, kv, size, unit, hq, hkv, n):
         assert np.median(np.abs(want)) > 0.3
         assert_contract(decode_of(be, case, dev, c.scale), want, "decode")
         assert_contract(dev.run(be), want, (first, second))
+
+
+@pytest.mark.parametrize("kv", [MX, BF16])
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.02, -0.0884])
+def test_scales_of_zero_and_below(be, kv, scale):
+    """As the decode has them: equal weights, or the smallest products first.
+    Blocks that are not full, absent pages, one query tile and two."""
+    class Scaled(wl.DecodeConfig):
+        @property
+        def scale(self):
+            return scale
+    for hq, hkv, n, p in ((8, 2, 5, 200), (8, 1, 33, 400), (4, 4, 3, 128)):
+        c = Scaled("shared", 1, hq, hkv, kv_dtype=kv)
+        case = pc.PrefixCase(c, [(p, suffixes(n, p, 30, 2))])
+        case.valid[:, [1, 6]] = False
+        dev = pc.OnDevice(case)
+        want = case.want()[0]
+        assert_contract(decode_of(be, case, dev, scale), want, "decode")
+        assert_contract(dev.run(be), want, (hq, hkv, n, p))

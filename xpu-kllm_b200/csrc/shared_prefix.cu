@@ -64,6 +64,7 @@
 #include "kllm_internal.h"
 #include "kllm_umma.cuh"
 
+#include <cfloat>
 #include <math_constants.h>
 
 namespace kllm {
@@ -610,13 +611,15 @@ __device__ __forceinline__ void softmax_rows(uint32_t tS, uint32_t tO, const uin
 // A warp's 32 query rows into the operand tile: bf16 as they are, or for MX f16
 // after a power of two that puts a row's largest element in [2^14, 2^15);
 // returns the inverse of that factor for row `lane`. off: where row `lane`
-// starts in q, in elements (-1: a row of zeros). Copied in by whole lines, then
+// starts in q, in elements (-1: a row of zeros). neg: the rows change sign, for a
+// softmax scale below 0 (the softmax takes |scale|: absent keys are -inf before
+// it, and the largest product is the largest score). Copied in by whole lines, then
 // converted in place, a row a lane (the swizzle spreads eight rows over all
 // banks). The loops stay rolled: this code runs once a piece, and unrolled it
 // spent 10k cycles on instruction fetches alone.
 template <int D, int KVT>
 __device__ __forceinline__ float load_queries(uint8_t *tile, int r0, int lane, const void *q,
-					      long long off)
+					      long long off, bool neg)
 {
 	constexpr int LPR = D / 8, RPP = 32 / LPR;
 	const int l = lane % LPR, sub = lane / LPR;
@@ -632,9 +635,17 @@ __device__ __forceinline__ float load_queries(uint8_t *tile, int r0, int lane, c
 	cp_async_commit();
 	cp_async_wait<0>();
 	__syncwarp();
-	if constexpr (KVT == 0)
-		return 1.f;
 	const int r = r0 + lane;
+	if constexpr (KVT == 0) {
+		if (neg)
+#pragma unroll 1
+			for (int c = 0; c < LPR; ++c) {
+				uint4 *p = reinterpret_cast<uint4 *>(tile + (c >> 3) * (kPRows * 128) + swz(r, c & 7));
+				const uint4 w = *p;
+				*p = make_uint4(w.x ^ 0x80008000u, w.y ^ 0x80008000u, w.z ^ 0x80008000u, w.w ^ 0x80008000u);
+			}
+		return 1.f;
+	}
 	uint32_t mb = 0u;                                // bf16 magnitudes order as integers
 #pragma unroll 4
 	for (int c = 0; c < LPR; ++c) {
@@ -646,7 +657,7 @@ __device__ __forceinline__ float load_queries(uint8_t *tile, int r0, int lane, c
 	}
 	const int E = mb ? (int)(mb >> 23) - 127 : 0;
 	const int e = min(max(14 - E, -100), 100);
-	const float f = __uint_as_float((uint32_t)(e + 127) << 23);
+	const float f = __uint_as_float(((uint32_t)(e + 127) << 23) | (neg ? 0x80000000u : 0u));
 #pragma unroll 2
 	for (int c = 0; c < LPR; ++c) {
 		uint4 *p = reinterpret_cast<uint4 *>(tile + (c >> 3) * (kPRows * 128) + swz(r, c & 7));
@@ -743,7 +754,8 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 				const int seq = p.row0 + rh / a.group, hh = rh % a.group;
 				const long long off = row < p.rows
 				    ? ((long long)seq * a.num_heads + (long long)p.h * a.group + hh) * D : -1;
-				qf = load_queries<D, KVT>(sm.q[qt], (warp & 3) * 32, lane, a.q, off);
+				qf = load_queries<D, KVT>(sm.q[qt], (warp & 3) * 32, lane, a.q, off,
+							  a.scale_log2 < 0.f);
 				if (G::MX && p.solo)
 					sm.qf[np & 1][rr] = qf;
 				fence_async_smem();
@@ -757,10 +769,14 @@ __device__ __forceinline__ void prefix_role(const kllm_prefix_args &a, PrefixSme
 					break;
 				}
 				tc_fence_after();
-				if (first)
-					sl2 = a.scale_log2 *
+				if (first) {
+					sl2 = fabsf(a.scale_log2) *
 					      (G::MX ? (p.solo && t ? sm.qf[np & 1][rr] : qf) * KLLM_MX_DEC_UNBIAS
 						     : 1.f);
+					// scale 0: the least factor that keeps an absent key at -inf
+					if (sl2 < FLT_MIN)
+						sl2 = FLT_MIN;
+				}
 				if (warp_live)
 					softmax_rows<D, KVT>(tS, tO, sm.key_ok[(kf + j) & 7], sl2, !first, m_ref,
 							     l_sum, &sm.p_half[t]);
