@@ -359,3 +359,18 @@ def test_scales_of_zero_and_below(be, kv, scale):
         want = case.want()[0]
         assert_contract(decode_of(be, case, dev, scale), want, "decode")
         assert_contract(dev.run(be), want, (hq, hkv, n, p))
+
+
+@pytest.mark.parametrize("kv", [MX, BF16])
+def test_rows_that_hold_the_whole_pages_only(be, kv):
+    """A row of 192 to 199 tokens does not hold a prefix of 200, so its pages
+    are its own, the first row's among them."""
+    case = pc.PrefixCase(cfg(kv), [(200, [195, 260, 192, 200, 199, 300])], loose=[195, 192, 199])
+    for row, other in ((0, 6), (2, 7), (4, 8)):
+        case.slots[row] = case.slots[other]
+    dev = pc.OnDevice(case)
+    pc.assert_near(dev.run(be), case.want())
+    case = pc.PrefixCase(cfg(kv), [(200, [195, 199])], loose=[195, 199])     # and no row that does
+    case.slots[0], case.slots[1] = case.slots[2], case.slots[3]
+    dev = pc.OnDevice(case)
+    pc.assert_near(dev.run(be), case.want())

@@ -232,11 +232,13 @@ plan_kernel(const kllm_prefix_args a)
 				const int b = a.group_starts[lo], e = a.group_starts[lo + 1];
 				if (b <= s && s < e && e - b >= a.min_share) {
 					P = prefix_tokens(a, lo);
-					if (P > 0 && L >= P) {
+					// A row without the whole prefix may have pages of its own, the
+					// prefix's whole pages included: all of it is suffix.
+					if (P > 0 && L >= a.prefix_lens[lo]) {
 						g = lo;
 						atomicMin(&sm.leader[lo], s);
 					} else {
-						P = 0;          // too short a row: all of it is suffix
+						P = 0;
 					}
 				}
 			}
