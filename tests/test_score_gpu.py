@@ -266,3 +266,39 @@ def test_the_likeliest_token_stays_at_or_below_zero(be):
     want = sc.rows(logits, np.full(R, 1e-3, np.float32), best, 3)
     sc.assert_near(got["logprob"], want["logprob"],
                    err[:, None] / 1e-3 + sc.distance_bound(want["entropy"], 0.0, V)[:, None], "best")
+
+
+def test_contexts_in_threads_with_joins_of_different_sizes(be):
+    """Two contexts on one GPU, each in a thread of its own: many ranges with 32
+    alternatives (43 KB of the join's shared memory) and few without (a call's
+    size must not become the other's limit)."""
+    import threading
+
+    import torch
+    other = kb.Backend()
+    cases = [(be, 128256, 32), (other, 200, 0)]
+    rcs = [[], []]
+
+    def calls(which):
+        b, V, top = cases[which]
+        h = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
+        w = torch.zeros((V, 64), dtype=torch.bfloat16, device="cuda")
+        f = torch.zeros((4, 32), device="cuda")
+        i = torch.zeros((4, 32), dtype=torch.int32, device="cuda")
+        nb = b.score_workspace_size(4, V, 0, top)
+        ws = torch.empty(nb, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        for _ in range(400):
+            rcs[which].append(b.score_tokens(
+                hidden=h.data_ptr(), weight=w.data_ptr(), num_rows=4, hidden_dim=64, vocab=V,
+                lse=f.data_ptr(), top_n=top, top_ids=i.data_ptr(), top_logprobs=f.data_ptr(),
+                workspace=ws.data_ptr(), workspace_bytes=nb))
+        torch.cuda.synchronize()
+
+    threads = [threading.Thread(target=calls, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    other.close()
+    assert rcs == [[0] * 400, [0] * 400]

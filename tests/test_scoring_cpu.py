@@ -91,3 +91,15 @@ def test_definition_of_the_layout():
     assert got["slot_map"].tolist() == [80, 81, 96, -1, -1]
     assert got["table"][2, 0].tolist() == [1000, 1500, 1]     # the parent's block
     assert got["counts"].tolist() == [3, 2] and got["err"] == 0
+
+
+def test_the_joins_shared_memory_is_no_function_attribute():
+    """An attribute is the function's for every context and thread of a device: a
+    size that changes from call to call would limit another thread's launch."""
+    src = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(kb.__file__))), "csrc",
+                       "score.cu")
+    with open(src) as f:
+        text = f.read()
+    calls = text.split("cudaFuncSetAttribute(")[1:]
+    assert len(calls) == 1 and calls[0].startswith("score_kernel,")
+    assert "static_assert(join_smem(kMaxSplits, KLLM_MAX_TOP_N_I) + 1024 <= 48 * 1024" in text

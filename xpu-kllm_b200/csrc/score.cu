@@ -500,6 +500,15 @@ score_kernel(const kllm_score_args a, const __grid_constant__ CUtensorMap tm_h,
 // ---- joining the ranges ---------------------------------------------------------
 
 constexpr int kJoinThreads = 128;
+// The join's candidates of a row: its shared memory grows with the ranges and
+// stays within what a launch may have without an attribute, which is the
+// function's for all callers of a device and so cannot follow one call's size.
+constexpr int kMaxSplits = 160;
+constexpr size_t join_smem(int splits, int top_n)
+{
+	return (size_t)splits * ((size_t)(top_n + kSlack) * 8 + 4);
+}
+static_assert(join_smem(kMaxSplits, KLLM_MAX_TOP_N_I) + 1024 <= 48 * 1024, "join's shared memory");
 
 __device__ __forceinline__ float dot8(uint4 x, uint4 y, float acc)
 {
@@ -681,6 +690,8 @@ extern "C" void kllm_score_plan(int num_rows, int vocab, int num_sms, struct kll
 	int q = num_sms / a->group_rb;
 	if (q < 1)
 		q = 1;
+	if (q > kMaxSplits)
+		q = kMaxSplits;
 	if (q > a->units)
 		q = a->units;
 	a->splits = q;
@@ -714,15 +725,11 @@ extern "C" int kllm_score_launch(struct kllm_score_args *a, void *workspace, voi
 	e = cudaGetLastError();
 	if (e != cudaSuccess)
 		return (int)e;
-	const size_t js = (size_t)a->splits * ((size_t)(a->top_n + kSlack) * 8 + 4);
-	e = cudaFuncSetAttribute(score_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)js);
-	if (e != cudaSuccess)
-		return (int)e;
 	// starts as the ranges' CTAs leave, with the targets' logits, which need none of them
 	cudaLaunchConfig_t cfg = {};
 	cfg.gridDim = dim3((unsigned)a->num_rows);
 	cfg.blockDim = dim3(kJoinThreads);
-	cfg.dynamicSmemBytes = js;
+	cfg.dynamicSmemBytes = join_smem(a->splits, a->top_n);
 	cfg.stream = st;
 	cudaLaunchAttribute at[1];
 	at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
