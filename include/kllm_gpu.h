@@ -606,7 +606,9 @@ void kllm_gpu_p2p_destroy(struct kllm_gpu_ctx *ctx);
  * itself in the same call; otherwise the row is laid out empty. That, a
  * free list that runs out, a slot outside [0, total_slots) (both leave a zero
  * entry) and more tokens than token_capacity are flagged with
- * KLLM_ERR_LAYOUT. num_seqs <= 4096. */
+ * KLLM_ERR_LAYOUT. num_seqs <= 4096. seq_lens may be ctx_lens or new_lens itself
+ * (lengths kept in place from step to step); no other output may overlap an
+ * input. */
 #define KLLM_ERR_LAYOUT         0x80u
 
 struct kllm_gpu_batch_layout_params {

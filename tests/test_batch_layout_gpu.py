@@ -186,3 +186,42 @@ def test_refusals(be):
         assert be.batch_layout(**{**ok, **change}) == code, change
     short = kb.BatchLayoutParams(struct_size=8)
     assert be.lib.kllm_gpu_batch_layout(be.ctx, ctypes.byref(short)) == kb.EINVAL
+
+
+@pytest.mark.parametrize("S,mb,max_new,fork", [(4096, 8, 3, 5), (700, 40, 200, 3), (9, 20, 1, 0)])
+@pytest.mark.parametrize("place", ["ctx", "new"])
+def test_lengths_in_place(be, S, mb, max_new, fork, place):
+    """seq_lens written over the lengths that the call reads: parents' lengths
+    among them, with more token rows than one CTA would take."""
+    import torch
+    rng = np.random.default_rng(S + len(place))
+    ctx, new, fk, table, free, total = make(rng, S, mb, 16, max_new, fork)
+    capacity = int(new.sum()) + 5
+    want = sc.layout(ctx, new, fk if fork else None, free, table.copy(), block=16, base=BASE,
+                     slot_bytes=SLOT, total=total, k_off=KO, v_off=VO, capacity=capacity)
+    up = lambda a: torch.from_numpy(np.asarray(a, np.int32)).cuda()  # noqa: E731
+    d = dict(ctx=up(ctx), new=up(new), fork=up(fk), free=up(free))
+    for shift in (0, 3):                     # the array itself, or one that begins inside it
+        both = torch.zeros(S + shift, dtype=torch.int32, device="cuda")
+        both[:S] = d[place]
+        src = dict(d, **{place: both})
+        lens = both[shift:]
+        tb = torch.from_numpy(table.copy()).cuda()
+        i = lambda n: torch.full((n,), -99, dtype=torch.int32, device="cuda")  # noqa: E731
+        cu, ts, tp, cn, err = i(S + 1), i(capacity), i(capacity), i(2), i(1)
+        err.zero_()
+        sm = torch.zeros(capacity, dtype=torch.int64, device="cuda")
+        assert be.batch_layout(
+            ctx_lens=src["ctx"].data_ptr(), new_lens=src["new"].data_ptr(),
+            fork_from=d["fork"].data_ptr() if fork else None, free_slots=d["free"].data_ptr(),
+            num_free=len(free), num_seqs=S, max_blocks_per_seq=mb, block_size=16, arena_base=BASE,
+            slot_bytes=SLOT, total_slots=total, k_offset=KO, v_offset=VO,
+            block_tables=tb.data_ptr(), seq_lens=lens.data_ptr(), cu_seqlens=cu.data_ptr(),
+            token_seq=ts.data_ptr(), token_pos=tp.data_ptr(), slot_map=sm.data_ptr(),
+            token_capacity=capacity, counts=cn.data_ptr(), err_word=err.data_ptr(),
+            stream=torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        got = dict(table=tb, seq_lens=lens, cu=cu, token_seq=ts, token_pos=tp, slot_map=sm, counts=cn)
+        for k, v in got.items():
+            assert np.array_equal(v.cpu().numpy(), want[k]), (k, shift)
+        assert int(err.item()) == want["err"] == 0
