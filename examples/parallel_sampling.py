@@ -71,6 +71,12 @@ def _ok(rc):
         raise RuntimeError(f"kllm_gpu call returned {rc}")
 
 
+def _stream():
+    """torch's current stream. Its default stream has the handle 0, which the
+    library takes for its context's own stream; 1 names the default one."""
+    return torch.cuda.current_stream().cuda_stream or 1
+
+
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 
@@ -91,7 +97,7 @@ class Cache:
         self.lens = torch.zeros(rows, **i32)
         self.cu = torch.zeros(rows + 1, **i32)
         self.err = torch.zeros(1, **i32)
-        self.stream = torch.cuda.current_stream().cuda_stream
+        self.stream = _stream()
 
     def layout(self, ctx, new, forks=None):
         """Pages for `new` more tokens of each row; the token rows' sequence and
@@ -132,7 +138,7 @@ def sample(be, model, prompts, samples, steps, temperature=0.8, top_n=5, block=1
     """`samples` continuations of `steps` tokens of each prompt (lists of token
     ids). Returns the prompts' log-probabilities, the tokens and their scores;
     with a list as `trace`, the queries and attentions of each step go there."""
-    P, R, stream = len(prompts), len(prompts) * samples, torch.cuda.current_stream().cuda_stream
+    P, R, stream = len(prompts), len(prompts) * samples, _stream()
     length = [len(p) for p in prompts]
     whole = [n // block * block for n in length]
     slots = sum(-(-n // block) for n in length) + R * (-(-steps // block) + 2) + 8

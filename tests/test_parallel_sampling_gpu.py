@@ -122,3 +122,18 @@ def test_forks_share_the_prompts_pages(be, ps):
     assert (t[1:, :4] == t[0, :4]).all()                      # 64 of 70 tokens
     assert len({int(x) for x in t[:, 4, 0]}) == 4             # then a page each
     assert r["cache"].lens.tolist() == [70, 72, 72, 72]
+
+
+def test_on_the_default_stream_and_on_a_side_stream(be, ps):
+    """The calls run where torch's tensors are made: the same samples and scores
+    whatever the current stream is."""
+    import torch
+    model = ps.Model(vocab=600)
+    prompts = [list(range(100)), list(range(200, 230))]
+    want = ps.sample(be, model, prompts, 4, 5, kv=kb.KV_BF16)
+    for stream in (torch.cuda.default_stream(), torch.cuda.Stream()):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            got = ps.sample(be, model, prompts, 4, 5, kv=kb.KV_BF16)
+        for k in ("tokens", "logprob", "rank", "entropy", "top_ids"):
+            assert torch.equal(got[k], want[k]), (k, stream)
