@@ -24,7 +24,10 @@
 // the end those that reach the k-th largest of 32 group maxima among them are
 // ordered by counting the better ones. When too many are collected (long runs
 // of equal logits, masks of the type's lowest value) the row is read again with
-// the last tau, and selected exactly by radix if that is too many as well.
+// the last tau, and selected exactly by radix if that is too many as well: by one
+// CTA, one after another, and slow (one row of 128,256 fp32 logits with seven
+// tokens allowed under a finite mask 475 us, 256 such rows 970 us; 999 bf16 rows of
+// 32,003 440 us; masks of -inf take no longer than none).
 // (Segment maxima in the pass and a second look at the best segments took 9 us
 // of 37 on 256 rows of 128,256: the second look waits behind other rows' loads.)
 //
@@ -32,10 +35,14 @@
 // rows still cover the GPU; the CTAs share maxima, sums and candidates through
 // distributed shared memory, so no workspace and no atomic on global memory is
 // needed and the result does not depend on the order in which CTAs finish.
-// Floor: HBM, each logit read once; bound: instruction issue (15 to 20 an element
-// with ranks and alternatives; without them the same pass runs at 5.2 TB/s).
-// Measured: 256 fp32 rows of 128,256 with a target and 20 alternatives 34 us,
-// 3.9 TB/s; 999 bf16 rows of 32,003 with three targets 35 us, 1.8 TB/s.
+// Floor: HBM, each logit read once. No unit is full: a scheduler issues in 49 % (256
+// fp32 rows of 128,256) or 58 % (999 bf16 rows of 32,003) of its cycles, with 15 to
+// 20 instructions an element for ranks and alternatives (without them the same pass
+// runs at 5.2 TB/s). Of the 12.7 (10.0) cycles between two instructions of a warp it
+// waits 3.8 (2.0) for loads, as a batch is used up before the next is loaded, 2.1
+// (2.0) for the instruction before and 2.0 (1.1) at barriers, mostly a row's end.
+// Measured, with a target and 20 alternatives (three targets and five): 34 us, 3.9
+// TB/s (35 us, 1.8 TB/s).
 
 #include "kllm_device.cuh"
 #include "kllm_internal.h"
@@ -363,7 +370,7 @@ logprobs_kernel(const kllm_logprobs_args a)
 	const float inv_t = temp > 0.f ? fminf(1.f / temp, FLT_MAX) : 1.f;
 	const float c = fminf(kLog2e * inv_t, FLT_MAX);
 
-	// ---- one pass: this thread's (m, S, W), ranks, segment maxima --------------
+	// ---- one pass: this thread's (m, S, W), ranks, group maxima, candidates ----
 	// A batch at a time: one maximum, one look at the reference and one at each
 	// target's place for its 32 elements (a vector at a time these took 35
 	// instructions an element, and the pass was bound by them). Its loads are in
