@@ -302,3 +302,40 @@ def test_contexts_in_threads_with_joins_of_different_sizes(be):
         t.join()
     other.close()
     assert rcs == [[0] * 400, [0] * 400]
+
+
+def test_as_many_rows_as_a_call_takes(be):
+    """2^20 rows: 512 groups of row blocks, offsets of the ranges' lists past 2^28
+    bytes; checked on the GPU in 64 bits."""
+    import torch
+    R, K, V = 1 << 20, 64, 130
+    gen = torch.Generator("cuda").manual_seed(3)
+    h = (torch.randn((R, K), generator=gen, device="cuda") * 8).round().clamp(-32, 32) / 4
+    w = (torch.randn((V, K), generator=gen, device="cuda") * 40).round().clamp(-127, 127) / 512
+    h, w = h.bfloat16(), w.bfloat16()
+    tgt = torch.randint(0, V, (R, 1), generator=gen, device="cuda", dtype=torch.int32)
+    f = lambda *s: torch.full(s, 7.5, device="cuda")  # noqa: E731
+    lp, lse, top = f(R, 1), f(R), f(R, 20)
+    ids = torch.full((R, 20), -77, dtype=torch.int32, device="cuda")
+    nb = be.score_workspace_size(R, V, 1, 20)
+    ws = torch.full((nb + 64,), 0xA5, dtype=torch.uint8, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert be.score_tokens(hidden=h.data_ptr(), weight=w.data_ptr(), num_rows=R, hidden_dim=K,
+                           vocab=V, num_targets=1, targets=tgt.data_ptr(),
+                           target_logprobs=lp.data_ptr(), lse=lse.data_ptr(), top_n=20,
+                           top_ids=ids.data_ptr(), top_logprobs=top.data_ptr(),
+                           workspace=ws.data_ptr(), workspace_bytes=nb, err_word=err.data_ptr(),
+                           stream=torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0 and (ws[nb:] == 0xA5).all()
+    for a in range(0, R, 1 << 17):
+        b = a + (1 << 17)
+        x = h[a:b].double() @ w.double().t()
+        want = x.logsumexp(1)
+        # |z| + ln V below 200: distance_bound and the rounding of lse at its size
+        tol = sc.distance_bound(np.log(V), 200.0, V) + 4 * sc.EPS * 200.0
+        assert ((lse[a:b].double() - want).abs() <= tol).all()
+        assert ((lp[a:b].double() - (x.gather(1, tgt[a:b].long()) - want[:, None])).abs() <= tol).all()
+        v, i = torch.sort(x, dim=1, descending=True, stable=True)
+        assert torch.equal(ids[a:b].long(), i[:, :20])
+        assert ((top[a:b].double() - (v[:, :20] - want[:, None])).abs() <= tol).all()
